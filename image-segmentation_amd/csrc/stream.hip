@@ -968,7 +968,12 @@ __global__ __launch_bounds__(kThreads) void upsample_fwd_half_kernel(const T* __
             float o[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                float val = wy0 * (wx0 * a[dy][dx][j] + wx1 * a[dy][dx + 1][j]) + wy1 * (wx0 * a[dy + 1][dx][j] + wx1 * a[dy + 1][dx + 1][j]);
+                // roundings fixed (a value next to zero passes the ReLU or not by its last bit): along x the product with 3/4 is
+                // rounded and the one with 1/4, which is exact, fused, whatever the compiler would contract
+                const float top = dx ? fmaf(wx1, a[dy][dx + 1][j], wx0 * a[dy][dx][j]) : fmaf(wx0, a[dy][dx][j], wx1 * a[dy][dx + 1][j]);
+                const float bottom = dx ? fmaf(wx1, a[dy + 1][dx + 1][j], wx0 * a[dy + 1][dx][j])
+                                        : fmaf(wx0, a[dy + 1][dx][j], wx1 * a[dy + 1][dx + 1][j]);
+                float val = fmaf(wy0, top, wy1 * bottom);
                 if (stats) val = (val - mean[j]) * rstd[j];
                 o[j] = relu ? fmaxf(val, 0.f) : val;
             }
