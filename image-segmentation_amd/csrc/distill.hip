@@ -1,0 +1,999 @@
+// Distillation from a teacher's top logits: the k greatest logits of every position (with the logsumexp of all of them), and the
+// loss between those and a student's logits with its gradient.
+//
+// For a position with student logits s over C classes, kept teacher logits t_j at classes i_j and temperature T:
+//     q   = softmax(s / T) over all classes
+//     p_j = softmax over the kept t_j / T                (no teacher logsumexp given),   r = 0
+//     p_j = exp(t_j / T - lse), r = 1 - sum_j p_j        (logsumexp of the teacher given: r is what it gave to the other classes)
+//     loss = T^2 [ sum_j p_j (log p_j - log q_{i_j}) + r (log r - log R) ],   R = sum of q over the classes that were not kept
+//     d loss / d s_c = T [ M q_c - p_c - [c not kept] r q_c / R ],            M = sum_j p_j + r,  p_c = sum of the p_j with i_j = c
+// All sums run over exp2((s - max) log2(e) / T) in fp32, the difference first: a mask of the type's lowest value times log2(e) would
+// overflow.  The classes outside the kept ones have a maximum and a sum of their own
+// (K_out, S_out): R and q_c / R then never come out of a difference of two almost equal sums, and cannot underflow.
+#include "common.h"
+
+namespace segk {
+
+constexpr int kTopMax = 64;               // kept logits of a position: one lane each
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+// A rest 1 - sum p of up to 2^-20 is rounding of at most 64 fp32 terms and of the logsumexp, not mass: it counts as none.
+constexpr float kRestFloor = 0x1p-20f;
+constexpr int kCountBlocks = 256;         // partial counts that the main kernels add up
+
+struct DistillArgs {
+    const void* z;             // student logits
+    int64_t ld;                // elements from one row / image to the next
+    int64_t s_c, s_p;          // elements from class to class and from position to position (thread-per-position kernel)
+    int64_t inner;             // positions of an image
+    int V;                     // classes
+    int k;
+    const void* t;             // kept teacher logits
+    const void* idx;           // their classes
+    const float* tlse;         // the teacher's logsumexp, or none
+    int64_t ts_c, ts_p;        // strides of t and idx
+    int t_bf16, idx64;
+    float T, invT, weight;
+    const float* upstream;     // gradient that reaches the loss: none (1), one value, or one for each position
+    int up_each, skip_if_one;
+    const int* counts;         // partial counts of the positions with a kept logit (mean), or none (sum)
+    float* row_loss;           // loss of each position
+    float* partial;            // sums that the finalize kernel adds (thread-per-position kernel)
+    void* dz;
+    int64_t ld_d, d_c, d_p;
+};
+
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+__device__ __forceinline__ int wave_sum_i(int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+// the class of a kept logit; -1 where it is none of [0, V): such an entry does not exist
+__device__ __forceinline__ int load_class(const DistillArgs& a, int64_t at) {
+    const int64_t i = a.idx64 ? static_cast<const int64_t*>(a.idx)[at] : (int64_t) static_cast<const int32_t*>(a.idx)[at];
+    return i >= 0 && i < a.V ? (int)i : -1;
+}
+__device__ __forceinline__ float load_kept(const DistillArgs& a, int64_t at) {
+    return a.t_bf16 ? (float)static_cast<const bf16*>(a.t)[at] : static_cast<const float*>(a.t)[at];
+}
+// the sum of the partial counts, at least 1; every lane of the wave has to call it
+__device__ __forceinline__ int count_of(const int* __restrict__ counts) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kCountBlocks / 64; ++i) n += counts[i * 64 + (threadIdx.x & 63)];
+    n = wave_sum_i(n);
+    return n > 0 ? n : 1;
+}
+// what multiplies T * (M q - p ...) of a position; every lane of the wave has to call it
+__device__ __forceinline__ float grad_scale(const DistillArgs& a, int64_t position) {
+    float g = a.weight * a.T;
+    if (a.counts) g /= (float)count_of(a.counts);
+    if (a.upstream) g *= a.upstream[a.up_each ? position : 0];
+    return g;
+}
+// exp of a logit over a base; c = log2(e) / T
+__device__ __forceinline__ float exp_over(float z, float base, float c) { return fast_exp2((z - base) * c); }
+// the same for a maximum that may be "no element" (-inf), whatever the base
+__device__ __forceinline__ float rebase(float k, float base, float c) { return k == -INFINITY ? 0.f : exp_over(k, base, c); }
+
+// ------------------------------------------------------------------------------------------------ rows in registers
+// A row is read in 16-byte pieces that are aligned in memory; the row may begin and end inside a piece.
+template <typename T> struct Piece {
+    static constexpr int VEC = 16 / (int)sizeof(T);
+    uint32_t w[4];
+    __device__ __forceinline__ float get(int v) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[v]);
+        else return __uint_as_float((v & 1) ? (w[v >> 1] & 0xFFFF0000u) : (w[v >> 1] << 16));
+    }
+    __device__ __forceinline__ void clear(int v) {      // element v <- -inf
+        if constexpr (sizeof(T) == 4) w[v] = 0xFF800000u;
+        else w[v >> 1] = (v & 1) ? ((w[v >> 1] & 0x0000FFFFu) | 0xFF800000u) : ((w[v >> 1] & 0xFFFF0000u) | 0x0000FF80u);
+    }
+};
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// Between two passes over packed pieces: makes the compiler unpack them again instead of keeping every element as a float of its
+// own from the first pass on (twice the registers, and spills in the tiers with 16 pieces).
+template <typename T, int N> __device__ __forceinline__ void stay_packed(Piece<T> (&x)[N]) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) asm volatile("" : "+v"(x[i].w[w]));
+    }
+}
+
+template <typename T> struct Row {
+    const T* p;      // element 0
+    int phase, V, pieces;
+    __device__ __forceinline__ Row(const T* row, int V_) : p(row), V(V_) {
+        constexpr int VEC = Piece<T>::VEC;
+        phase = (int)((reinterpret_cast<uintptr_t>(row) / sizeof(T)) % VEC);
+        pieces = (int)(((int64_t)V + phase + VEC - 1) / VEC);
+    }
+    // piece g: elements [g*VEC - phase, +VEC); what lies outside the row reads as -inf
+    __device__ __forceinline__ Piece<T> load(int g) const {
+        constexpr int VEC = Piece<T>::VEC;
+        Piece<T> r;
+        const int e0 = g * VEC - phase;
+        if (e0 >= 0 && e0 <= V - VEC) {
+            const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p + e0));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r.w[i] = x[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r.w[i] = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                const int e = e0 + v;
+                if (e >= 0 && e < V) {
+                    if constexpr (sizeof(T) == 4) r.w[v] = reinterpret_cast<const uint32_t*>(p)[e];
+                    else {
+                        const uint32_t h = reinterpret_cast<const uint16_t*>(p)[e];
+                        r.w[v >> 1] = (v & 1) ? ((r.w[v >> 1] & 0x0000FFFFu) | (h << 16)) : ((r.w[v >> 1] & 0xFFFF0000u) | h);
+                    }
+                }
+            }
+        }
+        return r;
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ void store_piece(T* dst, bool vec_ok, int e0, int V, const float (&f)[Piece<T>::VEC]) {
+    constexpr int VEC = Piece<T>::VEC;
+    if (vec_ok && e0 >= 0 && e0 <= V - VEC) {
+        if constexpr (sizeof(T) == 4) {
+            __builtin_nontemporal_store(f32x4{f[0], f[1], f[2], f[3]}, reinterpret_cast<f32x4*>(dst + e0));
+        } else {
+            bf16x8 o;
+#pragma unroll
+            for (int v = 0; v < 8; ++v) o[v] = (bf16)f[v];
+            __builtin_nontemporal_store(o, reinterpret_cast<bf16x8*>(dst + e0));
+        }
+    } else {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v)
+            if (e0 + v >= 0 && e0 + v < V) dst[e0 + v] = Elem<T>::from_f(f[v]);
+    }
+}
+
+// Kept classes that lie in the 64 pieces from g0 on (one for each lane): f(lane has it, element in the piece, entry)
+template <int VEC, typename F>
+__device__ __forceinline__ void for_kept(int cls, int phase, int g0, int lane, F&& f) {
+    const int rel = cls + phase - g0 * VEC;
+    uint64_t in = __ballot(cls >= 0 && rel >= 0 && rel < 64 * VEC);
+    while (in) {
+        const int j = __builtin_ctzll(in);
+        in &= in - 1;
+        const int at = __builtin_amdgcn_readlane(rel, j);
+        f(lane == at / VEC, at % VEC, j);
+    }
+}
+
+// One workgroup per row; with NCH > 0 the row stays in registers (NCH pieces per thread), with NCH == 0 it is read twice.
+template <typename T, int NT, int NCH, bool GRAD>
+__global__ __launch_bounds__(NT) void distill_rows_kernel(const DistillArgs a) {
+    constexpr int VEC = Piece<T>::VEC, NW = NT / 64;
+    __shared__ float sh_k[NW], sh_s[NW], sh_p[kTopMax], sh_z[kTopMax], sh_x[6];
+    if (a.skip_if_one && a.upstream[0] == 1.f) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t row = blockIdx.x;
+    const float c = a.invT * kLog2e;
+    const Row<T> r(static_cast<const T*>(a.z) + row * a.ld, a.V);
+    T* dst = GRAD ? static_cast<T*>(a.dz) + row * a.ld_d : nullptr;
+    const bool vec_ok = GRAD && (reinterpret_cast<uintptr_t>(dst) / sizeof(T)) % VEC == (unsigned)r.phase;
+
+    const int cls = lane < a.k ? load_class(a, row * a.k + lane) : -1;
+    if (__ballot(cls >= 0) == 0) {                       // nothing was kept here: no loss, no gradient, the row is not read
+        if (threadIdx.x == 0) a.row_loss[row] = 0.f;
+        if constexpr (GRAD) {
+            const float zero[VEC] = {};
+            for (int g = threadIdx.x; g < r.pieces; g += NT) store_piece<T>(dst, vec_ok, g * VEC - r.phase, a.V, zero);
+        }
+        return;
+    }
+
+    Piece<T> x[NCH > 0 ? NCH : 1];
+    if constexpr (NCH > 0) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int g = i * NT + (int)threadIdx.x;
+            if (g < r.pieces) x[i] = r.load(g);
+            else
+#pragma unroll
+                for (int w = 0; w < 4; ++w) x[i].w[w] = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;
+        }
+    }
+
+    // ---- the kept entries, one for each lane of the first wave
+    float p = 0.f, lp = -INFINITY, zj = -INFINITY;
+    if (wave == 0) {
+        float t = -INFINITY;
+        if (cls >= 0) {
+            t = load_kept(a, row * a.k + lane);
+            zj = Elem<T>::to_f(r.p[cls]);
+        }
+        if (a.tlse) {
+            lp = cls >= 0 ? fmaf(t, a.invT, -a.tlse[row]) * kLog2e : -INFINITY;
+            p = cls >= 0 ? fast_exp2(lp) : 0.f;
+        } else {
+            const float top = wave_max(t);
+            const float e = cls >= 0 && top != -INFINITY ? fast_exp2((t - top) * c) : 0.f;
+            const float sum = wave_sum(e);
+            p = sum == 0.f ? 0.f : e / sum;
+            lp = (t - top) * c - log2f(sum);
+        }
+        const float mass = wave_sum(p);
+        float total = p;                                  // of all entries with this class
+        bool first = cls >= 0;
+        for (int j = 0; j < a.k; ++j) {
+            const int cj = __builtin_amdgcn_readlane(cls, j);
+            const float pj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), j));
+            if (cj == cls && j != lane) {
+                total += pj;
+                if (j < lane) first = false;
+            }
+        }
+        const int distinct = __popcll(__ballot(first));
+        float rest = a.tlse ? 1.f - mass : 0.f;
+        if (!(rest > kRestFloor) || distinct == a.V) rest = 0.f;
+        const float zm = wave_max(first ? zj : -INFINITY);
+        const float sm = wave_sum(first && zm != -INFINITY ? exp_over(zj, zm, c) : 0.f);
+        const float gs = GRAD ? grad_scale(a, row) : 0.f;
+        sh_p[lane] = total;
+        sh_z[lane] = zj;
+        if (lane == 0) { sh_x[0] = zm; sh_x[1] = sm; sh_x[2] = rest; sh_x[3] = mass + rest; sh_x[4] = gs; }
+    }
+
+    // ---- maximum and sum of the classes that were not kept
+    float kw = -INFINITY, sw = 0.f;
+    if constexpr (NCH > 0) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            for_kept<VEC>(cls, r.phase, i * NT + wave * 64, lane, [&](bool here, int v, int) {
+#pragma unroll
+                for (int u = 0; u < VEC; ++u)
+                    if (here && u == v) x[i].clear(u);
+            });
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) m = fmaxf(m, x[i].get(v));
+        }
+        m = wave_max(m);
+        const float base = m == -INFINITY ? 0.f : m;
+        stay_packed(x);
+#pragma unroll
+        for (int i = 0; i < NCH; ++i)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) sw += exp_over(x[i].get(v), base, c);
+        sw = wave_sum(sw);
+        kw = m;
+    } else {
+        float m = -INFINITY;                              // of this lane
+        for (int g0 = wave * 64; g0 < r.pieces; g0 += NT) {
+            const int g = g0 + lane;
+            Piece<T> y;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) y.w[w] = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;
+            if (g < r.pieces) y = r.load(g);
+            for_kept<VEC>(cls, r.phase, g0, lane, [&](bool here, int v, int) {
+#pragma unroll
+                for (int u = 0; u < VEC; ++u)
+                    if (here && u == v) y.clear(u);
+            });
+            float mg = y.get(0);
+#pragma unroll
+            for (int v = 1; v < VEC; ++v) mg = fmaxf(mg, y.get(v));
+            if (mg > m) {
+                sw *= rebase(m, mg, c);
+                m = mg;
+            }
+            const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) sw += exp_over(y.get(v), base, c);
+        }
+        kw = wave_max(m);
+        sw = wave_sum(m == -INFINITY ? sw : sw * exp_over(m, kw, c));      // sw of an empty lane is 0 (or NaN, which stays)
+    }
+    if (lane == 0) { sh_k[wave] = kw; sh_s[wave] = sw; }
+    __syncthreads();
+
+    float ko = sh_k[0];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) ko = fmaxf(ko, sh_k[w]);
+    float so = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) so += sh_k[w] == -INFINITY ? sh_s[w] : sh_s[w] * exp_over(sh_k[w], ko, c);
+    const float km = sh_x[0], rest = sh_x[2], mass = sh_x[3], gs = sh_x[4];
+    const float kk = fmaxf(ko, km);
+    const float fo = rebase(ko, kk, c);
+    const float s = so * fo + sh_x[1] * rebase(km, kk, c) + (so != so ? so : 0.f);      // a NaN among the logits reaches the row
+
+    if (wave == 0) {
+        const float ls = log2f(s);
+        float l = p == 0.f ? 0.f : p * (lp - ((zj - kk) * c - ls));
+        l = wave_sum(l);
+        if (rest > 0.f) l += rest * (log2f(rest) - (log2f(so) + (ko - kk) * c - ls));
+        if (lane == 0) a.row_loss[row] = l * (kLn2 * a.T * a.T * a.weight);
+    }
+    if constexpr (GRAD) {
+        const float inv = 1.f / s;
+        const float gj = lane < a.k ? gs * (mass * exp_over(sh_z[lane], kk, c) * inv - sh_p[lane]) : 0.f;
+        const float b = gs * (mass * fo * inv - (rest > 0.f ? rest / so : 0.f));
+        const float base = ko == -INFINITY ? 0.f : ko;
+        auto write = [&](const Piece<T>& y, int g0) {
+            float f[VEC];
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) f[v] = b * exp_over(y.get(v), base, c);
+            for_kept<VEC>(cls, r.phase, g0, lane, [&](bool here, int v, int j) {
+                const float gv = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(gj), j));
+#pragma unroll
+                for (int u = 0; u < VEC; ++u)
+                    if (here && u == v) f[u] = gv;
+            });
+            const int g = g0 + lane;
+            if (g < r.pieces) store_piece<T>(dst, vec_ok, g * VEC - r.phase, a.V, f);
+        };
+        if constexpr (NCH > 0) {
+            stay_packed(x);
+#pragma unroll
+            for (int i = 0; i < NCH; ++i) write(x[i], i * NT + wave * 64);
+        } else {
+            for (int g0 = wave * 64; g0 < r.pieces; g0 += NT) {
+                Piece<T> y;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) y.w[w] = 0;
+                if (g0 + lane < r.pieces) y = r.load(g0 + lane);
+                write(y, g0);
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ one thread per position
+// Few classes (up to 32), all of them in the registers of one thread, VP neighbouring positions per thread: the class planes of
+// [N, C, ...] logits are read with coalesced 16-byte loads (VP = 4), class-last rows with strided ones (VP = 1).
+template <typename T, int CM, int VP, bool GRAD>
+__global__ __launch_bounds__(256) void distill_pixels_kernel(const DistillArgs a, int blocks_each) {
+    if (a.skip_if_one && a.upstream[0] == 1.f) return;
+    __shared__ float red[4];
+    const int64_t o = blockIdx.x / blocks_each;
+    const int64_t i0 = ((int64_t)(blockIdx.x % blocks_each) * 256 + threadIdx.x) * VP;
+    const float c = a.invT * kLog2e;
+    const T* z = static_cast<const T*>(a.z) + o * a.ld;
+    const int64_t t0 = o * a.k * a.inner;
+    const float gs = GRAD && !a.up_each ? grad_scale(a, 0) : 0.f;
+    float block = 0.f;
+    if (i0 < a.inner) {
+        float x[CM][VP];
+#pragma unroll
+        for (int q = 0; q < CM; ++q) {
+            if (q < a.V) {
+                if constexpr (VP == 4) Elem<T>::load4(z + q * a.s_c + i0, x[q]);
+                else x[q][0] = Elem<T>::to_f(z[q * a.s_c + i0 * a.s_p]);
+            } else {
+#pragma unroll
+                for (int v = 0; v < VP; ++v) x[q][v] = -INFINITY;
+            }
+        }
+        float e[CM][VP], top[VP], sum[VP], plogp[VP], lse[VP];
+        uint32_t kept[VP];
+#pragma unroll
+        for (int v = 0; v < VP; ++v) {
+            top[v] = -INFINITY;
+            sum[v] = plogp[v] = 0.f;
+            kept[v] = 0;
+            lse[v] = a.tlse ? a.tlse[o * a.inner + i0 + v] : 0.f;
+#pragma unroll
+            for (int q = 0; q < CM; ++q) e[q][v] = 0.f;
+        }
+        for (int j = 0; j < a.k; ++j)
+#pragma unroll
+            for (int v = 0; v < VP; ++v) {
+                const int64_t at = t0 + j * a.ts_c + (i0 + v) * a.ts_p;
+                const int cj = load_class(a, at);
+                if (cj >= 0) {
+                    kept[v] |= 1u << cj;
+                    if (!a.tlse) top[v] = fmaxf(top[v], load_kept(a, at));
+                }
+            }
+        for (int j = 0; j < a.k; ++j)
+#pragma unroll
+            for (int v = 0; v < VP; ++v) {
+                const int64_t at = t0 + j * a.ts_c + (i0 + v) * a.ts_p;
+                const int cj = load_class(a, at);
+                if (cj < 0) continue;
+                const float t = load_kept(a, at);
+                const float lp = a.tlse ? fmaf(t, a.invT, -lse[v]) * kLog2e : (top[v] == -INFINITY ? -INFINITY : (t - top[v]) * c);
+                const float ej = fast_exp2(lp);
+                sum[v] += ej;
+                plogp[v] += ej == 0.f ? 0.f : ej * lp;
+#pragma unroll
+                for (int q = 0; q < CM; ++q) e[q][v] += q == cj ? ej : 0.f;
+            }
+#pragma unroll
+        for (int v = 0; v < VP; ++v) {
+            const int64_t pos = o * a.inner + i0 + v;
+            float l = 0.f, g = gs;
+            if constexpr (GRAD)
+                if (a.up_each) g = a.weight * a.T * a.upstream[pos];       // no mean goes with one gradient for each position
+            float mass = sum[v], rest = 0.f;
+            if (a.tlse) {
+                rest = 1.f - mass;
+                if (!(rest > kRestFloor) || __popc(kept[v]) == a.V) rest = 0.f;
+            } else {
+                const float inv = sum[v] == 0.f ? 0.f : 1.f / sum[v];
+#pragma unroll
+                for (int q = 0; q < CM; ++q) e[q][v] *= inv;
+                plogp[v] = sum[v] == 0.f ? 0.f : plogp[v] * inv - log2f(sum[v]);
+                mass = sum[v] * inv;
+            }
+            const float all = mass + rest;
+            float zo = -INFINITY, zm = -INFINITY;
+#pragma unroll
+            for (int q = 0; q < CM; ++q) {
+                const bool in = (kept[v] >> q) & 1u;
+                zo = fmaxf(zo, in ? -INFINITY : x[q][v]);
+                zm = fmaxf(zm, in ? x[q][v] : -INFINITY);
+            }
+            const float ko = zo, km = zm, kk = fmaxf(ko, km);
+            const float bo = ko == -INFINITY ? 0.f : ko, bm = km == -INFINITY ? 0.f : km;
+            float so = 0.f, sm = 0.f, w[CM];
+#pragma unroll
+            for (int q = 0; q < CM; ++q) {
+                const bool in = (kept[v] >> q) & 1u;
+                w[q] = exp_over(x[q][v], in ? bm : bo, c);
+                so += in ? 0.f : w[q];
+                sm += in ? w[q] : 0.f;
+            }
+            const float fo = rebase(ko, kk, c), fm = rebase(km, kk, c);
+            const float s = so * fo + sm * fm + (so != so ? so : 0.f);
+            if (kept[v]) {
+                const float ls = log2f(s);
+                l = plogp[v];
+#pragma unroll
+                for (int q = 0; q < CM; ++q) l -= e[q][v] == 0.f ? 0.f : e[q][v] * ((x[q][v] - kk) * c - ls);
+                if (rest > 0.f) l += rest * (log2f(rest) - (log2f(so) + (ko - kk) * c - ls));
+                l *= kLn2 * a.T * a.T * a.weight;
+            }
+            if (a.row_loss) a.row_loss[pos] = l;
+            block += l;
+            if constexpr (GRAD) {
+                const float inv = 1.f / s;
+                const float fk = g * all * fm * inv, fr = g * (all * fo * inv - (rest > 0.f ? rest / so : 0.f));
+#pragma unroll
+                for (int q = 0; q < CM; ++q)
+                    x[q][v] = !kept[v] ? 0.f : ((kept[v] >> q) & 1u) ? w[q] * fk - g * e[q][v] : w[q] * fr;
+            }
+        }
+        if constexpr (GRAD) {
+            T* d = static_cast<T*>(a.dz) + o * a.ld_d;
+#pragma unroll
+            for (int q = 0; q < CM; ++q)
+                if (q < a.V) {
+                    if constexpr (VP == 4) Elem<T>::store4(d + q * a.d_c + i0, x[q]);
+                    else d[q * a.d_c + i0 * a.d_p] = Elem<T>::from_f(x[q][0]);
+                }
+        }
+    }
+    if (a.partial) {
+        block = wave_sum(block);
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = block;
+        __syncthreads();
+        if (threadIdx.x == 0) a.partial[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+    }
+}
+
+// positions with at least one kept logit: one partial count for each workgroup
+__global__ __launch_bounds__(256) void distill_count_kernel(const DistillArgs a, int64_t positions, int* __restrict__ counts) {
+    if (a.skip_if_one && a.upstream[0] == 1.f) return;
+    __shared__ int red[4];
+    int n = 0;
+    for (int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x; p < positions; p += (int64_t)kCountBlocks * 256) {
+        const int64_t o = p / a.inner, i = p - o * a.inner;
+        int any = 0;
+        for (int j = 0; j < a.k && !any; ++j) any = load_class(a, o * a.k * a.inner + j * a.ts_c + i * a.ts_p) >= 0;
+        n += any;
+    }
+    n = wave_sum_i(n);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = n;
+    __syncthreads();
+    if (threadIdx.x == 0) counts[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+}
+
+__device__ __forceinline__ double block_sum_1024(double s, double* red) {
+    s = wave_sum_d(s);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    double t = 0.0;
+    if (threadIdx.x == 0)
+        for (int i = 0; i < 16; ++i) t += red[i];
+    return t;
+}
+// level 1 of the final sum (many positions): workgroup b adds its own range in double
+__global__ __launch_bounds__(1024) void distill_collect_kernel(const float* __restrict__ v, int64_t n, float* __restrict__ out) {
+    __shared__ double red[16];
+    const int64_t per = (n + gridDim.x - 1) / gridDim.x, lo = per * blockIdx.x, hi = lo + per < n ? lo + per : n;
+    double s = 0.0;
+    for (int64_t i = lo + threadIdx.x; i < hi; i += 1024) s += (double)v[i];
+    s = block_sum_1024(s, red);
+    if (threadIdx.x == 0) out[blockIdx.x] = (float)s;
+}
+__global__ __launch_bounds__(1024) void distill_finalize_kernel(const float* __restrict__ v, int n, const int* __restrict__ counts,
+                                                                float* __restrict__ loss) {
+    __shared__ double red[16];
+    const int m = counts ? count_of(counts) : 1;
+    double s = 0.0;
+    for (int i = threadIdx.x; i < n; i += 1024) s += (double)v[i];
+    s = block_sum_1024(s, red);
+    if (threadIdx.x == 0) loss[0] = (float)(s / (double)m);
+}
+
+// ------------------------------------------------------------------------------------------------ the k greatest of a row
+// A float as an integer that orders like it: NaN above everything, both zeros alike.
+__device__ __forceinline__ uint32_t order_key(float f) {
+    const uint32_t b = __float_as_uint(f + 0.f);
+    if ((b & 0x7FFFFFFFu) > 0x7F800000u) return 0xFFFFFFFFu;
+    return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+
+constexpr int kCandidates = 1024;
+
+// Selection in three steps.  (1) Every thread takes the maximum of its part of the row (and the row's logsumexp is formed).
+// (2) The first wave finds a value that at least k of these maxima reach, by a binary search over the bits with ballots: at least
+// k elements of the row reach it, and hardly more than k in unordered data.  (3) The elements that reach it are collected in LDS
+// and ranked by counting; ties go to the lower index.  Where more than kCandidates reach it (many ties) or a NaN is in the row,
+// the exact k-th key and then the last index that still belongs are found by binary searches over the whole row.
+template <typename T, int NT, int NCH>
+__global__ __launch_bounds__(NT) void top_rows_kernel(const T* __restrict__ z, int64_t ld, int V, int k, float invT, T* __restrict__ values,
+                                                      int32_t* __restrict__ indices, float* __restrict__ lse) {
+    constexpr int VEC = Piece<T>::VEC, NW = NT / 64;
+    __shared__ float sh_m[NT], sh_k[NW], sh_s[NW];
+    __shared__ uint32_t ck[kCandidates];
+    __shared__ int ci[kCandidates], sh_n[NW], sh_count, sh_slow;
+    __shared__ uint32_t sh_bound;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t row = blockIdx.x;
+    const float c = invT * kLog2e;
+    const Row<T> r(z + row * ld, V);
+    Piece<T> x[NCH > 0 ? NCH : 1];
+    float m = -INFINITY, sw = 0.f, kw;
+    if constexpr (NCH > 0) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int g = i * NT + (int)threadIdx.x;
+            if (g < r.pieces) x[i] = r.load(g);
+            else
+#pragma unroll
+                for (int w = 0; w < 4; ++w) x[i].w[w] = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;
+        }
+#pragma unroll
+        for (int i = 0; i < NCH; ++i)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) m = fmaxf(m, x[i].get(v));
+        const float mw = wave_max(m);
+        kw = mw;
+        const float base = mw == -INFINITY ? 0.f : mw;
+        stay_packed(x);
+#pragma unroll
+        for (int i = 0; i < NCH; ++i)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) sw += exp_over(x[i].get(v), base, c);
+        sw = wave_sum(sw);
+    } else {
+        for (int g = threadIdx.x; g < r.pieces; g += NT) {
+            const Piece<T> y = r.load(g);
+            float mg = y.get(0);
+#pragma unroll
+            for (int v = 1; v < VEC; ++v) mg = fmaxf(mg, y.get(v));
+            if (mg > m) {
+                sw *= rebase(m, mg, c);
+                m = mg;
+            }
+            const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) sw += exp_over(y.get(v), base, c);
+        }
+        kw = wave_max(m);
+        sw = wave_sum(m == -INFINITY ? sw : sw * exp_over(m, kw, c));
+    }
+    sh_m[threadIdx.x] = m;
+    if (lane == 0) { sh_k[wave] = kw; sh_s[wave] = sw; }
+    if (threadIdx.x == 0) sh_count = 0;
+    __syncthreads();
+    if (wave == 0) {
+        float kk = sh_k[0], s = 0.f;
+#pragma unroll
+        for (int w = 1; w < NW; ++w) kk = fmaxf(kk, sh_k[w]);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) s += sh_k[w] == -INFINITY ? sh_s[w] : sh_s[w] * exp_over(sh_k[w], kk, c);
+        if (lane == 0 && lse) lse[row] = (kk == -INFINITY && s == 0.f) ? -INFINITY : kk * invT + log2f(s) * kLn2;
+        uint32_t key[NW];
+#pragma unroll
+        for (int w = 0; w < NW; ++w) key[w] = order_key(sh_m[w * 64 + lane]);
+        uint32_t bound = 0;
+        for (int bit = 31; bit >= (sizeof(T) == 2 ? 16 : 0); --bit) {
+            const uint32_t cand = bound | (1u << bit);
+            int n = 0;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) n += __popcll(__ballot(key[w] >= cand));
+            if (n >= k) {
+                bound = cand;
+                if (n <= k + (k >> 2) + 2) break;
+            }
+        }
+        if (lane == 0) {
+            sh_bound = bound;
+            sh_slow = s != s;
+        }
+    }
+    __syncthreads();
+
+    auto take = [&](uint32_t key, int e) {
+        const int at = atomicAdd(&sh_count, 1);
+        if (at < kCandidates) { ck[at] = key; ci[at] = e; }
+    };
+    auto each_in_memory = [&](auto&& f) {
+        for (int g = threadIdx.x; g < r.pieces; g += NT) {
+            const Piece<T> y = r.load(g);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                const int e = g * VEC - r.phase + v;
+                if (e >= 0 && e < V) f(y.get(v), e);
+            }
+        }
+    };
+    const uint32_t bound = sh_bound;
+    bool slow = sh_slow != 0;
+    if (!slow) {
+        // the bound as a float: keys of floats order as the floats do, so the elements are compared unconverted
+        const float fb = bound <= 0x007FFFFFu ? -INFINITY      // no key lies between 0 and that of -inf: everything belongs
+                                              : __uint_as_float((bound & 0x80000000u) ? bound & 0x7FFFFFFFu : ~bound);
+        if constexpr (NCH > 0) {
+            if (m >= fb) {
+                stay_packed(x);
+#pragma unroll
+                for (int i = 0; i < NCH; ++i) {
+                    uint32_t hit = 0;
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) hit |= x[i].get(v) >= fb ? 1u << v : 0u;
+                    const int e0 = (i * NT + (int)threadIdx.x) * VEC - r.phase;
+                    while (hit) {
+                        const int v = __builtin_ctz(hit);
+                        hit &= hit - 1;
+                        float f = x[i].get(0);
+#pragma unroll
+                        for (int u = 1; u < VEC; ++u) f = u == v ? x[i].get(u) : f;
+                        if (e0 + v >= 0 && e0 + v < V) take(order_key(f), e0 + v);
+                    }
+                }
+            }
+        } else {
+            if (m >= fb)
+                each_in_memory([&](float f, int e) {
+                    if (f >= fb) take(order_key(f), e);
+                });
+        }
+        __syncthreads();
+        slow = sh_count > kCandidates;
+    }
+    if (slow) {
+        auto count = [&](auto&& pred) {
+            int n = 0;
+            each_in_memory([&](float f, int e) { n += pred(order_key(f), e) ? 1 : 0; });
+            n = wave_sum_i(n);
+            __syncthreads();
+            if (lane == 0) sh_n[wave] = n;
+            __syncthreads();
+            int t = 0;
+            for (int w = 0; w < NW; ++w) t += sh_n[w];
+            return t;
+        };
+        uint32_t kth = 0;
+        for (int bit = 31; bit >= 0; --bit) {
+            const uint32_t cand = kth | (1u << bit);
+            if (count([&](uint32_t q, int) { return q >= cand; }) >= k) kth = cand;
+        }
+        const int need = k - count([&](uint32_t q, int) { return q > kth; });     // of the elements equal to the k-th
+        int last = 0;
+        for (int bit = 30; bit >= 0; --bit) {
+            const int cand = last | (1 << bit);
+            if (cand < V && count([&](uint32_t q, int e) { return q == kth && e < cand; }) < need) last = cand;
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) sh_count = 0;
+        __syncthreads();
+        each_in_memory([&](float f, int e) {
+            const uint32_t q = order_key(f);
+            if (q > kth || (q == kth && e <= last)) take(q, e);
+        });
+        __syncthreads();
+    }
+    const int n = sh_count < kCandidates ? sh_count : kCandidates;
+    for (int i = threadIdx.x; i < n; i += NT) {
+        const uint32_t q = ck[i];
+        const int e = ci[i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += (ck[j] > q || (ck[j] == q && ci[j] < e)) ? 1 : 0;
+        if (rank < k) {
+            indices[row * k + rank] = e;
+            values[row * k + rank] = r.p[e];
+        }
+    }
+}
+
+// elements widened to floats and written back with their bits as they were: a conversion may turn one NaN into another
+__device__ __forceinline__ float load_same(const float* p) { return *p; }
+__device__ __forceinline__ float load_same(const bf16* p) { return __uint_as_float((uint32_t) * reinterpret_cast<const uint16_t*>(p) << 16); }
+__device__ __forceinline__ void load_same4(const float* p, float (&v)[4]) { Elem<float>::load4(p, v); }
+__device__ __forceinline__ void load_same4(const bf16* p, float (&v)[4]) {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    v[0] = __uint_as_float(w.x << 16);
+    v[1] = __uint_as_float(w.x & 0xFFFF0000u);
+    v[2] = __uint_as_float(w.y << 16);
+    v[3] = __uint_as_float(w.y & 0xFFFF0000u);
+}
+__device__ __forceinline__ void store_same(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_same(bf16* p, float v) { *reinterpret_cast<uint16_t*>(p) = (uint16_t)(__float_as_uint(v) >> 16); }
+__device__ __forceinline__ void store_same4(float* p, const float (&v)[4]) { Elem<float>::store4(p, v); }
+__device__ __forceinline__ void store_same4(bf16* p, const float (&v)[4]) {
+    *reinterpret_cast<uint2*>(p) = make_uint2((__float_as_uint(v[0]) >> 16) | (__float_as_uint(v[1]) & 0xFFFF0000u),
+                                              (__float_as_uint(v[2]) >> 16) | (__float_as_uint(v[3]) & 0xFFFF0000u));
+}
+
+// one thread per position, up to 32 classes in its registers: k rounds of "greatest that is left"
+template <typename T, int CM, int VP>
+__global__ __launch_bounds__(256) void top_pixels_kernel(const T* __restrict__ z, int64_t ld, int64_t s_c, int64_t s_p, int64_t inner, int V,
+                                                         int k, float invT, T* __restrict__ values, int32_t* __restrict__ indices,
+                                                         int64_t ts_c, int64_t ts_p, float* __restrict__ lse, int blocks_each) {
+    const int64_t o = blockIdx.x / blocks_each;
+    const int64_t i0 = ((int64_t)(blockIdx.x % blocks_each) * 256 + threadIdx.x) * VP;
+    if (i0 >= inner) return;
+    const float c = invT * kLog2e;
+    z += o * ld;
+    float x[CM][VP];
+#pragma unroll
+    for (int q = 0; q < CM; ++q) {
+        if (q < V) {
+            if constexpr (VP == 4) load_same4(z + q * s_c + i0, x[q]);
+            else x[q][0] = load_same(z + q * s_c + i0 * s_p);
+        } else {
+#pragma unroll
+            for (int v = 0; v < VP; ++v) x[q][v] = -INFINITY;
+        }
+    }
+    uint32_t done[VP];
+    float out[VP];
+#pragma unroll
+    for (int v = 0; v < VP; ++v) {
+        done[v] = 0;
+        float m = -INFINITY, s = 0.f;
+#pragma unroll
+        for (int q = 0; q < CM; ++q) m = fmaxf(m, x[q][v]);
+        const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int q = 0; q < CM; ++q) s += exp_over(x[q][v], base, c);
+        out[v] = (m == -INFINITY && s == 0.f) ? -INFINITY : base * invT + log2f(s) * kLn2;
+    }
+    if (lse) {
+        if constexpr (VP == 4) Elem<float>::store4(lse + o * inner + i0, out);
+        else lse[o * inner + i0] = out[0];
+    }
+    const int64_t t0 = o * k * inner;
+    for (int j = 0; j < k; ++j) {
+        int at[VP];
+        float val[VP];
+#pragma unroll
+        for (int v = 0; v < VP; ++v) {
+            uint32_t best = 0;
+            at[v] = 0;
+            val[v] = x[0][v];
+            bool have = false;
+#pragma unroll
+            for (int q = 0; q < CM; ++q) {
+                const uint32_t key = order_key(x[q][v]);
+                const bool better = q < V && !((done[v] >> q) & 1u) && (!have || key > best);
+                best = better ? key : best;
+                at[v] = better ? q : at[v];
+                val[v] = better ? x[q][v] : val[v];
+                have = have || better;
+            }
+            done[v] |= 1u << at[v];
+        }
+        T* out_v = values + t0 + j * ts_c + i0 * ts_p;
+        int32_t* out_i = indices + t0 + j * ts_c + i0 * ts_p;
+        if constexpr (VP == 4) {
+            store_same4(out_v, val);
+            *reinterpret_cast<int4*>(out_i) = make_int4(at[0], at[1], at[2], at[3]);
+        } else {
+            store_same(out_v, val[0]);
+            *out_i = at[0];
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+constexpr int kPixelClasses = 32;    // more classes than this: one workgroup (or wave) per row
+
+// `rows` launches with the tier of a row of V classes: (threads, pieces in registers per thread)
+template <typename T, typename F> static void row_tier(int64_t V, F&& f) {
+    constexpr int VEC = 16 / (int)sizeof(T);
+    const int64_t pieces = (V + 2 * (VEC - 1)) / VEC;           // wherever the row begins
+#define SEGK_TIER(nt, nch) if (pieces <= (int64_t)(nt) * (nch)) return f(std::integral_constant<int, nt>{}, std::integral_constant<int, nch>{})
+    SEGK_TIER(64, 1);
+    SEGK_TIER(64, 2);
+    SEGK_TIER(64, 4);
+    SEGK_TIER(64, 8);
+    SEGK_TIER(256, 4);
+    SEGK_TIER(256, 8);
+    SEGK_TIER(256, 16);
+    SEGK_TIER(1024, 8);
+    SEGK_TIER(1024, 16);
+#undef SEGK_TIER
+    return f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 0>{});
+}
+
+static int check_logits(const char* who, const void* z, int dtype, int64_t outer, int64_t C, int64_t inner, int64_t ld, int64_t k,
+                        float temperature) {
+    SEGK_REQUIRE(z, SEGK_EINVAL, "%s: null pointer", who);
+    SEGK_REQUIRE(dtype == SEGK_F32 || dtype == SEGK_BF16, SEGK_EINVAL, "%s: unknown dtype %d", who, dtype);
+    SEGK_REQUIRE(outer > 0 && C > 0 && inner > 0 && outer < (1ll << 31) && C < (1ll << 30) && inner < (1ll << 40), SEGK_ESHAPE, "%s: bad shape", who);
+    SEGK_REQUIRE(outer <= (1ll << 40) / inner, SEGK_ESHAPE, "%s: too many positions", who);
+    SEGK_REQUIRE(inner == 1 || C <= kPixelClasses, SEGK_ESHAPE, "%s: more than %d classes have to be the innermost dimension", who, kPixelClasses);
+    SEGK_REQUIRE(ld >= C * inner, SEGK_ESHAPE, "%s: ld smaller than one row / image", who);
+    SEGK_REQUIRE(k >= 1 && k <= kTopMax && k <= C, SEGK_ESHAPE, "%s: k must be between 1 and %d and at most the number of classes", who, kTopMax);
+    SEGK_REQUIRE(temperature > 0.f && temperature < INFINITY, SEGK_EINVAL, "%s: temperature must be positive and finite", who);
+    SEGK_REQUIRE(reinterpret_cast<uintptr_t>(z) % esize(dtype) == 0, SEGK_EALIGN, "%s: logits are not aligned to their type", who);
+    return SEGK_OK;
+}
+
+// geometry of the thread-per-position kernels: rows of few classes count as the positions of one image, classes innermost
+struct Pixels {
+    int64_t outer, inner, s_c, s_p, ts_c, ts_p;
+    int vp, blocks_each;
+    int64_t blocks;
+};
+static Pixels pixels(int64_t outer, int64_t C, int64_t inner, int64_t ld, int64_t k, bool may_vec) {
+    Pixels p;
+    if (inner == 1) {
+        p = {1, outer, 1, ld, 1, k, 1, 0, 0};
+    } else {
+        p = {outer, inner, inner, 1, inner, 1, 1, 0, 0};
+        if (may_vec && C <= 8 && inner % 4 == 0 && ld % 4 == 0) p.vp = 4;
+    }
+    p.blocks_each = (int)((p.inner + 256 * p.vp - 1) / (256 * p.vp));
+    p.blocks = p.outer * p.blocks_each;
+    return p;
+}
+static bool few(int64_t C, int64_t inner) { return C <= kPixelClasses && (inner > 1 || C <= 8); }
+
+template <typename F> static void class_tier(int64_t C, int vp, F&& f) {
+    if (C <= 4) return vp == 4 ? f(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{}) : f(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
+    if (C <= 8) return vp == 4 ? f(std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{}) : f(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
+    if (C <= 16) return f(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
+    return f(std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{});
+}
+
+}  // namespace segk
+
+using namespace segk;
+
+extern "C" int segk_top_logits(const void* logits, int dtype, int64_t outer, int64_t C, int64_t inner, int64_t ld, int64_t k, float temperature,
+                               void* values, int32_t* indices, float* lse, int dev, void* stream) {
+    if (const int rc = check_logits("top_logits", logits, dtype, outer, C, inner, ld, k, temperature)) return rc;
+    SEGK_REQUIRE(values && indices, SEGK_EINVAL, "top_logits: null output");
+    SEGK_REQUIRE(aligned16(values) && aligned16(indices) && aligned16(lse), SEGK_EALIGN, "top_logits: outputs must be 16-byte aligned");
+    const bool pix = few(C, inner);
+    const Pixels px = pixels(outer, C, inner, ld, k, aligned16(logits));
+    SEGK_REQUIRE(!pix || px.blocks < (1ll << 31), SEGK_ESHAPE, "top_logits: too many positions");
+    SEGK_USE_DEVICE(dev);
+    hipStream_t st = (hipStream_t)stream;
+    SEGK_DISPATCH_DTYPE(dtype, T, {
+        if (pix) {
+            class_tier(C, px.vp, [&](auto cm, auto vp) {
+                hipLaunchKernelGGL((top_pixels_kernel<T, cm(), vp()>), dim3((unsigned)px.blocks), dim3(256), 0, st, (const T*)logits, ld, px.s_c,
+                                   px.s_p, px.inner, (int)C, (int)k, 1.f / temperature, (T*)values, indices, px.ts_c, px.ts_p, lse, px.blocks_each);
+            });
+        } else {
+            row_tier<T>(C, [&](auto nt, auto nch) {
+                hipLaunchKernelGGL((top_rows_kernel<T, nt(), nch()>), dim3((unsigned)outer), dim3(nt()), 0, st, (const T*)logits, ld, (int)C, (int)k,
+                                   1.f / temperature, (T*)values, indices, lse);
+            });
+        }
+    });
+    SEGK_LAUNCH_CHECK();
+    return SEGK_OK;
+}
+
+static constexpr int kCollect = 256;
+// floats of the workspace: partial counts, level-1 sums, then one sum per row or workgroup
+static size_t distill_partials(int64_t outer, int64_t C, int64_t inner) {
+    if (!few(C, inner)) return (size_t)outer;
+    return (size_t)(pixels(outer, C, inner, C * inner, 1, false).blocks);      // an upper bound for either vector width
+}
+extern "C" size_t segk_distill_workspace(int64_t outer, int64_t C, int64_t inner) {
+    if (outer <= 0 || C <= 0 || inner <= 0) return 0;
+    return 4 * (kCountBlocks + kCollect + distill_partials(outer, C, inner));
+}
+
+extern "C" int segk_distill(const void* logits, int dtype, int64_t outer, int64_t C, int64_t inner, int64_t ld, const void* values, int values_dtype,
+                            const void* indices, int index_bytes, const float* teacher_lse, int64_t k, float temperature, float weight, int flags,
+                            const float* upstream, float* loss, float* position_loss, void* dlogits, int64_t ld_d, void* workspace,
+                            size_t workspace_bytes, int dev, void* stream) {
+    if (const int rc = check_logits("distill", logits, dtype, outer, C, inner, ld, k, temperature)) return rc;
+    const bool mean = flags & 1, each = flags & 2, skip = flags & 4;
+    SEGK_REQUIRE(values && indices && workspace, SEGK_EINVAL, "distill: null pointer");
+    SEGK_REQUIRE(values_dtype == SEGK_F32 || values_dtype == SEGK_BF16, SEGK_EINVAL, "distill: unknown dtype %d of the values", values_dtype);
+    SEGK_REQUIRE(index_bytes == 4 || index_bytes == 8, SEGK_EINVAL, "distill: indices have 4 or 8 bytes, not %d", index_bytes);
+    SEGK_REQUIRE(loss || position_loss || dlogits, SEGK_EINVAL, "distill: no output");
+    SEGK_REQUIRE(!(mean && each), SEGK_EINVAL, "distill: a mean has one upstream gradient, not one for each position");
+    SEGK_REQUIRE(!(each || skip) || (upstream && dlogits), SEGK_EINVAL, "distill: this flag needs an upstream gradient and dlogits");
+    SEGK_REQUIRE(!(skip && (each || loss || position_loss)), SEGK_EINVAL, "distill: only the gradient of a scalar can be left as it is");
+    SEGK_REQUIRE(!dlogits || (ld_d >= C * inner && reinterpret_cast<uintptr_t>(dlogits) % esize(dtype) == 0), SEGK_ESHAPE, "distill: bad dlogits");
+    SEGK_REQUIRE(workspace_bytes >= segk_distill_workspace(outer, C, inner), SEGK_EWORKSPACE, "distill: workspace too small");
+    SEGK_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 4 == 0, SEGK_EALIGN, "distill: workspace must be 4-byte aligned");
+    const bool pix = few(C, inner);
+    const bool vec = aligned16(logits) && (!dlogits || (aligned16(dlogits) && ld_d % 4 == 0));
+    const Pixels px = pixels(outer, C, inner, ld, k, vec);
+    SEGK_REQUIRE(!pix || px.blocks < (1ll << 31), SEGK_ESHAPE, "distill: too many positions");
+    SEGK_USE_DEVICE(dev);
+    hipStream_t st = (hipStream_t)stream;
+    int* counts = static_cast<int*>(workspace);
+    float* collected = reinterpret_cast<float*>(counts + kCountBlocks);
+    float* partial = collected + kCollect;
+    DistillArgs a = {};
+    a.z = logits; a.ld = ld; a.V = (int)C; a.k = (int)k;
+    a.t = values; a.t_bf16 = values_dtype == SEGK_BF16; a.idx = indices; a.idx64 = index_bytes == 8; a.tlse = teacher_lse;
+    a.T = temperature; a.invT = 1.f / temperature; a.weight = weight;
+    a.upstream = upstream; a.up_each = each; a.skip_if_one = skip;
+    a.counts = mean ? counts : nullptr;
+    a.dz = dlogits; a.ld_d = ld_d;
+    if (pix) {
+        a.inner = px.inner; a.s_c = px.s_c; a.s_p = px.s_p; a.ts_c = px.ts_c; a.ts_p = px.ts_p;
+        a.d_c = px.s_c; a.d_p = inner == 1 ? ld_d : 1;
+        a.row_loss = position_loss; a.partial = loss ? partial : nullptr;
+    } else {
+        a.inner = 1; a.ts_c = 1; a.ts_p = k;
+        a.row_loss = position_loss ? position_loss : partial;
+    }
+    if (mean) {
+        hipLaunchKernelGGL(distill_count_kernel, dim3(kCountBlocks), dim3(256), 0, st, a, outer * inner, counts);
+        SEGK_LAUNCH_CHECK();
+    }
+    int64_t n = pix ? px.blocks : outer;
+    SEGK_DISPATCH_DTYPE(dtype, T, {
+        if (pix) {
+            class_tier(C, px.vp, [&](auto cm, auto vp) {
+                if (dlogits) hipLaunchKernelGGL((distill_pixels_kernel<T, cm(), vp(), true>), dim3((unsigned)n), dim3(256), 0, st, a, px.blocks_each);
+                else hipLaunchKernelGGL((distill_pixels_kernel<T, cm(), vp(), false>), dim3((unsigned)n), dim3(256), 0, st, a, px.blocks_each);
+            });
+        } else {
+            row_tier<T>(C, [&](auto nt, auto nch) {
+                if (dlogits) hipLaunchKernelGGL((distill_rows_kernel<T, nt(), nch(), true>), dim3((unsigned)n), dim3(nt()), 0, st, a);
+                else hipLaunchKernelGGL((distill_rows_kernel<T, nt(), nch(), false>), dim3((unsigned)n), dim3(nt()), 0, st, a);
+            });
+        }
+    });
+    SEGK_LAUNCH_CHECK();
+    if (loss) {
+        const float* v = pix ? partial : a.row_loss;
+        if (n > 16384) {
+            hipLaunchKernelGGL(distill_collect_kernel, dim3(kCollect), dim3(1024), 0, st, v, n, collected);
+            SEGK_LAUNCH_CHECK();
+            v = collected;
+            n = kCollect;
+        }
+        hipLaunchKernelGGL(distill_finalize_kernel, dim3(1), dim3(1024), 0, st, v, (int)n, (const int*)a.counts, loss);
+        SEGK_LAUNCH_CHECK();
+    }
+    return SEGK_OK;
+}

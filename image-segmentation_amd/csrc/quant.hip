@@ -1,0 +1,296 @@
+// Microscaled 4-bit floating point (e2m1 values, one power-of-two scale for each 32 values of a row): packing, unpacking, and the
+// linear layer y = x w^T + bias with both operands in that form on the scaled matrix instructions.
+//
+//     e = floor(log2(max |x| of the 32 values)) - 2,   code = e2m1(x / 2^e), nearest, ties to even, beyond 6 -> 6
+// The scale is stored as the byte e + 127 (e >= -127; all-zero blocks get 0); a NaN or an infinity among the 32 makes it 255, which
+// stands for NaN.  Rows are padded with zeros to whole slices of 128 values:
+//     codes  [rows][slices][64 bytes], two codes a byte, the even column in the low half
+//     scales [slices][rows][4 bytes]: the four scales of a row's slice are one dword, and those of neighbouring rows are
+//            neighbours, so a tile of rows gets its scales with coalesced loads
+#include "common.h"
+
+namespace segk {
+
+constexpr int kSlice = 128;
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// n / d for n < 2^31 by a multiplication (d fixed on the host)
+struct Divide {
+    uint32_t d, magic, shift;
+    explicit Divide(uint32_t d_) : d(d_) {
+        uint32_t l = 0;
+        while ((1ull << l) < d) ++l;
+        shift = 31 + l;
+        magic = (uint32_t)(((1ull << shift) + d - 1) / d);
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (uint32_t)(((uint64_t)n * magic) >> shift); }
+};
+
+// 16 bytes from an address that is only aligned to its elements
+template <typename T> struct alignas(sizeof(T)) Raw16 { T e[16 / sizeof(T)]; };
+
+template <typename T> __device__ __forceinline__ void load8_any(const T* p, float (&v)[8]) {
+    constexpr int N = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int h = 0; h < 8 / N; ++h) {
+        Raw16<T> r;
+        __builtin_memcpy(&r, p + h * N, 16);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[h * N + i] = Elem<T>::to_f(r.e[i]);
+    }
+}
+template <typename T> __device__ __forceinline__ void store8_any(T* p, const float (&v)[8]) {
+    constexpr int N = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int h = 0; h < 8 / N; ++h) {
+        Raw16<T> r;
+#pragma unroll
+        for (int i = 0; i < N; ++i) r.e[i] = Elem<T>::from_f(v[h * N + i]);
+        __builtin_memcpy(p + h * N, &r, 16);
+    }
+}
+
+// The scale byte of a block from the bits of its largest magnitude, and the factor that divides by the scale.  The exponent field
+// of a float is floor(log2) + 127, so the byte is that field less 2; fields up to 2 (and subnormals) give the smallest scale.
+__device__ __forceinline__ uint32_t scale_byte(uint32_t top) {
+    const uint32_t f = top >> 23;
+    return f == 255u ? 255u : (f > 2u ? f - 2u : 0u);
+}
+__device__ __forceinline__ float scale_inverse(uint32_t byte) { return byte == 255u ? 0.f : __uint_as_float((254u - byte) << 23); }
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+    return __uint_as_float(byte == 255u ? 0x7FC00000u : byte == 0u ? 0x00400000u : byte << 23);
+}
+// eight values, already divided by their scale, as eight codes
+__device__ __forceinline__ uint32_t pack_codes(const float (&y)[8]) {
+    uint32_t r = 0;
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, y[0], y[1], 1.f, 0);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, y[2], y[3], 1.f, 1);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, y[4], y[5], 1.f, 2);
+    r = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(r, y[6], y[7], 1.f, 3);
+    return r;
+}
+__device__ __forceinline__ uint32_t quad_max(uint32_t v) {
+    uint32_t o = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xF, 0xF, true);      // lane ^ 1
+    v = v > o ? v : o;
+    o = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xF, 0xF, true);               // lane ^ 2
+    return v > o ? v : o;
+}
+
+// One thread for 8 values, four neighbouring threads for a block, sixteen for a slice of a row: 16 bytes (bf16) read and 4 written
+// per thread, both coalesced.
+template <typename T>
+__global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const T* __restrict__ x, int64_t ld, int cols, uint32_t items, Divide per_row,
+                                                             int64_t rows, int64_t row0, uint32_t* __restrict__ codes,
+                                                             uint32_t* __restrict__ scales) {
+    const uint32_t item = blockIdx.x * 256u + threadIdx.x;
+    if (item >= items) return;                                     // items are whole slices: a group of 16 lanes leaves together
+    const uint32_t r = per_row(item), i = item - r * per_row.d;
+    const int64_t row = row0 + r;
+    const int c0 = (int)i * 8;
+    float v[8];
+    const T* p = x + row * ld + c0;
+    if (c0 + 8 <= cols) load8_any<T>(p, v);
+    else
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = c0 + j < cols ? Elem<T>::to_f(p[j]) : 0.f;
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t b = __float_as_uint(v[j]) & 0x7FFFFFFFu;
+        top = top > b ? top : b;
+    }
+    const uint32_t byte = scale_byte(quad_max(top));
+    const float inv = scale_inverse(byte);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = byte == 255u ? 0.f : v[j] * inv;
+    codes[row * per_row.d + i] = pack_codes(v);
+    const int lane = threadIdx.x & 63;
+    const uint32_t b1 = __shfl(byte, (lane & 48) + 4, 64), b2 = __shfl(byte, (lane & 48) + 8, 64), b3 = __shfl(byte, (lane & 48) + 12, 64);
+    if ((i & 15u) == 0) scales[(int64_t)(i >> 4) * rows + row] = byte | (b1 << 8) | (b2 << 16) | (b3 << 24);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void mxfp4_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales, int cols,
+                                                               uint32_t items, Divide per_row, int64_t rows, int64_t row0, T* __restrict__ y,
+                                                               int64_t ld) {
+    const uint32_t item = blockIdx.x * 256u + threadIdx.x;
+    if (item >= items) return;
+    const uint32_t r = per_row(item), i = item - r * per_row.d;
+    const int64_t row = row0 + r;
+    const int c0 = (int)i * 8;
+    if (c0 >= cols) return;
+    const uint32_t c = codes[row * per_row.d + i];
+    const float s = scale_value(scales[((int64_t)(i >> 4) * rows + row) * 4 + ((i >> 2) & 3)]);
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        // the magnitude 0, .5, 1, 1.5, 2, 3, 4, 6 as a float: two exponent bits and one fraction bit moved to their places
+        const uint32_t m = (c >> (4 * j)) & 7u;
+        const float f = m < 2u ? 0.5f * (float)m : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1u) << 22);
+        v[j] = __uint_as_float(__float_as_uint(f * s) | ((c >> (4 * j)) & 8u) << 28);
+    }
+    T* p = y + row * ld + c0;
+    if (c0 + 8 <= cols) store8_any<T>(p, v);
+    else
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (c0 + j < cols) p[j] = Elem<T>::from_f(v[j]);
+}
+
+// ------------------------------------------------------------------------------------------------ the product
+__device__ __forceinline__ f32x4 mfma_fp4(const u32x4 a, const u32x4 b, const f32x4 acc, uint32_t sa, uint32_t sb) {
+    const i32x8 av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0}, bv = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, acc, 4, 4, 0, (int)sa, 0, (int)sb);
+}
+
+struct LinearArgs {
+    const uint8_t* w;            // codes of the weights [N][ldc]
+    const uint32_t* ws;          // their scales [slices][N]
+    const uint8_t* x;            // codes of the inputs [M][ldc]
+    const uint32_t* xs;
+    const float* bias;
+    void* y;
+    int64_t M, N, ldc, ldy;
+    int slices, vec;             // vec: four neighbouring outputs may be stored at once
+};
+
+template <typename TO>
+__device__ __forceinline__ void store_outputs(const LinearArgs& a, int64_t m, int64_t n, const f32x4 acc) {
+    if (m >= a.M) return;
+    TO* y = static_cast<TO*>(a.y) + m * a.ldy + n;
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = acc[i] + (a.bias && n + i < a.N ? a.bias[n + i] : 0.f);
+    if (a.vec && n + 4 <= a.N) Elem<TO>::store4(y, v);
+    else
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (n + i < a.N) y[i] = Elem<TO>::from_f(v[i]);
+}
+
+// Few rows: a workgroup computes 16 outputs of 16 rows, its four waves share the slices.  Operands go straight from memory to the
+// matrix instruction: lane l holds the 32 values (16 bytes) of row l % 16 in the block l / 16 of the slice.
+template <typename TO>
+__global__ __launch_bounds__(256) void mxfp4_rows_kernel(const LinearArgs a) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * 16;
+    const int64_t n = n0 + r < a.N ? n0 + r : a.N - 1, m = m0 + r < a.M ? m0 + r : a.M - 1;
+    const uint8_t *wp = a.w + n * a.ldc + q * 16, *xp = a.x + m * a.ldc + q * 16;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int s = wave; s < a.slices; s += 4) {
+        const u32x4 wv = *reinterpret_cast<const u32x4*>(wp + (int64_t)s * 64), xv = *reinterpret_cast<const u32x4*>(xp + (int64_t)s * 64);
+        const uint32_t sw = a.ws[(int64_t)s * a.N + n] >> (8 * q), sx = a.xs[(int64_t)s * a.M + m] >> (8 * q);
+        acc = mfma_fp4(wv, xv, acc, sw, sx);
+    }
+    __shared__ f32x4 part[4][64];
+    part[wave][lane] = acc;
+    __syncthreads();
+    if (wave == 0) {
+        acc = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+        store_outputs<TO>(a, m0 + r, n0 + 4 * q, acc);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+static int64_t slices_of(int64_t cols) { return (cols + kSlice - 1) / kSlice; }
+
+static int check_matrix(const char* who, int dtype, const void* x, int64_t ld, int64_t rows, int64_t cols) {
+    SEGK_REQUIRE(x, SEGK_EINVAL, "%s: null pointer", who);
+    SEGK_REQUIRE(dtype == SEGK_F32 || dtype == SEGK_BF16, SEGK_EINVAL, "%s: unknown dtype %d", who, dtype);
+    SEGK_REQUIRE(rows > 0 && cols > 0 && rows < (1ll << 31) && cols < (1ll << 30), SEGK_ESHAPE, "%s: bad shape", who);
+    SEGK_REQUIRE(ld >= cols, SEGK_ESHAPE, "%s: ld smaller than a row", who);
+    SEGK_REQUIRE(reinterpret_cast<uintptr_t>(x) % esize(dtype) == 0, SEGK_EALIGN, "%s: matrix is not aligned to its type", who);
+    return SEGK_OK;
+}
+static int check_packed(const char* who, const void* codes, const void* scales) {
+    SEGK_REQUIRE(codes && scales, SEGK_EINVAL, "%s: null pointer", who);
+    SEGK_REQUIRE(aligned16(codes), SEGK_EALIGN, "%s: codes must be 16-byte aligned", who);
+    SEGK_REQUIRE(reinterpret_cast<uintptr_t>(scales) % 4 == 0, SEGK_EALIGN, "%s: scales must be 4-byte aligned", who);
+    return SEGK_OK;
+}
+
+// f(first row, rows) for pieces of at most 2^31 - 1 items
+template <typename F> static int by_rows(int64_t rows, int64_t per_row, F&& f) {
+    const int64_t most = ((1ll << 31) - 256) / per_row;
+    for (int64_t r0 = 0; r0 < rows; r0 += most) {
+        if (const int rc = f(r0, rows - r0 < most ? rows - r0 : most)) return rc;
+    }
+    return SEGK_OK;
+}
+
+static int quantize(int dtype, const void* x, int64_t ld, int64_t rows, int64_t cols, void* codes, void* scales, hipStream_t st) {
+    const int64_t per_row = slices_of(cols) * 16;
+    return by_rows(rows, per_row, [&](int64_t r0, int64_t n) -> int {
+        const uint32_t items = (uint32_t)(n * per_row);
+        SEGK_DISPATCH_DTYPE(dtype, T, hipLaunchKernelGGL((mxfp4_quantize_kernel<T>), dim3((items + 255) / 256), dim3(256), 0, st, (const T*)x, ld,
+                                                         (int)cols, items, Divide((uint32_t)per_row), rows, r0, (uint32_t*)codes, (uint32_t*)scales));
+        SEGK_LAUNCH_CHECK();
+        return SEGK_OK;
+    });
+}
+
+}  // namespace segk
+
+using namespace segk;
+
+extern "C" size_t segk_mxfp4_codes_bytes(int64_t rows, int64_t cols) { return rows > 0 && cols > 0 ? (size_t)(rows * slices_of(cols) * 64) : 0; }
+extern "C" size_t segk_mxfp4_scales_bytes(int64_t rows, int64_t cols) { return rows > 0 && cols > 0 ? (size_t)(rows * slices_of(cols) * 4) : 0; }
+
+extern "C" int segk_mxfp4_quantize(int dtype, const void* x, int64_t ld, int64_t rows, int64_t cols, void* codes, void* scales, int dev, void* stream) {
+    if (const int rc = check_matrix("mxfp4_quantize", dtype, x, ld, rows, cols)) return rc;
+    if (const int rc = check_packed("mxfp4_quantize", codes, scales)) return rc;
+    SEGK_USE_DEVICE(dev);
+    return quantize(dtype, x, ld, rows, cols, codes, scales, (hipStream_t)stream);
+}
+
+extern "C" int segk_mxfp4_dequantize(int dtype, const void* codes, const void* scales, int64_t rows, int64_t cols, void* y, int64_t ld, int dev,
+                                     void* stream) {
+    if (const int rc = check_matrix("mxfp4_dequantize", dtype, y, ld, rows, cols)) return rc;
+    if (const int rc = check_packed("mxfp4_dequantize", codes, scales)) return rc;
+    SEGK_USE_DEVICE(dev);
+    const int64_t per_row = slices_of(cols) * 16;
+    return by_rows(rows, per_row, [&](int64_t r0, int64_t n) -> int {
+        const uint32_t items = (uint32_t)(n * per_row);
+        SEGK_DISPATCH_DTYPE(dtype, T, hipLaunchKernelGGL((mxfp4_dequantize_kernel<T>), dim3((items + 255) / 256), dim3(256), 0, (hipStream_t)stream,
+                                                         (const uint32_t*)codes, (const uint8_t*)scales, (int)cols, items,
+                                                         Divide((uint32_t)per_row), rows, r0, (T*)y, ld));
+        SEGK_LAUNCH_CHECK();
+        return SEGK_OK;
+    });
+}
+
+extern "C" size_t segk_mxfp4_linear_workspace(int64_t M, int64_t K, int64_t N) {
+    (void)N;
+    return align_up(segk_mxfp4_codes_bytes(M, K), 16) + segk_mxfp4_scales_bytes(M, K);
+}
+
+extern "C" int segk_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const void* x_codes, const void* x_scales, int64_t M, int64_t K,
+                                 const void* w_codes, const void* w_scales, int64_t N, const float* bias, void* y, int y_dtype, int64_t ldy,
+                                 void* workspace, size_t workspace_bytes, int dev, void* stream) {
+    SEGK_REQUIRE((x != nullptr) != (x_codes != nullptr), SEGK_EINVAL, "mxfp4_linear: either x or x_codes is given");
+    SEGK_REQUIRE(M > 0 && K > 0 && N > 0 && M < (1ll << 31) && N < (1ll << 31) && K < (1ll << 30), SEGK_ESHAPE, "mxfp4_linear: bad shape");
+    if (const int rc = check_matrix("mxfp4_linear", y_dtype, y, ldy, M, N)) return rc;
+    if (const int rc = check_packed("mxfp4_linear", w_codes, w_scales)) return rc;
+    if (x) {
+        if (const int rc = check_matrix("mxfp4_linear", x_dtype, x, ldx, M, K)) return rc;
+        SEGK_REQUIRE(workspace && workspace_bytes >= segk_mxfp4_linear_workspace(M, K, N), SEGK_EWORKSPACE, "mxfp4_linear: workspace too small");
+        SEGK_REQUIRE(aligned16(workspace), SEGK_EALIGN, "mxfp4_linear: workspace must be 16-byte aligned");
+    } else if (const int rc = check_packed("mxfp4_linear", x_codes, x_scales)) return rc;
+    SEGK_REQUIRE((M + 15) / 16 < 65536, SEGK_ESHAPE, "mxfp4_linear: too many rows");
+    SEGK_USE_DEVICE(dev);
+    hipStream_t st = (hipStream_t)stream;
+    if (x) {
+        x_codes = workspace;
+        x_scales = (const uint8_t*)workspace + align_up(segk_mxfp4_codes_bytes(M, K), 16);
+        if (const int rc = quantize(x_dtype, x, ldx, M, K, workspace, const_cast<void*>(x_scales), st)) return rc;
+    }
+    LinearArgs a = {};
+    a.w = (const uint8_t*)w_codes; a.ws = (const uint32_t*)w_scales; a.x = (const uint8_t*)x_codes; a.xs = (const uint32_t*)x_scales;
+    a.bias = bias; a.y = y; a.M = M; a.N = N; a.ldc = slices_of(K) * 64; a.ldy = ldy; a.slices = (int)slices_of(K);
+    a.vec = reinterpret_cast<uintptr_t>(y) % (4 * esize(y_dtype)) == 0 && ldy % 4 == 0;
+    SEGK_DISPATCH_DTYPE(y_dtype, TO, hipLaunchKernelGGL((mxfp4_rows_kernel<TO>), dim3((unsigned)((N + 15) / 16), (unsigned)((M + 15) / 16)), dim3(256),
+                                                        0, st, a));
+    SEGK_LAUNCH_CHECK();
+    return SEGK_OK;
+}

@@ -26,6 +26,9 @@ _PROTOS = {
     "segk_dice_focal_finalize": (I, [P, P, L, L, L, I, P, I, P]),
     "segk_dice_focal_bwd": (I, [P, I, P, P, L, L, L, F, P, I, P, P, P, P, P, I, P]),
     "segk_argmax_dice": (I, [P, I, P, L, L, L, P, P, P, I, P]),
+    "segk_top_logits": (I, [P, I, L, L, L, L, L, F, P, P, P, I, P]),
+    "segk_distill_workspace": (Z, [L, L, L]),
+    "segk_distill": (I, [P, I, L, L, L, L, P, I, P, I, P, L, F, F, I, P, P, P, P, L, P, Z, I, P]),
     "segk_edge_workspace": (Z, [L, L, L]),
     "segk_edge_bwd_workspace": (Z, [L, L, L]),
     "segk_edge_fwd": (I, [P, L, L, L, F, P, P, P, Z, I, P]),
@@ -97,6 +100,12 @@ _PROTOS = {
     "segk_upsample2x_bwd": (I, [I, P, L, P, L, L, L, L, L, I, P, L, I, P]),
     "segk_colsum_workspace": (Z, [L, L]),
     "segk_colsum": (I, [I, P, L, L, L, P, I, P, Z, I, P]),
+    "segk_mxfp4_codes_bytes": (Z, [L, L]),
+    "segk_mxfp4_scales_bytes": (Z, [L, L]),
+    "segk_mxfp4_quantize": (I, [I, P, L, L, L, P, P, I, P]),
+    "segk_mxfp4_dequantize": (I, [I, P, P, L, L, P, L, I, P]),
+    "segk_mxfp4_linear_workspace": (Z, [L, L, L]),
+    "segk_mxfp4_linear": (I, [P, I, L, P, P, L, L, P, P, L, P, P, I, L, P, Z, I, P]),
     "segk_copy_slice": (I, [I, P, L, P, L, L, L, I, I, P]),
     "segk_block2": (I, [I, P, L, P, L, L, L, L, L, I, I, P]),
     "segk_resize_bilinear_fwd": (I, [I, P, L, L, L, L, L, L, L, F, F, P, I, P, L, I, P]),

@@ -1,0 +1,234 @@
+"""Distillation: a teacher's top logits (`top_logits`) and the loss of a student against them (`distill_loss_topk`), autograd over
+the C ABI (segk_top_logits, segk_distill).  CPU tensors are served by the same formulas in torch ops (`_host_*`)."""
+import math
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import ops
+from ._lib import call, query
+from .ops import _env, dt
+
+MEAN, EACH, SKIP = 1, 2, 4          # flag bits of segk_distill
+MAX_K = 64
+PLANE_CLASSES = 32                  # up to this many classes the kernels read class planes [N, C, ...] as they are
+REST_FLOOR = 2.0 ** -20             # a rest of the teacher's mass up to this is rounding and counts as none
+
+
+class TopLogits(NamedTuple):
+    """What is kept of a teacher's logits: the k greatest of each position in descending order, their classes (int32; -1 or any
+    other value that is no class marks an entry that does not exist), and the logsumexp of all classes at the temperature the
+    loss will use (None: the kept logits are renormalised).  `values` and `indices` have the logits' shape with k in place of the
+    class dimension, `lse` the shape without it.  Batches like any named tuple in a DataLoader."""
+    values: torch.Tensor
+    indices: torch.Tensor
+    lse: Optional[torch.Tensor] = None
+
+    def to(self, *args, **kw):
+        v = self.values.to(*args, **kw)
+        nb = bool(kw.get("non_blocking", False))
+        return TopLogits(v, self.indices.to(v.device, non_blocking=nb), None if self.lse is None else self.lse.to(v.device, non_blocking=nb))
+
+    def cuda(self, device=None):
+        return self.to(torch.device("cuda" if device is None else device))
+
+    def cpu(self):
+        return self.to(torch.device("cpu"))
+
+
+def _check(logits, dim, temperature):
+    if logits.dim() < 1 or not logits.dtype.is_floating_point:
+        raise TypeError(f"logits of floating point type are expected, got {logits.dtype} with {logits.dim()} dimensions")
+    if not -logits.dim() <= dim < logits.dim():
+        raise IndexError(f"dimension {dim} is out of range for logits with {logits.dim()} dimensions")
+    if not (isinstance(temperature, (int, float)) and 0 < temperature < math.inf):
+        raise ValueError(f"temperature has to be positive and finite, got {temperature}")
+    return dim % logits.dim()
+
+
+def _canonical(x, dim):
+    """(tensor, outer, C, inner, ld, moved): x as `outer` images of C x `inner`, in place where its strides allow it.  More than
+    PLANE_CLASSES classes in front of other dimensions are moved to the end (a copy)."""
+    shape = x.shape
+    C, outer, inner = shape[dim], math.prod(shape[:dim]), math.prod(shape[dim + 1:])
+    moved = inner > 1 and C > PLANE_CLASSES
+    if moved:
+        x, outer, inner = x.movedim(dim, -1), outer * inner, 1
+    x = x.reshape(outer, C, inner)
+    if (C > 1 and x.stride(1) != inner) or (inner > 1 and x.stride(2) != 1) or (outer > 1 and x.stride(0) < C * inner):
+        x = x.contiguous()
+    return x, outer, C, inner, (x.stride(0) if outer > 1 else C * inner), moved
+
+
+def _restore(y, shape, dim, n, moved):
+    """The kernels' [outer][n][inner] (or [outer * inner][n] if the classes were moved) in the caller's order of dimensions."""
+    if moved:
+        return y.reshape(shape[:dim] + shape[dim + 1:] + (n,)).movedim(-1, dim)
+    return y.reshape(shape[:dim] + (n,) + shape[dim + 1:])
+
+
+def top_logits(logits, k, dim=1, temperature=1.0):
+    """The k greatest logits along `dim` (1 <= k <= min(64, classes)) as TopLogits(values, indices int32, lse): descending, ties to
+    the lower class, NaN as the greatest; lse = logsumexp(logits / temperature) over all classes, fp32.  float32, bfloat16 and
+    float16 logits; values keep their type.  Not differentiable: a teacher's answer is data.
+
+    The class dimension may stand anywhere: last (rows of any number of classes, read where they are) or in front of others as in
+    [N, C, H, W] (up to 32 classes read where they are, more are copied once into rows)."""
+    dim = _check(logits, dim, temperature)
+    C = logits.shape[dim]
+    if not 1 <= k <= min(MAX_K, C):
+        raise ValueError(f"k has to be between 1 and min({MAX_K}, {C} classes), got {k}")
+    z = logits.detach()
+    rest = z.shape[:dim] + z.shape[dim + 1:]
+    if not z.is_cuda or z.numel() == 0:
+        return _host_top(z, k, dim, temperature)
+    z, outer, C, inner, ld, moved = _canonical(z.float() if z.dtype == torch.float16 else z, dim)
+    values = torch.empty((outer, k, inner), dtype=z.dtype, device=z.device)
+    indices = torch.empty((outer, k, inner), dtype=torch.int32, device=z.device)
+    lse = torch.empty(rest, dtype=torch.float32, device=z.device)
+    dev, st = _env(z)
+    with ops._streamed("top logits", z.numel() * z.element_size()):
+        call("segk_top_logits", z.data_ptr(), dt(z.dtype), outer, C, inner, ld, k, temperature, values.data_ptr(), indices.data_ptr(),
+             lse.data_ptr(), dev, st)
+    return TopLogits(_restore(values, logits.shape, dim, k, moved).to(logits.dtype), _restore(indices, logits.shape, dim, k, moved), lse)
+
+
+class _DistillFn(torch.autograd.Function):
+    """(student logits, target) -> loss.  Where a scalar's gradient will be wanted, the forward pass writes it for an upstream
+    gradient of 1 while the row is still in registers; the backward pass hands it over, recomputed only if upstream is not 1."""
+
+    @staticmethod
+    def forward(ctx, logits, values, indices, lse, dim, temperature, weight, reduction, want_grad):
+        z, outer, C, inner, ld, moved = _canonical(logits.float() if logits.dtype == torch.float16 else logits, dim)
+        k = values.shape[dim]
+        if moved:
+            values, indices = values.movedim(dim, -1), indices.movedim(dim, -1)
+        values, indices = values.contiguous(), indices.contiguous()
+        lse = None if lse is None else lse.contiguous()
+        ctx.meta = (outer, C, inner, ld, moved, k, dim, float(temperature), float(weight), reduction, logits.shape, logits.dtype)
+        rest = logits.shape[:dim] + logits.shape[dim + 1:]
+        each = reduction == "none"
+        out = torch.empty(rest if each else (), dtype=torch.float32, device=z.device)
+        dz = torch.empty((outer, C, inner), dtype=z.dtype, device=z.device) if want_grad and not each else None
+        _DistillFn._launch(ctx.meta, z, values, indices, lse, None, MEAN if reduction == "mean" else 0, None if each else out, out if each else None, dz)
+        ctx.save_for_backward(z, values, indices, lse)
+        ctx.dz = dz
+        return out
+
+    @staticmethod
+    def _launch(meta, z, values, indices, lse, upstream, flags, loss, each, dz):
+        outer, C, inner, ld, moved, k, dim, T, weight, reduction, shape, in_dtype = meta
+        # a buffer of its own for every call: launches on other streams and replays of captured graphs never share one
+        ws = torch.empty(query("segk_distill_workspace", outer, C, inner), dtype=torch.uint8, device=z.device)
+        p = ops._p
+        dev, st = _env(z)
+        with ops._streamed("distillation loss", z.numel() * z.element_size() * (2 if dz is not None else 1)):
+            call("segk_distill", z.data_ptr(), dt(z.dtype), outer, C, inner, ld, values.data_ptr(), dt(values.dtype), indices.data_ptr(),
+                 indices.element_size(), p(lse), k, T, weight, flags, p(upstream), p(loss), p(each), p(dz), C * inner, ws.data_ptr(), ws.numel(),
+                 dev, st)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        z, values, indices, lse = ctx.saved_tensors
+        outer, C, inner, ld, moved, k, dim, T, weight, reduction, shape, in_dtype = ctx.meta
+        dz, ctx.dz = ctx.dz, None               # handed over once; a second backward pass computes its own
+        flags = EACH if reduction == "none" else MEAN if reduction == "mean" else 0
+        if dz is None:
+            dz = torch.empty((outer, C, inner), dtype=z.dtype, device=z.device)
+        else:
+            flags |= SKIP
+        _DistillFn._launch(ctx.meta, z, values, indices, lse, g.float().contiguous(), flags, None, None, dz)
+        return (_restore(dz, shape, dim, C, moved).to(in_dtype),) + (None,) * 8
+
+
+def distill_loss_topk(pred, target, temperature=1.0, reduction="mean", dim=1, weight=1.0):
+    """Distillation loss of the student's logits `pred` against a teacher's top logits.
+
+    With q = softmax(pred / T) over all classes along `dim`, a position contributes
+        T^2 [ sum_j p_j (log p_j - log q_(i_j)) + r (log r - log R) ]
+    where, if target.lse is None, p = softmax(values / T) over the kept entries and r = 0; otherwise p_j = exp(value_j / T - lse) and
+    r = 1 - sum p is what the teacher gave to the other classes together, R what the student gives them (`lse` has to be taken at
+    the same temperature).  Entries whose index is no class do not exist; a position without entries (padding) has loss 0 and
+    gradient 0.  reduction: 'mean' over the positions that have an entry (0 if there are none), 'sum', or 'none' (a map).
+    `weight` scales loss and gradient; it costs nothing, where multiplying the returned loss costs another pass over the logits.
+
+    pred: float32, bfloat16 or float16, any strides; target: TopLogits or a tuple (values, indices[, lse]) with float32 / bfloat16 /
+    float16 values and int32 / int64 indices.  Returns float32; the gradient has pred's type.  Sums run in float32."""
+    dim = _check(pred, dim, temperature)
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError('Reduction parameter unknown.')
+    target = TopLogits(*target)
+    values, indices, lse = target
+    shape, C = pred.shape, pred.shape[dim]
+    k = values.shape[dim] if values.dim() == pred.dim() else 0
+    want = shape[:dim] + (k,) + shape[dim + 1:]
+    if values.shape != want or indices.shape != want:
+        raise ValueError(f"values and indices need the logits' shape {tuple(shape)} with the kept entries in dimension {dim}, got "
+                         f"{tuple(values.shape)} and {tuple(indices.shape)}")
+    if not 1 <= k <= min(MAX_K, C):
+        raise ValueError(f"between 1 and min({MAX_K}, {C} classes) kept entries are expected, got {k}")
+    if indices.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"indices have to be int32 or int64, got {indices.dtype}")
+    if not values.dtype.is_floating_point:
+        raise TypeError(f"values of floating point type are expected, got {values.dtype}")
+    if lse is not None and (lse.shape != shape[:dim] + shape[dim + 1:] or not lse.dtype.is_floating_point):
+        raise ValueError(f"lse has to have the logits' shape without dimension {dim} and a floating point type, got {tuple(lse.shape)} {lse.dtype}")
+    if any(t is not None and t.device != pred.device for t in target):
+        raise ValueError("logits and target have to be on the same device")
+    if any(t is not None and t.requires_grad for t in target):
+        raise ValueError("the target is data: detach the teacher's logits")
+    if not pred.is_cuda or pred.numel() == 0:
+        return _host_distill(pred, values, indices, lse, dim, temperature, weight, reduction)
+    if values.dtype == torch.float16:
+        values = values.float()
+    dt(torch.float32 if pred.dtype == torch.float16 else pred.dtype), dt(values.dtype)       # refuses what the kernels do not read
+    want_grad = torch.is_grad_enabled() and pred.requires_grad
+    return _DistillFn.apply(pred, values, indices, None if lse is None else lse.float(), dim, temperature, weight, reduction, want_grad)
+
+
+# ------------------------------------------------------------------------------------ host tensors
+def _host_top(z, k, dim, temperature):
+    w = z.float() if z.dtype in (torch.float16, torch.bfloat16) else z
+    if z.numel() == 0:
+        shape = z.shape[:dim] + (k,) + z.shape[dim + 1:]
+        return TopLogits(z.new_empty(shape), torch.empty(shape, dtype=torch.int32, device=z.device),
+                         torch.empty(z.shape[:dim] + z.shape[dim + 1:], dtype=torch.float32, device=z.device))
+    indices = torch.sort(w, dim=dim, descending=True, stable=True).indices.narrow(dim, 0, k)
+    # two-byte types are gathered as integers: torch's gather on the CPU turns their NaNs into other ones
+    raw = z.view(torch.int16) if z.element_size() == 2 else z
+    return TopLogits(torch.gather(raw, dim, indices).view(z.dtype), indices.to(torch.int32), torch.logsumexp(w / temperature, dim).float())
+
+
+def _host_distill(pred, values, indices, lse, dim, T, weight, reduction):
+    z = (pred if pred.dtype == torch.float64 else pred.float()).movedim(dim, -1) / T
+    t = values.movedim(dim, -1).to(z.dtype) / T
+    at = indices.movedim(dim, -1).to(torch.int64)
+    valid = (at >= 0) & (at < z.shape[-1])
+    counted = valid.any(-1)
+    z = torch.where(counted.unsqueeze(-1), z, torch.zeros((), dtype=z.dtype))          # unread: NaN there does not matter
+    at = torch.where(valid, at, torch.zeros((), dtype=at.dtype))
+    minus = torch.tensor(-math.inf, dtype=z.dtype)
+    t = torch.where(valid, t, minus)
+    logq = torch.log_softmax(z, -1)
+    if lse is None:
+        top = t.amax(-1, keepdim=True)
+        e = torch.where(valid & (top > -math.inf), torch.exp(t - top), torch.zeros((), dtype=z.dtype))
+        s = e.sum(-1, keepdim=True)
+        p = torch.where(s == 0, torch.zeros((), dtype=z.dtype), e / s)
+    else:
+        p = torch.where(valid, torch.exp(t - lse.to(z.dtype).unsqueeze(-1)), torch.zeros((), dtype=z.dtype))
+    term = p * (torch.log(torch.where(p == 0, torch.ones((), dtype=z.dtype), p)) - torch.where(p == 0, torch.zeros((), dtype=z.dtype), torch.gather(logq, -1, at)))
+    row = term.sum(-1)
+    if lse is not None:
+        kept = torch.zeros_like(z, dtype=torch.int32).scatter_add_(-1, at, valid.to(torch.int32)) > 0
+        r = 1 - p.sum(-1)
+        has = (r > REST_FLOOR) & ~kept.all(-1) & counted
+        outside = torch.logsumexp(torch.where(kept & has.unsqueeze(-1), minus, logq), -1)
+        r = torch.where(has, r, torch.ones((), dtype=z.dtype))
+        row = row + torch.where(has, r * (torch.log(r) - outside), torch.zeros((), dtype=z.dtype))
+    row = torch.where(counted, row * (T * T * weight), torch.zeros((), dtype=z.dtype))
+    if reduction == "none":
+        return row.to(torch.float32 if pred.dtype != torch.float64 else torch.float64)
+    total = row.sum()
+    return total / counted.sum().clamp(min=1) if reduction == "mean" else total

@@ -102,6 +102,39 @@ int segk_argmax_dice(const void* logits, int logits_dtype, const int64_t* labels
                      int64_t HW, uint8_t* mask, float* counts, int32_t* out_flags, int dev, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * Distillation from a teacher's top logits.  No counterpart in the reference, whose networks learn from label maps only; stands
+ * beside the losses above.  Logits are `outer` images (rows) of C classes x `inner` positions: element (o, c, i) at
+ * logits[o*ld + c*inner + i], ld >= C*inner; inner = 1 gives rows [outer][C] with the classes innermost, C*inner = an NCHW image
+ * otherwise (C <= 32 then).  fp32 or bf16, aligned to their type only.  Kept logits: `values` and `indices` [outer][k][inner],
+ * contiguous, 1 <= k <= min(64, C); `lse` [outer][inner] fp32 = log(sum over the classes of exp(logit / temperature)).
+ * ---------------------------------------------------------------------------------------------- */
+
+/* The k greatest logits of every position in descending order (NaN counts as greatest; ties: the lower class first), the classes
+ * they belong to (int32) and, if lse is not NULL, the logsumexp of all classes.  values have the dtype of logits.
+ * Outputs 16-byte aligned.  One pass over the logits. */
+int segk_top_logits(const void* logits, int dtype, int64_t outer, int64_t C, int64_t inner, int64_t ld, int64_t k, float temperature,
+                    void* values, int32_t* indices, float* lse, int dev, void* stream);
+
+/* loss of a position = T^2 [ sum_j p_j (log p_j - log q_(i_j)) + r (log r - log R) ], q = softmax(logits / T) over all classes and
+ *   teacher_lse NULL:   p = softmax of the kept values / T, r = 0
+ *   teacher_lse given:  p_j = exp(value_j / T - teacher_lse), r = 1 - sum p (counted as 0 up to 2^-20, and where every class was
+ *                       kept), R = sum of q over the classes that were not kept
+ * An entry whose index lies outside [0, C) does not exist; the p of entries with the same index add up; a position without any
+ * entry has loss 0 and gradient 0 and its logits are not read.  All losses and gradients are times `weight`.
+ *   loss          (optional) fp32: sum over the positions; flags bit0: their mean over the positions with an entry (0 if none)
+ *   position_loss (optional) fp32 [outer][inner]
+ *   dlogits       (optional) gradient of `loss` times *upstream (1 if NULL); element (o, c, i) at o*ld_d + c*inner + i, dtype of
+ *                 logits.  flags bit1: upstream has one value per position (not with bit0): gradient of position_loss.
+ * flags bit2 (upstream and dlogits given, no other output): dlogits already holds the gradient for an upstream of 1, and the
+ * call leaves it as it is if *upstream is 1 -- a backward pass that finds the gradient of the forward pass still right.
+ * values_dtype fp32 or bf16, index_bytes 4 or 8 (int32 / int64).  Deterministic. */
+size_t segk_distill_workspace(int64_t outer, int64_t C, int64_t inner);
+int segk_distill(const void* logits, int dtype, int64_t outer, int64_t C, int64_t inner, int64_t ld, const void* values, int values_dtype,
+                 const void* indices, int index_bytes, const float* teacher_lse, int64_t k, float temperature, float weight, int flags,
+                 const float* upstream, float* loss, float* position_loss, void* dlogits, int64_t ld_d, void* workspace,
+                 size_t workspace_bytes, int dev, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
  * Layout conversion at the network boundary.
  * ---------------------------------------------------------------------------------------------- */
 
@@ -522,6 +555,32 @@ int segk_linear_fwd(const float* x, const float* w, const float* bias, int64_t N
  * Fixed summation order (deterministic).   replaces: nn.Linear backward.                           */
 int segk_linear_bwd(const float* x, const float* w, const float* dy, int64_t N, int64_t K, int64_t O, float* dx, float* dw,
                     float* dbias, int flags, int dev, void* stream);
+
+/* ---- microscaled 4-bit floating point ------------------------------------------------------------
+ * No counterpart in the reference; stands beside the linear layer above for networks whose trained weights are packed.
+ * A matrix [rows][cols] is held as e2m1 values (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) with a power-of-two scale for
+ * each 32 values of a row, every row padded with zeros to S = ceil(cols / 128) slices of 128 values:
+ *   codes  [rows][S][64] bytes: two codes a byte, the even column in the low half; sign bit, two exponent bits, one fraction bit
+ *   scales [S][rows][4]  bytes: byte b of a row's slice belongs to its values 32 b .. 32 b + 31 and stands for 2^(byte - 127);
+ *                               255 stands for NaN
+ * Packing: e = floor(log2(largest magnitude of the 32)) - 2, at least -127 (all zeros: -127), values / 2^e to the nearest code, ties
+ * to the even one, magnitudes beyond 6 to 6; a NaN or an infinity among the 32 makes their scale 255.
+ * codes 16-byte aligned, scales 4-byte aligned; matrices aligned to their type (fp32 or bf16), ld in elements. */
+size_t segk_mxfp4_codes_bytes(int64_t rows, int64_t cols);
+size_t segk_mxfp4_scales_bytes(int64_t rows, int64_t cols);
+int segk_mxfp4_quantize(int dtype, const void* x, int64_t ld, int64_t rows, int64_t cols, void* codes, void* scales, int dev, void* stream);
+/* y = the values that the packed matrix stands for (exact in either type). */
+int segk_mxfp4_dequantize(int dtype, const void* codes, const void* scales, int64_t rows, int64_t cols, void* y, int64_t ld, int dev,
+                          void* stream);
+
+/* y[M][N] = x[M][K] w[N][K]^T + bias with both operands in packed form on the scaled matrix instructions, fp32 accumulation in an
+ * order fixed by the shape (deterministic), one rounding to y's type.  x is given as a matrix, packed by the call as above, or as
+ * x_codes / x_scales (the other NULL).  bias: fp32 [N] or NULL.
+ * workspace: segk_mxfp4_linear_workspace(M, K, N) bytes, 16-byte aligned; contents need not be cleared. */
+size_t segk_mxfp4_linear_workspace(int64_t M, int64_t K, int64_t N);
+int segk_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const void* x_codes, const void* x_scales, int64_t M, int64_t K,
+                      const void* w_codes, const void* w_scales, int64_t N, const float* bias, void* y, int y_dtype, int64_t ldy,
+                      void* workspace, size_t workspace_bytes, int dev, void* stream);
 
 #ifdef __cplusplus
 }

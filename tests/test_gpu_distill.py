@@ -1,0 +1,342 @@
+"""Top logits and the distillation loss on the GPU against the definitions in 64 bits (tests/distill_oracle.py, which also derives
+the error bounds)."""
+import math
+
+import pytest
+import torch
+
+from distill_oracle import half_step, loss_and_gradient, top
+from loss.distill import TopLogits, distill_loss_topk, top_logits
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def problem(P, V, k, seed=0, dtype=F32, ignored=0.0, T=1.0, values_dtype=None):
+    g = torch.Generator().manual_seed(seed)
+    t = (2.5 * torch.randn(P, V, generator=g)).to(dtype)
+    z = (0.5 * t.float() + 1.5 * torch.randn(P, V, generator=g)).to(dtype)
+    values, indices = torch.topk(t.float(), k, 1)
+    lse = torch.logsumexp(t.float() / T, 1)
+    indices = indices.to(torch.int32)
+    if ignored:
+        indices[torch.rand(P, generator=g) < ignored] = -1
+    return z, values.to(values_dtype or dtype), indices, lse
+
+
+def check(z, values, indices, lse, T, weight=1.0, dim=1, upstream=1.0, cuda=None, gtol_extra=0.0):
+    """All reductions, loss and gradient, of [P, V] problems; `cuda` turns the host logits into the device tensor to be used."""
+    cuda = cuda or (lambda x: x.cuda())
+    loss, grad, counted, lerr, gerr = loss_and_gradient(z, values, indices, lse, T, weight)
+    n = max(1, int(counted.sum()))
+    target = TopLogits(values.cuda(), indices.cuda(), None if lse is None else lse.cuda())
+    eps = half_step(z.dtype) + gtol_extra
+    for reduction, scale in (("mean", 1.0 / n), ("sum", 1.0), ("none", 1.0)):
+        x = cuda(z).detach().requires_grad_()
+        got = distill_loss_topk(x, target, temperature=T, reduction=reduction, weight=weight, dim=dim)
+        assert got.dtype == F32
+        want, tol = (loss, lerr) if reduction == "none" else (loss.sum() * scale, lerr.sum() * scale)
+        err = (got.detach().double().cpu() - want).abs()
+        assert bool((err <= tol + 2.0 ** -23 * want.abs()).all()), (reduction, float(err.max()), float(tol.max()))
+        (got * upstream).sum().backward()
+        g = x.grad.double().cpu()
+        # the gradient's rounding to its type; once more to fp32 and for the scale factors before it
+        bound = scale * abs(upstream) * (gerr + (eps + 2.0 ** -21) * grad.abs())
+        err = (g - grad * (scale * upstream)).abs()
+        # below the smallest normal number the type's step is fixed, tiny * eps (fp16: 2^-14 * 2^-10 = 2^-24): half of it
+        fixed = max(2.0 ** -133, torch.finfo(z.dtype).tiny * half_step(z.dtype))
+        assert x.grad.dtype == z.dtype and bool((err <= bound + fixed).all()), (reduction, float((err - bound).max()))
+        with torch.no_grad():
+            again = distill_loss_topk(x, target, temperature=T, reduction=reduction, weight=weight, dim=dim)
+        assert torch.equal(again, got.detach())
+
+
+# every tier of the rows (one wave, 256 and 1024 threads, in registers or read twice), rows that end inside a 16-byte piece, and the
+# thread-per-position kernel (up to 8 classes)
+WIDTHS = [1, 2, 3, 5, 8, 9, 31, 64, 80, 127, 255, 256, 257, 512, 513, 1000, 1025, 2047, 4096, 4097, 8191, 8193, 16383, 16385, 32767, 32769, 65535, 65537, 131071, 131073]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", WIDTHS)
+def test_rows(V, dtype):
+    k = min(V, 1 + V % 13, 64)
+    z, values, indices, lse = problem(5, V, k, seed=V, dtype=dtype, ignored=0.25, T=2.0)
+    check(z, values, indices, lse, 2.0)
+    check(z, values, indices, None, 1.0, weight=0.5)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V,k", [(70, 64), (64, 64), (5000, 64), (40, 40), (6, 6)])
+def test_many_entries(V, k, dtype):
+    z, values, indices, lse = problem(6, V, k, seed=k, dtype=dtype, T=1.5)
+    check(z, values, indices, lse, 1.5)
+    check(z, values, indices, None, 1.5)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [6, 100, 3001])
+def test_entries_that_repeat_or_do_not_exist(V, dtype):
+    z, values, indices, lse = problem(6, V, 5, seed=V, dtype=dtype)
+    indices[0, :3] = indices[0, 3]                       # four entries of one class
+    indices[1] = torch.tensor([-1, V, -(1 << 31), (1 << 31) - 1, 2], dtype=torch.int32)
+    indices[2] = indices[2, 0]
+    indices[3, 1:] = V
+    indices[4] = -7
+    lse = lse + 2.0                                      # keeps the sum of the p below 1 where entries repeat
+    check(z, values, indices, lse, 1.0)
+    check(z, values, indices, None, 1.0)
+    wide = indices.to(torch.int64)
+    wide[5, 0] += 1 << 32                                # no class, although its low half is one
+    check(z, values, wide, lse, 1.0)
+    values[0, 0] = -math.inf                             # a kept class without mass
+    values[2] = torch.finfo(dtype).min
+    check(z, values, indices, lse, 1.0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [7, 90, 1500, 70001])
+def test_masked_logits(V, dtype):
+    z, values, indices, lse = problem(6, V, 4, seed=V, dtype=dtype)
+    kept = torch.zeros(6, V, dtype=torch.bool).scatter_(1, indices.long(), True)
+    g = torch.Generator().manual_seed(1)
+    mask = (torch.rand(6, V, generator=g) < 0.5) & ~kept
+    mask[:, (~kept).float().argmax(1)] = False           # one class outside stays
+    mask &= ~kept
+    for low in (-math.inf, float(torch.finfo(dtype).min)):
+        y = torch.where(mask, torch.tensor(low, dtype=dtype), z)
+        # the lowest value takes no part in sums; the bounds go by the logits that do
+        loss, grad, counted, lerr, gerr = loss_and_gradient(torch.where(mask, torch.tensor(-math.inf, dtype=dtype), z), values, indices, lse, 1.0)
+        x = y.cuda().requires_grad_()
+        got = distill_loss_topk(x, TopLogits(values.cuda(), indices.cuda(), lse.cuda()), reduction="none")
+        assert bool(((got.detach().double().cpu() - loss).abs() <= lerr + 2.0 ** -23 * loss).all())
+        got.sum().backward()
+        err = (x.grad.double().cpu() - grad).abs()
+        assert bool((err <= gerr + (half_step(dtype) + 2.0 ** -21) * grad.abs()).all()) and not x.grad.cpu()[mask].any()
+    # everything outside the kept classes masked: the student gives them nothing
+    y = torch.where(kept, z, torch.tensor(-math.inf, dtype=dtype))
+    check(y, values, indices, None, 1.0)
+    x = y.cuda()
+    got = distill_loss_topk(x, TopLogits(values.cuda(), indices.cuda(), lse.cuda()), reduction="none")
+    assert torch.isinf(got).all()                        # the teacher gave them something
+    # one NaN or infinity spoils its own row only
+    for bad in (math.nan, math.inf):
+        y = z.clone()
+        y[2, (~kept[2]).float().argmax()] = bad
+        x = y.cuda().requires_grad_()
+        got = distill_loss_topk(x, TopLogits(values.cuda(), indices.cuda(), lse.cuda()), reduction="none")
+        got.sum().backward()
+        others = [i for i in range(6) if i != 2]
+        assert torch.isnan(got[2]) and torch.isnan(x.grad[2]).any() and torch.isfinite(got[others]).all() and torch.isfinite(x.grad[others]).all()
+
+
+def test_rows_without_entries_are_not_read():
+    z, values, indices, lse = problem(4, 1000, 4)
+    z[1] = math.nan
+    indices[1] = -1
+    x = z.cuda().requires_grad_()
+    loss = distill_loss_topk(x, TopLogits(values.cuda(), indices.cuda(), lse.cuda()))
+    loss.backward()
+    assert torch.isfinite(loss) and not x.grad[1].any() and x.grad[0].any()
+    x = z.cuda().requires_grad_()
+    loss = distill_loss_topk(x, TopLogits(values.cuda(), torch.full_like(indices, 1000).cuda(), None))
+    loss.backward()
+    assert float(loss.detach()) == 0 and not x.grad.any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N,C,side,k", [(2, 4, 8, 2), (1, 3, 7, 3), (2, 8, 6, 4), (3, 7, 12, 2), (1, 16, 5, 5), (2, 21, 9, 3), (1, 32, 4, 32), (2, 33, 3, 4), (1, 2, 64, 1), (1, 1, 6, 1)])
+def test_planes(N, C, side, k, dtype):
+    z, values, indices, lse = problem(N * side * side, C, k, seed=C, dtype=dtype, ignored=0.2, T=2.0)
+    planes = lambda t: t.view(N, side, side, -1).permute(0, 3, 1, 2).contiguous()  # noqa: E731
+    loss, grad, counted, lerr, gerr = loss_and_gradient(z, values, indices, lse, 2.0)
+    n = max(1, int(counted.sum()))
+    target = TopLogits(planes(values).cuda(), planes(indices).cuda(), lse.view(N, side, side).cuda())
+    for form in (lambda t: t, lambda t: t.to(memory_format=torch.channels_last), lambda t: torch.nn.functional.pad(t, (0, 3))[..., :side]):
+        for reduction, scale in (("mean", 1 / n), ("sum", 1.0), ("none", 1.0)):
+            x = form(planes(z).cuda()).detach().requires_grad_()
+            got = distill_loss_topk(x, target, temperature=2.0, reduction=reduction)
+            want, tol = (loss.view(N, side, side), lerr.view(N, side, side)) if reduction == "none" else (loss.sum() * scale, lerr.sum() * scale)
+            assert got.shape == want.shape and bool(((got.detach().double().cpu() - want).abs() <= tol + 2.0 ** -23 * want.abs()).all())
+            got.sum().backward()
+            g = x.grad.permute(0, 2, 3, 1).reshape(-1, C).double().cpu()
+            assert bool(((g - grad * scale).abs() <= scale * (gerr + (half_step(dtype) + 2.0 ** -21) * grad.abs()) + 2.0 ** -133).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [5, 77, 1030, 9001])
+def test_strides_offsets_and_dimensions(V, dtype):
+    z, values, indices, lse = problem(6, V, 3, seed=V, dtype=dtype)
+    wide = lambda x: torch.nn.functional.pad(x, (3, 2), value=9.0).cuda()[:, 3:-2]   # noqa: E731  rows that begin anywhere
+    check(z, values, indices, lse, 1.0, cuda=wide)
+    check(z, values, indices, lse, 1.0, cuda=lambda x: x.t().contiguous().cuda().t())          # classes strided
+    x = z.view(2, 3, V).cuda().requires_grad_()
+    y = z.cuda().requires_grad_()
+    target = TopLogits(values.cuda(), indices.cuda(), lse.cuda())
+    a = distill_loss_topk(x, TopLogits(target.values.view(2, 3, 3), target.indices.view(2, 3, 3), target.lse.view(2, 3)), dim=-1)
+    b = distill_loss_topk(y, target)
+    (a + b).backward()
+    assert torch.equal(a, b) and torch.equal(x.grad.view(6, V), y.grad)
+    one = z[:1].expand(6, V).cuda()                                                              # stride 0
+    same = TopLogits(target.values[:1].expand(6, 3), target.indices[:1].expand(6, 3), target.lse[:1].expand(6))
+    alone = distill_loss_topk(one[:1], TopLogits(target.values[:1], target.indices[:1], target.lse[:1]), reduction="none")
+    assert torch.equal(distill_loss_topk(one, same, reduction="none"), alone.expand(6))
+
+
+def test_half_precision_logits_and_values_types():
+    z, values, indices, lse = problem(4, 333, 6, dtype=torch.float16)
+    check(z, values, indices, lse, 1.0)
+    z, values, indices, lse = problem(4, 333, 6, dtype=BF16, values_dtype=F32)
+    check(z, values, indices.long(), lse, 1.0)
+    with pytest.raises(TypeError, match="float32 or bfloat16"):
+        distill_loss_topk(z.double().cuda(), TopLogits(values.cuda(), indices.cuda(), None))
+    with pytest.raises(ValueError, match="same device"):
+        distill_loss_topk(z.cuda(), TopLogits(values, indices, None))
+
+
+@pytest.mark.parametrize("shape", [(7, 50), (3, 4, 8, 8), (5, 3000)])
+def test_upstream_gradients_and_a_second_backward_pass(shape):
+    C = shape[1]
+    P = math.prod(shape) // C
+    z, values, indices, lse = problem(P, C, 3, T=2.0)
+    to = lambda t, c: t.view(shape[0], *shape[2:], c).movedim(-1, 1).contiguous().cuda() if len(shape) > 2 else t.view(-1, c).cuda()  # noqa: E731
+    target = TopLogits(to(values, 3), to(indices, 3), lse.view(shape[0], *shape[2:]).cuda())
+    if len(shape) == 2:
+        check(z, values, indices, lse, 2.0, upstream=-3.0)
+    for reduction in ("mean", "sum", "none"):
+        x = to(z, C).requires_grad_()
+        loss = distill_loss_topk(x, target, temperature=2.0, reduction=reduction)
+        total = loss.sum()
+        g1, = torch.autograd.grad(total, x, retain_graph=True)
+        keep = g1.clone()
+        g2, = torch.autograd.grad(total, x, retain_graph=True)
+        g3, = torch.autograd.grad(2 * total, x)              # a power of two: exact
+        assert torch.equal(keep, g2) and torch.equal(2 * keep, g3) and torch.equal(keep, g1)
+    x = to(z, C).requires_grad_()
+    w = torch.rand(target.lse.shape, device="cuda")
+    (distill_loss_topk(x, target, temperature=2.0, reduction="none") * w).sum().backward()
+    y = to(z, C).requires_grad_()
+    g, = torch.autograd.grad(distill_loss_topk(y, target, temperature=2.0, reduction="sum"), y)
+    # T (M q - p) is a difference of two products of at most T = 2 each, whose factors (weight, T, upstream, 1 / sum) are multiplied in
+    # another order: up to four roundings of 2^-24 * 2 on either side of the difference and on either side of this comparison
+    torch.testing.assert_close(x.grad, g * w.unsqueeze(1), rtol=2.0 ** -20, atol=2 * 2 * 4 * 2.0 ** -24 * 2)
+
+
+def test_gradient_against_differences_of_the_definition():
+    z, values, indices, lse = problem(5, 400, 7, T=1.5)
+    x = z.cuda().requires_grad_()
+    distill_loss_topk(x, TopLogits(values.cuda(), indices.cuda(), lse.cuda()), temperature=1.5, reduction="sum").backward()
+    _, _, _, _, gerr = loss_and_gradient(z, values, indices, lse, 1.5)
+    g = torch.Generator().manual_seed(2)
+    for _ in range(3):
+        d = torch.randn(z.shape, generator=g, dtype=torch.float64)
+        up, down = (loss_and_gradient(z.double() + s * 1e-5 * d, values, indices, lse, 1.5)[0].sum() for s in (1, -1))
+        got = float((x.grad.double().cpu() * d).sum())
+        # central difference: 1e-10 times third derivatives, 1e-16 * loss / 1e-5
+        assert abs(float(up - down) / 2e-5 - got) <= float((gerr * d.abs()).sum()) + 2.0 ** -23 * abs(got) + 1e-7
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", WIDTHS)
+def test_top_rows(V, dtype):
+    g = torch.Generator().manual_seed(V)
+    z = (3 * torch.randn(4, V, generator=g)).to(dtype)
+    for k in {1, min(V, 5), min(V, 64)}:
+        for x in (z.cuda(), torch.nn.functional.pad(z, (1, 4)).cuda()[:, 1:-4]):
+            values, indices, lse = top_logits(x, k, temperature=2.0)
+            host = top_logits(z, k, temperature=2.0)
+            assert torch.equal(values.cpu(), host.values) and torch.equal(indices.cpu(), host.indices) and values.dtype == dtype
+            want = torch.logsumexp(z.double() / 2, 1)
+            # exp arguments up to 1.45 * |z| / 2 in base 2, log of the sum: as derived for the loss
+            assert bool(((lse.double().cpu() - want).abs() <= 2.0 ** -21 * (8 + 3 * z.double().abs().amax(1) / 2)).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [8, 70, 700, 5000, 40000, 140000])
+def test_top_rows_where_order_is_hard(V, dtype):
+    g = torch.Generator().manual_seed(V)
+    rows = [torch.zeros(V), torch.full((V,), -math.inf), torch.full((V,), torch.finfo(dtype).min), torch.arange(V) / V, -torch.arange(V) / V,
+            torch.randint(0, 3, (V,), generator=g).float(), torch.randn(V, generator=g), torch.randn(V, generator=g), torch.randn(V, generator=g),
+            torch.where(torch.arange(V) % 2 == 0, 0.0, -0.0), -torch.rand(V, generator=g) - 1]
+    z = torch.stack(rows).to(dtype)
+    z[6, V // 2] = math.nan
+    z[6, V - 1] = math.nan
+    z[7, V // 3] = math.inf
+    z[8, : V - 2] = -math.inf
+    for k in {1, min(V, 3), min(V, 64)}:
+        values, indices, lse = top_logits(z.cuda(), k)
+        host = top_logits(z, k)
+        assert torch.equal(indices.cpu(), host.indices)
+        assert torch.equal(values.cpu().view(torch.int16 if dtype == BF16 else torch.int32), host.values.view(torch.int16 if dtype == BF16 else torch.int32))
+        assert float(lse[1]) == -math.inf and math.isnan(float(lse[6])) and abs(float(lse[0]) - math.log(V)) < 2.0 ** -20 * 12
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N,C,side", [(2, 4, 8), (1, 3, 5), (2, 8, 12), (1, 13, 7), (1, 32, 6), (2, 40, 5), (1, 1, 4)])
+def test_top_planes(N, C, side, dtype):
+    g = torch.Generator().manual_seed(C)
+    z = torch.randint(-3, 4, (N, C, side, side), generator=g).to(dtype) / 2          # ties everywhere
+    z[0, 0, 0, 0] = math.nan
+    for k in {1, min(C, 3), C}:
+        if k > 64:
+            continue
+        for x in (z.cuda(), z.cuda().to(memory_format=torch.channels_last)):
+            values, indices, lse = top_logits(x, k)
+            host = top_logits(z, k)
+            assert torch.equal(indices.cpu(), host.indices) and torch.equal(torch.nan_to_num(values.cpu(), 99.0), torch.nan_to_num(host.values, 99.0))
+            torch.testing.assert_close(lse.cpu(), host.lse, rtol=2.0 ** -20, atol=2.0 ** -20, equal_nan=True)
+
+
+def test_other_stream_and_captured_graph():
+    z, values, indices, lse = problem(64, 2000, 8, T=2.0)
+    target = TopLogits(values.cuda(), indices.cuda(), lse.cuda())
+
+    def step(x):
+        t = top_logits(x, 4, temperature=2.0)
+        loss = distill_loss_topk(x, target, temperature=2.0)
+        return (*t, loss, torch.autograd.grad(loss, x)[0])
+    x = z.cuda().requires_grad_()
+    want = [t.clone() for t in step(x)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [t.clone() for t in step(x)]
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    static = z.cuda().requires_grad_()
+    with torch.cuda.stream(side):
+        step(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(static)
+        graphs.append((g, out))
+    for seed in (5, 6, 7):
+        new = problem(64, 2000, 8, seed=seed)[0].cuda()
+        with torch.no_grad():
+            static.copy_(new)
+        want = [t.clone() for t in step(new.requires_grad_())]
+        for g, out in graphs:
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(want, out))
+
+
+def test_far_rows_of_a_large_tensor():
+    """Element offsets beyond 2^31."""
+    V, P = 131072, 16400
+    z = torch.zeros(P, V, dtype=BF16, device="cuda")
+    host = problem(3, V, 6, dtype=BF16)
+    z[-3:] = host[0].cuda()
+    values, indices, lse = top_logits(z, 6)
+    near = top_logits(z[-3:].clone(), 6)
+    assert torch.equal(values[-3:], near.values) and torch.equal(indices[-3:], near.indices) and torch.equal(lse[-3:], near.lse)
+    assert indices[:-3].cpu().eq(torch.arange(6, dtype=torch.int32)).all()
+    keep = TopLogits(torch.zeros(P, 6, device="cuda", dtype=BF16), torch.full((P, 6), -1, device="cuda"), torch.zeros(P, device="cuda"))
+    keep.values[-3:], keep.indices[-3:], keep.lse[-3:] = host[1].cuda(), host[2].cuda().long(), host[3].cuda()
+    x = z.requires_grad_()
+    g, = torch.autograd.grad(distill_loss_topk(x, keep), x)
+    y = z[-3:].detach().clone().requires_grad_()
+    w, = torch.autograd.grad(distill_loss_topk(y, TopLogits(*(t[-3:] for t in keep))), y)
+    assert torch.equal(g[-3:], w) and not g[:4].any() and not g[-4].any()
