@@ -192,6 +192,130 @@ __global__ __launch_bounds__(256) void mxfp4_rows_kernel(const LinearArgs a) {
     }
 }
 
+// Many rows: a workgroup of WM x WN waves computes BM rows x BN outputs.  Two stages of LDS hold two slices (256 values, 128 bytes a
+// row) of both operands; the next stage is filled by LDS DMA while the matrix instructions run on the present one, with one barrier
+// a stage.  The eight 16-byte blocks of a row lie at block ^ (row % 8), which spreads the 16 rows of a fragment over all banks; the
+// DMA writes LDS in lane order, so the permutation is applied to its source addresses.  Scales: LDS [row][2] dwords, the two slices
+// of the stage; a lane takes the byte of its block by a shift.
+template <int BM, int BN> struct TileLds {
+    static constexpr int kData = (BM + BN) * 128, kScale = (BM + BN) * 8, kStage = kData + kScale;
+};
+
+// 16 (4) bytes per lane from base + off to lds_addr + 16 (4) * lane, invisible to the compiler's dependence tracking: the kernel
+// waits for them itself before the barrier that publishes the stage.  lds_addr and base are the same for the whole wave.
+__device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t lds_addr) {
+    uint32_t keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(off), "s"(base), "s"(lds_addr) : "memory");
+}
+__device__ __forceinline__ void dma4(const void* base, uint32_t off, uint32_t lds_addr) {
+    uint32_t keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(off), "s"(base), "s"(lds_addr) : "memory");
+}
+
+template <typename TO, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM * WN * 64, (WM * WN * 64 >= 512 ? 2 : 0)) void mxfp4_tile_kernel(const LinearArgs a, int tiles_m, int tiles_n) {
+    constexpr int W = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
+    constexpr int kStage = TileLds<BM, BN>::kStage, kData = TileLds<BM, BN>::kData;
+    constexpr int kLoads = (BM + BN) / 8 / W, kScaleLoads = (BM + BN) * 2 / 64 / W;
+    static_assert((BM + BN) % (8 * W) == 0 && BN % 8 == 0 && (BM + BN) * 2 % (64 * W) == 0 && BN % 32 == 0, "whole DMA transfers per wave");
+    extern __shared__ __align__(16) char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
+
+    // Workgroups go to the 8 XCDs in turn: each XCD takes one contiguous eighth of the tiles, and walks it in stripes of 8 tiles
+    // along n so that the tiles in flight on its 32 CUs share rows of both operands in its L2.
+    const int total = tiles_m * tiles_n, per = total / 8, extra = total % 8;
+    const int xcd = blockIdx.x % 8, pos = blockIdx.x / 8;
+    const int t = xcd * per + (xcd < extra ? xcd : extra) + pos;
+    const int stripe = t / (8 * tiles_m), within = t - stripe * 8 * tiles_m, width = tiles_n - stripe * 8 < 8 ? tiles_n - stripe * 8 : 8;
+    const int64_t m0 = (int64_t)(within / width) * BM, n0 = (int64_t)(stripe * 8 + within % width) * BN;
+
+    // rows of the stage: 0..BN-1 weights, BN..BN+BM-1 inputs; a wave's transfer i moves rows (i*W + wave)*8 .. +8
+    const int block = (lane & 7) ^ (lane >> 3);                 // source block of this lane's LDS slot (rows of a transfer start at multiples of 8)
+    uint32_t off[kLoads], soff[kScaleLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const int row = (i * W + wave) * 8 + (lane >> 3);
+        const int64_t last = row < BN ? a.N - 1 - n0 : a.M - 1 - m0, rel = row < BN ? row : row - BN;
+        off[i] = (uint32_t)((rel < last ? rel : last) * a.ldc + block * 16);
+    }
+#pragma unroll
+    for (int i = 0; i < kScaleLoads; ++i) {
+        const int row = (i * W + wave) * 32 + (lane >> 1);
+        const bool w = row < BN;
+        const int64_t last = w ? a.N - 1 - n0 : a.M - 1 - m0, rel = w ? row : row - BN;
+        soff[i] = (uint32_t)((rel < last ? rel : last) * 4 + (lane & 1) * (w ? a.N : a.M) * 4);
+    }
+    const uint8_t *wp = a.w + n0 * a.ldc, *xp = a.x + m0 * a.ldc;
+    const uint32_t *wsp = a.ws + n0, *xsp = a.xs + m0;
+    const uint32_t lds0 = (uint32_t)(size_t)(const __attribute__((address_space(3))) char*)lds;
+    auto fill = [&](int step) {                                  // slices 2 step, 2 step + 1 (the second of them only if there is one)
+        const bool half = 2 * step + 1 >= a.slices;
+        const uint32_t at = lds0 + (step & 1) * kStage;
+        const uint32_t back = half ? (block & 4) * 16 : 0;       // no second slice: its slots take the first one's blocks and are not read
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int first = (i * W + wave) * 8;
+            dma16(first < BN ? wp + (int64_t)step * 128 : xp + (int64_t)step * 128, off[i] - back, at + first * 128);
+        }
+#pragma unroll
+        for (int i = 0; i < kScaleLoads; ++i) {
+            const int first = (i * W + wave) * 32;
+            const uint32_t sback = half ? (lane & 1) * (uint32_t)(first < BN ? a.N : a.M) * 4 : 0;
+            dma4(first < BN ? wsp + (int64_t)step * 2 * a.N : xsp + (int64_t)step * 2 * a.M, soff[i] - sback, at + kData + first * 8);
+        }
+    };
+
+    f32x4 acc[TN][TM];
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int j = 0; j < TM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int nw = (wave % WN) * TN * 16 + r, mw = BN + (wave / WN) * TM * 16 + r;      // this lane's first fragment rows
+    const int steps = (a.slices + 1) / 2;
+    fill(0);
+    for (int step = 0; step < steps; ++step) {
+        // this wave's transfers into the stage have landed, and its reads of the other stage, which is filled next, are done
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (step + 1 < steps) fill(step + 1);
+        const char* st = lds + (step & 1) * kStage;
+        uint64_t sw[TN], sx[TM];
+#pragma unroll
+        for (int i = 0; i < TN; ++i) sw[i] = *reinterpret_cast<const uint64_t*>(st + kData + (nw + i * 16) * 8);
+#pragma unroll
+        for (int j = 0; j < TM; ++j) sx[j] = *reinterpret_cast<const uint64_t*>(st + kData + (mw + j * 16) * 8);
+        auto half = [&](int h) {
+            u32x4 fw[TN], fx[TM];
+            const int slot = ((h * 4 + q) ^ (r & 7)) * 16;      // fragment rows are r modulo 16, so modulo 8 as well
+#pragma unroll
+            for (int i = 0; i < TN; ++i) fw[i] = *reinterpret_cast<const u32x4*>(st + (nw + i * 16) * 128 + slot);
+#pragma unroll
+            for (int j = 0; j < TM; ++j) fx[j] = *reinterpret_cast<const u32x4*>(st + (mw + j * 16) * 128 + slot);
+            uint32_t bw[TN], bx[TM];
+#pragma unroll
+            for (int i = 0; i < TN; ++i) bw[i] = (uint32_t)(sw[i] >> (32 * h)) >> (8 * q);
+#pragma unroll
+            for (int j = 0; j < TM; ++j) bx[j] = (uint32_t)(sx[j] >> (32 * h)) >> (8 * q);
+#pragma unroll
+            for (int i = 0; i < TN; ++i)
+#pragma unroll
+                for (int j = 0; j < TM; ++j) acc[i][j] = mfma_fp4(fw[i], fx[j], acc[i][j], bw[i], bx[j]);
+        };
+        half(0);
+        if (2 * step + 1 < a.slices) half(1);
+    }
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+            const int64_t n = n0 + (wave % WN) * TN * 16 + i * 16 + 4 * q;
+            if (n < a.N) store_outputs<TO>(a, m0 + (wave / WN) * TM * 16 + j * 16 + r, n, acc[i][j]);
+        }
+}
+
 // ------------------------------------------------------------------------------------------------ host
 static int64_t slices_of(int64_t cols) { return (cols + kSlice - 1) / kSlice; }
 
@@ -228,6 +352,25 @@ static int quantize(int dtype, const void* x, int64_t ld, int64_t rows, int64_t 
         SEGK_LAUNCH_CHECK();
         return SEGK_OK;
     });
+}
+
+template <typename TO, int BM, int BN, int WM, int WN> static int launch_tile(const LinearArgs& a, hipStream_t st) {
+    constexpr int bytes = 2 * TileLds<BM, BN>::kStage;
+    const int64_t tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN;
+    SEGK_REQUIRE(tm * tn < (1ll << 31), SEGK_ESHAPE, "mxfp4_linear: too many tiles");
+    auto kernel = mxfp4_tile_kernel<TO, BM, BN, WM, WN>;
+    if (bytes > 65536) SEGK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(WM * WN * 64), bytes, st, a, (int)tm, (int)tn);
+    SEGK_LAUNCH_CHECK();
+    return SEGK_OK;
+}
+
+static int pick_tile(int64_t M, int64_t N) {
+    if (M <= 32) return 16;
+    for (int t : {256, 128}) {
+        if (((M + t - 1) / t) * ((N + t - 1) / t) >= 256) return t;
+    }
+    return 64;
 }
 
 }  // namespace segk
@@ -269,7 +412,7 @@ extern "C" int segk_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const 
                                  const void* w_codes, const void* w_scales, int64_t N, const float* bias, void* y, int y_dtype, int64_t ldy,
                                  void* workspace, size_t workspace_bytes, int dev, void* stream) {
     SEGK_REQUIRE((x != nullptr) != (x_codes != nullptr), SEGK_EINVAL, "mxfp4_linear: either x or x_codes is given");
-    SEGK_REQUIRE(M > 0 && K > 0 && N > 0 && M < (1ll << 31) && N < (1ll << 31) && K < (1ll << 30), SEGK_ESHAPE, "mxfp4_linear: bad shape");
+    SEGK_REQUIRE(M > 0 && K > 0 && N > 0 && M < (1ll << 28) && N < (1ll << 28) && K < (1ll << 24), SEGK_ESHAPE, "mxfp4_linear: bad shape");
     if (const int rc = check_matrix("mxfp4_linear", y_dtype, y, ldy, M, N)) return rc;
     if (const int rc = check_packed("mxfp4_linear", w_codes, w_scales)) return rc;
     if (x) {
@@ -289,8 +432,13 @@ extern "C" int segk_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const 
     a.w = (const uint8_t*)w_codes; a.ws = (const uint32_t*)w_scales; a.x = (const uint8_t*)x_codes; a.xs = (const uint32_t*)x_scales;
     a.bias = bias; a.y = y; a.M = M; a.N = N; a.ldc = slices_of(K) * 64; a.ldy = ldy; a.slices = (int)slices_of(K);
     a.vec = reinterpret_cast<uintptr_t>(y) % (4 * esize(y_dtype)) == 0 && ldy % 4 == 0;
-    SEGK_DISPATCH_DTYPE(y_dtype, TO, hipLaunchKernelGGL((mxfp4_rows_kernel<TO>), dim3((unsigned)((N + 15) / 16), (unsigned)((M + 15) / 16)), dim3(256),
-                                                        0, st, a));
+    const int choice = pick_tile(M, N);
+    SEGK_DISPATCH_DTYPE(y_dtype, TO, {
+        if (choice == 256) return launch_tile<TO, 256, 256, 2, 4>(a, st);
+        if (choice == 128) return launch_tile<TO, 128, 128, 2, 2>(a, st);
+        if (choice == 64) return launch_tile<TO, 64, 64, 2, 2>(a, st);
+        hipLaunchKernelGGL((mxfp4_rows_kernel<TO>), dim3((unsigned)((N + 15) / 16), (unsigned)((M + 15) / 16)), dim3(256), 0, st, a);
+    });
     SEGK_LAUNCH_CHECK();
     return SEGK_OK;
 }
