@@ -8,6 +8,7 @@
 //     scales [slices][rows][4 bytes]: the four scales of a row's slice are one dword, and those of neighbouring rows are
 //            neighbours, so a tile of rows gets its scales with coalesced loads
 #include "common.h"
+#include <type_traits>
 
 namespace segk {
 
@@ -81,7 +82,7 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
 // per thread, both coalesced.
 template <typename T>
 __global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const T* __restrict__ x, int64_t ld, int cols, uint32_t items, Divide per_row,
-                                                             int64_t rows, int64_t row0, uint32_t* __restrict__ codes,
+                                                             int64_t scale_rows, int64_t row0, uint32_t* __restrict__ codes,
                                                              uint32_t* __restrict__ scales) {
     const uint32_t item = blockIdx.x * 256u + threadIdx.x;
     if (item >= items) return;                                     // items are whole slices: a group of 16 lanes leaves together
@@ -107,7 +108,7 @@ __global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const T* __restrict
     codes[row * per_row.d + i] = pack_codes(v);
     const int lane = threadIdx.x & 63;
     const uint32_t b1 = __shfl(byte, (lane & 48) + 4, 64), b2 = __shfl(byte, (lane & 48) + 8, 64), b3 = __shfl(byte, (lane & 48) + 12, 64);
-    if ((i & 15u) == 0) scales[(int64_t)(i >> 4) * rows + row] = byte | (b1 << 8) | (b2 << 16) | (b3 << 24);
+    if ((i & 15u) == 0) scales[(int64_t)(i >> 4) * scale_rows + row] = byte | (b1 << 8) | (b2 << 16) | (b3 << 24);
 }
 
 template <typename T>
@@ -151,13 +152,13 @@ struct LinearArgs {
     const uint32_t* xs;
     const float* bias;
     void* y;
-    int64_t M, N, ldc, ldy;
-    int slices, vec;             // vec: four neighbouring outputs may be stored at once
+    int64_t M, N, ldc, ldy, xs_rows;      // xs_rows: rows from one slice to the next in xs
+    int slices, vec;             // vec: so many neighbouring outputs, from a column that is a multiple of it, may be stored at once (0: one)
 };
 
 template <typename TO>
 __device__ __forceinline__ void store_outputs(const LinearArgs& a, int64_t m, int64_t n, const f32x4 acc) {
-    if (m >= a.M) return;
+    if (m >= a.M || n >= a.N) return;
     TO* y = static_cast<TO*>(a.y) + m * a.ldy + n;
     float v[4];
 #pragma unroll
@@ -167,6 +168,41 @@ __device__ __forceinline__ void store_outputs(const LinearArgs& a, int64_t m, in
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             if (n + i < a.N) y[i] = Elem<TO>::from_f(v[i]);
+}
+
+// Row m of a wave's tile: lane group q holds outputs n + i*16 + 4q .. +3 for the TN fragments i.  bf16: the lane groups of two
+// fragments exchange halves so that a lane stores 8 neighbouring outputs, and a store covers 64 instead of 32 bytes of each row.
+template <typename TO, int TN, int TM>
+__device__ __forceinline__ void store_rows(const LinearArgs& a, int64_t m, int64_t n, int q, const f32x4 (&acc)[TN][TM], int j) {
+    if constexpr (sizeof(TO) == 2 && TN % 2 == 0) {
+        if (a.vec == 8 && n + TN * 16 <= a.N) {
+#pragma unroll
+            for (int i = 0; i < TN; i += 2) {
+                uint32_t w[2][2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    f32x4 v = acc[i + h][j];
+                    if (a.bias) {
+                        const float* b = a.bias + n + (i + h) * 16 + 4 * q;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] += b[e];
+                    }
+                    const bf16x4 o = {(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
+                    const uint2 u = __builtin_bit_cast(uint2, o);
+                    w[h][0] = u.x;
+                    w[h][1] = u.y;
+                }
+                // after the swap of odd 16-lane rows of fragment i with even ones of fragment i + 1, group q holds columns
+                // (q / 2) * 8 .. +7 of fragment i + q % 2: the first half in [0], the second in [1]
+                const auto lo = __builtin_amdgcn_permlane16_swap(w[0][0], w[1][0], false, false), hi = __builtin_amdgcn_permlane16_swap(w[0][1], w[1][1], false, false);
+                if (m < a.M)
+                    *reinterpret_cast<u32x4*>(static_cast<bf16*>(a.y) + m * a.ldy + n + (i + (q & 1)) * 16 + (q >> 1) * 8) = u32x4{lo[0], hi[0], lo[1], hi[1]};
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < TN; ++i) store_outputs<TO>(a, m, n + i * 16 + 4 * q, acc[i][j]);
 }
 
 // Few rows: a workgroup computes 16 outputs of 16 rows, its four waves share the slices.  Operands go straight from memory to the
@@ -180,7 +216,7 @@ __global__ __launch_bounds__(256) void mxfp4_rows_kernel(const LinearArgs a) {
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     for (int s = wave; s < a.slices; s += 4) {
         const u32x4 wv = *reinterpret_cast<const u32x4*>(wp + (int64_t)s * 64), xv = *reinterpret_cast<const u32x4*>(xp + (int64_t)s * 64);
-        const uint32_t sw = a.ws[(int64_t)s * a.N + n] >> (8 * q), sx = a.xs[(int64_t)s * a.M + m] >> (8 * q);
+        const uint32_t sw = a.ws[(int64_t)s * a.N + n] >> (8 * q), sx = a.xs[(int64_t)s * a.xs_rows + m] >> (8 * q);
         acc = mfma_fp4(wv, xv, acc, sw, sx);
     }
     __shared__ f32x4 part[4][64];
@@ -193,127 +229,163 @@ __global__ __launch_bounds__(256) void mxfp4_rows_kernel(const LinearArgs a) {
 }
 
 // Many rows: a workgroup of WM x WN waves computes BM rows x BN outputs.  Two stages of LDS hold two slices (256 values, 128 bytes a
-// row) of both operands; the next stage is filled by LDS DMA while the matrix instructions run on the present one, with one barrier
-// a stage.  The eight 16-byte blocks of a row lie at block ^ (row % 8), which spreads the 16 rows of a fragment over all banks; the
-// DMA writes LDS in lane order, so the permutation is applied to its source addresses.  Scales: LDS [row][2] dwords, the two slices
-// of the stage; a lane takes the byte of its block by a shift.
+// row) of both operands and are filled by LDS DMA.  The eight 16-byte blocks of a row lie at block ^ (row % 8), which spreads the 16
+// rows of a fragment over all banks; the DMA writes LDS in lane order, so the permutation is applied to its source addresses.
+// Scales: LDS [slice of the stage][row] dwords, of which a lane reads the byte of its block.
+//
+// The loop is skewed: while the products of one slice run, every fragment register is refilled for the next slice as soon as its
+// last product has been issued, so the matrix pipe does not wait for LDS.  The one barrier of a stage stands between its two
+// slices: the second slice's fragments are in registers by then, so the stage may be overwritten behind it, and the next stage,
+// requested one stage earlier, has landed.  The transfers are spread over the products of the second slice.
 template <int BM, int BN> struct TileLds {
     static constexpr int kData = (BM + BN) * 128, kScale = (BM + BN) * 8, kStage = kData + kScale;
 };
 
 // 16 (4) bytes per lane from base + off to lds_addr + 16 (4) * lane, invisible to the compiler's dependence tracking: the kernel
 // waits for them itself before the barrier that publishes the stage.  lds_addr and base are the same for the whole wave.
+// M0 holds the LDS address; nothing else in this kernel uses it.
 __device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t lds_addr) {
-    uint32_t keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep) : "v"(off), "s"(base), "s"(lds_addr) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds_addr));
 }
 __device__ __forceinline__ void dma4(const void* base, uint32_t off, uint32_t lds_addr) {
-    uint32_t keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep) : "v"(off), "s"(base), "s"(lds_addr) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(lds_addr));
 }
 
-template <typename TO, int BM, int BN, int WM, int WN>
+template <typename TO, int BM, int BN, int WM, int WN, bool WIDE>
 __global__ __launch_bounds__(WM * WN * 64, (WM * WN * 64 >= 512 ? 2 : 0)) void mxfp4_tile_kernel(const LinearArgs a, int tiles_m, int tiles_n) {
-    constexpr int W = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
+    constexpr int W = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, kRows = BM + BN;
     constexpr int kStage = TileLds<BM, BN>::kStage, kData = TileLds<BM, BN>::kData;
-    constexpr int kLoads = (BM + BN) / 8 / W, kScaleLoads = (BM + BN) * 2 / 64 / W;
-    static_assert((BM + BN) % (8 * W) == 0 && BN % 8 == 0 && (BM + BN) * 2 % (64 * W) == 0 && BN % 32 == 0, "whole DMA transfers per wave");
+    // WIDE: the scales of 256 rows of a slice in one transfer (their rows come in fours), else of 64 rows.  With fewer transfers than
+    // waves some waves repeat another's: a branch around it would cost more.
+    constexpr int kScaleRows = WIDE ? 256 : 64, kScalePieces = kRows * 2 / kScaleRows;
+    constexpr int kLoads = kRows / 8 / W, kScaleLoads = (kScalePieces + W - 1) / W, kPieces = kLoads + kScaleLoads;
+    static_assert(BM % (8 * W) == 0 && BN % (8 * W) == 0 && BN % 64 == 0 && BM % 64 == 0 && kRows % kScaleRows == 0 && TM >= TN, "whole DMA transfers per wave");
     extern __shared__ __align__(16) char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
 
     // Workgroups go to the 8 XCDs in turn: each XCD takes one contiguous eighth of the tiles, and walks it in stripes of 8 tiles
     // along n so that the tiles in flight on its 32 CUs share rows of both operands in its L2.
-    const int total = tiles_m * tiles_n, per = total / 8, extra = total % 8;
-    const int xcd = blockIdx.x % 8, pos = blockIdx.x / 8;
-    const int t = xcd * per + (xcd < extra ? xcd : extra) + pos;
+    const int total = tiles_m * tiles_n, per = total / 8, extra = total % 8, xcd = blockIdx.x % 8;
+    const int t = xcd * per + (xcd < extra ? xcd : extra) + blockIdx.x / 8;
     const int stripe = t / (8 * tiles_m), within = t - stripe * 8 * tiles_m, width = tiles_n - stripe * 8 < 8 ? tiles_n - stripe * 8 : 8;
     const int64_t m0 = (int64_t)(within / width) * BM, n0 = (int64_t)(stripe * 8 + within % width) * BN;
 
-    // rows of the stage: 0..BN-1 weights, BN..BN+BM-1 inputs; a wave's transfer i moves rows (i*W + wave)*8 .. +8
-    const int block = (lane & 7) ^ (lane >> 3);                 // source block of this lane's LDS slot (rows of a transfer start at multiples of 8)
+    // rows of the stage: 0..BN-1 weights, BN..BN+BM-1 inputs (beyond the last row: the last row again, never stored)
+    const int block = (lane & 7) ^ (lane >> 3);                 // source block of this lane's slot (rows of a transfer start at multiples of 8)
+    // an odd last slice comes as the second of its stage, behind its predecessor, which is not used again; a single slice takes both places
+    const int last_slice = a.slices > 1 ? a.slices - 2 : 0, span = a.slices > 1 ? 1 : 0;
+    const uint32_t fold = span ? 0 : (block & 4) * 16;
     uint32_t off[kLoads], soff[kScaleLoads];
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-        const int row = (i * W + wave) * 8 + (lane >> 3);
-        const int64_t last = row < BN ? a.N - 1 - n0 : a.M - 1 - m0, rel = row < BN ? row : row - BN;
-        off[i] = (uint32_t)((rel < last ? rel : last) * a.ldc + block * 16);
-    }
-#pragma unroll
-    for (int i = 0; i < kScaleLoads; ++i) {
-        const int row = (i * W + wave) * 32 + (lane >> 1);
-        const bool w = row < BN;
-        const int64_t last = w ? a.N - 1 - n0 : a.M - 1 - m0, rel = w ? row : row - BN;
-        soff[i] = (uint32_t)((rel < last ? rel : last) * 4 + (lane & 1) * (w ? a.N : a.M) * 4);
-    }
+    const uint32_t* sp[kScaleLoads];        // scales of this wave's transfers in the first slice
     const uint8_t *wp = a.w + n0 * a.ldc, *xp = a.x + m0 * a.ldc;
-    const uint32_t *wsp = a.ws + n0, *xsp = a.xs + m0;
+    const int last_n = (int)(a.N - 1 - n0 < BN ? a.N - 1 - n0 : BN), last_m = (int)(a.M - 1 - m0 < BM ? a.M - 1 - m0 : BM);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {                          // transfer i of this wave: rows (i*W + wave)*8 .. +8
+        const int row = (i * W + wave) * 8 + (lane >> 3);
+        const int rel = i * W * 8 < BN ? (row < last_n ? row : last_n) : (row - BN < last_m ? row - BN : last_m);
+        off[i] = (uint32_t)rel * (uint32_t)a.ldc + block * 16 - fold;
+    }
+#pragma unroll
+    for (int i = 0; i < kScaleLoads; ++i) {                     // kScaleRows rows of one slice
+        const int p = (i * W + wave) % kScalePieces, sub = p / (kRows / kScaleRows) * span, row = p % (kRows / kScaleRows) * kScaleRows;
+        const bool w = row < BN;
+        sp[i] = w ? a.ws + n0 + (int64_t)sub * a.N : a.xs + m0 + (int64_t)sub * a.xs_rows;
+        const int64_t left = (w ? a.N - n0 : a.xs_rows - m0) - kScaleRows / 64;
+        const int rel = (w ? row : row - BN) + lane * (kScaleRows / 64);
+        soff[i] = (uint32_t)(rel < left ? rel : (int)left) * 4;
+    }
     const uint32_t lds0 = (uint32_t)(size_t)(const __attribute__((address_space(3))) char*)lds;
-    auto fill = [&](int step) {                                  // slices 2 step, 2 step + 1 (the second of them only if there is one)
-        const bool half = 2 * step + 1 >= a.slices;
+    // piece i of this wave for the stage of slices 2 step and 2 step + 1
+    auto fill = [&](int step, int i) {
+        const int slice = 2 * step < last_slice ? 2 * step : last_slice;
         const uint32_t at = lds0 + (step & 1) * kStage;
-        const uint32_t back = half ? (block & 4) * 16 : 0;       // no second slice: its slots take the first one's blocks and are not read
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int first = (i * W + wave) * 8;
-            dma16(first < BN ? wp + (int64_t)step * 128 : xp + (int64_t)step * 128, off[i] - back, at + first * 128);
-        }
-#pragma unroll
-        for (int i = 0; i < kScaleLoads; ++i) {
-            const int first = (i * W + wave) * 32;
-            const uint32_t sback = half ? (lane & 1) * (uint32_t)(first < BN ? a.N : a.M) * 4 : 0;
-            dma4(first < BN ? wsp + (int64_t)step * 2 * a.N : xsp + (int64_t)step * 2 * a.M, soff[i] - sback, at + kData + first * 8);
+        if (i < kLoads) {
+            dma16((i * W * 8 < BN ? wp : xp) + slice * 64, off[i < kLoads ? i : 0], at + (i * W + wave) * 1024);
+        } else {
+            const int e = i < kLoads ? 0 : i - kLoads, p = (e * W + wave) % kScalePieces;
+            const int64_t rows = p % (kRows / kScaleRows) * kScaleRows < BN ? a.N : a.xs_rows;
+            if constexpr (WIDE) dma16(sp[e] + slice * rows, soff[e], at + kData + p * kScaleRows * 4);
+            else dma4(sp[e] + slice * rows, soff[e], at + kData + p * kScaleRows * 4);
         }
     };
 
     f32x4 acc[TN][TM];
-#pragma unroll
-    for (int i = 0; i < TN; ++i)
-#pragma unroll
-        for (int j = 0; j < TM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int nw = (wave % WN) * TN * 16 + r, mw = BN + (wave / WN) * TM * 16 + r;      // this lane's first fragment rows
+    const int nw = (wave % WN) * TN * 16, mw = BN + (wave / WN) * TM * 16;      // this wave's first fragment rows
     const int steps = (a.slices + 1) / 2;
-    fill(0);
-    for (int step = 0; step < steps; ++step) {
-        // this wave's transfers into the stage have landed, and its reads of the other stage, which is filled next, are done
+    u32x4 fw[2][TN], fx[TM];
+    uint32_t sw[2][TN], sx[TM];
+    auto publish = [&]() {       // this wave's transfers have landed and its reads are done; behind the barrier this holds for all waves
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (step + 1 < steps) fill(step + 1);
-        const char* st = lds + (step & 1) * kStage;
-        uint64_t sw[TN], sx[TM];
+    };
+    // The products of the fragments in set h; meanwhile the other set is refilled from slice `half` of stage `next`, and stage
+    // `ahead` is requested.
+    auto multiply = [&](auto h, int next, int half, auto request, int ahead) {
+        // fragment rows are r modulo 16, so r modulo 8 decides the slot
+        const char* d = lds + (next & 1) * kStage + r * 128 + ((half * 4 + q) ^ (r & 7)) * 16;
+        const char* c = lds + (next & 1) * kStage + kData + half * kRows * 4 + r * 4 + q;
 #pragma unroll
-        for (int i = 0; i < TN; ++i) sw[i] = *reinterpret_cast<const uint64_t*>(st + kData + (nw + i * 16) * 8);
+        for (int j = 0; j < TM; ++j) {
 #pragma unroll
-        for (int j = 0; j < TM; ++j) sx[j] = *reinterpret_cast<const uint64_t*>(st + kData + (mw + j * 16) * 8);
-        auto half = [&](int h) {
-            u32x4 fw[TN], fx[TM];
-            const int slot = ((h * 4 + q) ^ (r & 7)) * 16;      // fragment rows are r modulo 16, so modulo 8 as well
+            for (int i = 0; i < TN; ++i) acc[i][j] = mfma_fp4(fw[h()][i], fx[j], acc[i][j], sw[h()][i], sx[j]);
+            __builtin_amdgcn_sched_barrier(0);
+            fx[j] = *reinterpret_cast<const u32x4*>(d + (mw + j * 16) * 128);
+            sx[j] = *reinterpret_cast<const uint8_t*>(c + (mw + j * 16) * 4);
+            if (j < TN) {
+                fw[1 - h()][j] = *reinterpret_cast<const u32x4*>(d + (nw + j * 16) * 128);
+                sw[1 - h()][j] = *reinterpret_cast<const uint8_t*>(c + (nw + j * 16) * 4);
+            }
+            if constexpr (request()) {
 #pragma unroll
-            for (int i = 0; i < TN; ++i) fw[i] = *reinterpret_cast<const u32x4*>(st + (nw + i * 16) * 128 + slot);
+                for (int i = j * kPieces / TM; i < (j + 1) * kPieces / TM; ++i) fill(ahead, i);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    constexpr std::integral_constant<int, 0> first{};
+    constexpr std::integral_constant<int, 1> second{};
+    const bool odd = a.slices & 1;
 #pragma unroll
-            for (int j = 0; j < TM; ++j) fx[j] = *reinterpret_cast<const u32x4*>(st + (mw + j * 16) * 128 + slot);
-            uint32_t bw[TN], bx[TM];
+    for (int i = 0; i < kPieces; ++i) fill(0, i);
+    if (steps > 1) {
 #pragma unroll
-            for (int i = 0; i < TN; ++i) bw[i] = (uint32_t)(sw[i] >> (32 * h)) >> (8 * q);
-#pragma unroll
-            for (int j = 0; j < TM; ++j) bx[j] = (uint32_t)(sx[j] >> (32 * h)) >> (8 * q);
-#pragma unroll
-            for (int i = 0; i < TN; ++i)
-#pragma unroll
-                for (int j = 0; j < TM; ++j) acc[i][j] = mfma_fp4(fw[i], fx[j], acc[i][j], bw[i], bx[j]);
-        };
-        half(0);
-        if (2 * step + 1 < a.slices) half(1);
+        for (int i = 0; i < kPieces; ++i) fill(1, i);
     }
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
+        for (int j = 0; j < TM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    publish();
+    {
+        const char* d = lds + r * 128 + (q ^ (r & 7)) * 16;
+        const char* c = lds + kData + r * 4 + q;
+#pragma unroll
         for (int j = 0; j < TM; ++j) {
-            const int64_t n = n0 + (wave % WN) * TN * 16 + i * 16 + 4 * q;
-            if (n < a.N) store_outputs<TO>(a, m0 + (wave / WN) * TM * 16 + j * 16 + r, n, acc[i][j]);
+            fx[j] = *reinterpret_cast<const u32x4*>(d + (mw + j * 16) * 128);
+            sx[j] = *reinterpret_cast<const uint8_t*>(c + (mw + j * 16) * 4);
         }
+#pragma unroll
+        for (int i = 0; i < TN; ++i) {
+            fw[0][i] = *reinterpret_cast<const u32x4*>(d + (nw + i * 16) * 128);
+            sw[0][i] = *reinterpret_cast<const uint8_t*>(c + (nw + i * 16) * 4);
+        }
+    }
+    int step = 0;
+    for (; step + 2 < steps; ++step) {
+        multiply(first, step, 1, std::false_type{}, 0);
+        publish();
+        multiply(second, step + 1, step + 2 == steps && odd ? 1 : 0, std::true_type{}, step + 2);
+    }
+    for (; step < steps; ++step) {       // the last two stages; what is read ahead of the end is not used
+        multiply(first, step, 1, std::false_type{}, 0);
+        if (step + 1 == steps && odd) break;
+        publish();
+        multiply(second, step + 1, step + 2 == steps && odd ? 1 : 0, std::false_type{}, 0);
+    }
+    const int64_t m = m0 + (wave / WN) * TM * 16 + r, n = n0 + (wave % WN) * TN * 16;
+#pragma unroll
+    for (int j = 0; j < TM; ++j) store_rows<TO, TN, TM>(a, m + j * 16, n, q, acc, j);
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -343,22 +415,22 @@ template <typename F> static int by_rows(int64_t rows, int64_t per_row, F&& f) {
     return SEGK_OK;
 }
 
-static int quantize(int dtype, const void* x, int64_t ld, int64_t rows, int64_t cols, void* codes, void* scales, hipStream_t st) {
+static int quantize(int dtype, const void* x, int64_t ld, int64_t rows, int64_t cols, void* codes, void* scales, int64_t scale_rows, hipStream_t st) {
     const int64_t per_row = slices_of(cols) * 16;
     return by_rows(rows, per_row, [&](int64_t r0, int64_t n) -> int {
         const uint32_t items = (uint32_t)(n * per_row);
         SEGK_DISPATCH_DTYPE(dtype, T, hipLaunchKernelGGL((mxfp4_quantize_kernel<T>), dim3((items + 255) / 256), dim3(256), 0, st, (const T*)x, ld,
-                                                         (int)cols, items, Divide((uint32_t)per_row), rows, r0, (uint32_t*)codes, (uint32_t*)scales));
+                                                         (int)cols, items, Divide((uint32_t)per_row), scale_rows, r0, (uint32_t*)codes, (uint32_t*)scales));
         SEGK_LAUNCH_CHECK();
         return SEGK_OK;
     });
 }
 
-template <typename TO, int BM, int BN, int WM, int WN> static int launch_tile(const LinearArgs& a, hipStream_t st) {
+template <typename TO, int BM, int BN, int WM, int WN, bool WIDE> static int launch_tile(const LinearArgs& a, hipStream_t st) {
     constexpr int bytes = 2 * TileLds<BM, BN>::kStage;
     const int64_t tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN;
     SEGK_REQUIRE(tm * tn < (1ll << 31), SEGK_ESHAPE, "mxfp4_linear: too many tiles");
-    auto kernel = mxfp4_tile_kernel<TO, BM, BN, WM, WN>;
+    auto kernel = mxfp4_tile_kernel<TO, BM, BN, WM, WN, WIDE>;
     if (bytes > 65536) SEGK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
     hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(WM * WN * 64), bytes, st, a, (int)tm, (int)tn);
     SEGK_LAUNCH_CHECK();
@@ -384,7 +456,7 @@ extern "C" int segk_mxfp4_quantize(int dtype, const void* x, int64_t ld, int64_t
     if (const int rc = check_matrix("mxfp4_quantize", dtype, x, ld, rows, cols)) return rc;
     if (const int rc = check_packed("mxfp4_quantize", codes, scales)) return rc;
     SEGK_USE_DEVICE(dev);
-    return quantize(dtype, x, ld, rows, cols, codes, scales, (hipStream_t)stream);
+    return quantize(dtype, x, ld, rows, cols, codes, scales, rows, (hipStream_t)stream);
 }
 
 extern "C" int segk_mxfp4_dequantize(int dtype, const void* codes, const void* scales, int64_t rows, int64_t cols, void* y, int64_t ld, int dev,
@@ -405,7 +477,7 @@ extern "C" int segk_mxfp4_dequantize(int dtype, const void* codes, const void* s
 
 extern "C" size_t segk_mxfp4_linear_workspace(int64_t M, int64_t K, int64_t N) {
     (void)N;
-    return align_up(segk_mxfp4_codes_bytes(M, K), 16) + segk_mxfp4_scales_bytes(M, K);
+    return align_up(segk_mxfp4_codes_bytes(M, K), 16) + segk_mxfp4_scales_bytes((int64_t)align_up(M > 0 ? M : 0, 4), K);
 }
 
 extern "C" int segk_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const void* x_codes, const void* x_scales, int64_t M, int64_t K,
@@ -426,17 +498,20 @@ extern "C" int segk_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const 
     if (x) {
         x_codes = workspace;
         x_scales = (const uint8_t*)workspace + align_up(segk_mxfp4_codes_bytes(M, K), 16);
-        if (const int rc = quantize(x_dtype, x, ldx, M, K, workspace, const_cast<void*>(x_scales), st)) return rc;
+        if (const int rc = quantize(x_dtype, x, ldx, M, K, workspace, const_cast<void*>(x_scales), (int64_t)align_up(M, 4), st)) return rc;
     }
     LinearArgs a = {};
     a.w = (const uint8_t*)w_codes; a.ws = (const uint32_t*)w_scales; a.x = (const uint8_t*)x_codes; a.xs = (const uint32_t*)x_scales;
-    a.bias = bias; a.y = y; a.M = M; a.N = N; a.ldc = slices_of(K) * 64; a.ldy = ldy; a.slices = (int)slices_of(K);
-    a.vec = reinterpret_cast<uintptr_t>(y) % (4 * esize(y_dtype)) == 0 && ldy % 4 == 0;
+    a.bias = bias; a.y = y; a.M = M; a.N = N; a.xs_rows = x ? (int64_t)align_up(M, 4) : M; a.ldc = slices_of(K) * 64; a.ldy = ldy; a.slices = (int)slices_of(K);
+    for (int v : {4, 8})
+        if (reinterpret_cast<uintptr_t>(y) % (v * esize(y_dtype)) == 0 && ldy % v == 0) a.vec = v;
     const int choice = pick_tile(M, N);
+    const bool wide = N % 4 == 0 && a.xs_rows % 4 == 0 && aligned16(w_scales) && aligned16(x_scales);
     SEGK_DISPATCH_DTYPE(y_dtype, TO, {
-        if (choice == 256) return launch_tile<TO, 256, 256, 2, 4>(a, st);
-        if (choice == 128) return launch_tile<TO, 128, 128, 2, 2>(a, st);
-        if (choice == 64) return launch_tile<TO, 64, 64, 2, 2>(a, st);
+        if (choice == 256 && wide) return launch_tile<TO, 256, 256, 2, 4, true>(a, st);
+        if (choice == 256) return launch_tile<TO, 256, 256, 2, 4, false>(a, st);
+        if (choice == 128) return launch_tile<TO, 128, 128, 2, 2, false>(a, st);
+        if (choice == 64) return launch_tile<TO, 64, 64, 2, 2, false>(a, st);
         hipLaunchKernelGGL((mxfp4_rows_kernel<TO>), dim3((unsigned)((N + 15) / 16), (unsigned)((M + 15) / 16)), dim3(256), 0, st, a);
     });
     SEGK_LAUNCH_CHECK();
