@@ -64,6 +64,29 @@ __device__ __forceinline__ int load_class(const DistillArgs& a, int64_t at) {
 __device__ __forceinline__ float load_kept(const DistillArgs& a, int64_t at) {
     return a.t_bf16 ? (float)static_cast<const bf16*>(a.t)[at] : static_cast<const float*>(a.t)[at];
 }
+// Rows (of k contiguous entries) with at least one kept logit among every `step`-th group of 64 / kp rows from `first` on, for a
+// whole wave, four groups in flight
+__device__ __forceinline__ int count_rows(const DistillArgs& a, int64_t rows, int log_kp, int64_t first, int64_t step, int lane) {
+    const int per = 64 >> log_kp, j = lane & ((1 << log_kp) - 1);
+    const int64_t groups = (rows + per - 1) / per;
+    int n = 0;
+    for (int64_t g = first; g < groups; g += 4 * step) {
+        bool have[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t row = (g + u * step) * per + (lane >> log_kp);
+            have[u] = j < a.k && row < rows && load_class(a, row * a.k + j) >= 0;
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            uint64_t m = __ballot(have[u]);
+            for (int d = 1; d < (1 << log_kp); d *= 2) m |= m >> d;         // any entry of a row into the bit of its first
+            n += j == 0 && ((m >> lane) & 1ull);
+        }
+    }
+    return wave_sum_i(n);
+}
+
 // the sum of the partial counts, at least 1; every lane of the wave has to call it
 __device__ __forceinline__ int count_of(const int* __restrict__ counts) {
     int n = 0;
@@ -71,6 +94,33 @@ __device__ __forceinline__ int count_of(const int* __restrict__ counts) {
     for (int i = 0; i < kCountBlocks / 64; ++i) n += counts[i * 64 + (threadIdx.x & 63)];
     n = wave_sum_i(n);
     return n > 0 ? n : 1;
+}
+// the same for VP neighbouring positions: 16-byte loads for four of them
+template <int VP> __device__ __forceinline__ void load_classes(const DistillArgs& a, int64_t at, int (&c)[VP]) {
+    if constexpr (VP == 4) {
+        if (a.idx64) {
+            typedef int64_t i64x2 __attribute__((ext_vector_type(2)));
+            const i64x2 lo = *reinterpret_cast<const i64x2*>(static_cast<const int64_t*>(a.idx) + at), hi = *reinterpret_cast<const i64x2*>(static_cast<const int64_t*>(a.idx) + at + 2);
+            const int64_t i[4] = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+            for (int v = 0; v < 4; ++v) c[v] = i[v] >= 0 && i[v] < a.V ? (int)i[v] : -1;
+        } else {
+            const int4 i = *reinterpret_cast<const int4*>(static_cast<const int32_t*>(a.idx) + at);
+            c[0] = i.x; c[1] = i.y; c[2] = i.z; c[3] = i.w;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) c[v] = c[v] >= 0 && c[v] < a.V ? c[v] : -1;
+        }
+    } else {
+        c[0] = load_class(a, at);
+    }
+}
+template <int VP> __device__ __forceinline__ void load_kepts(const DistillArgs& a, int64_t at, float (&t)[VP]) {
+    if constexpr (VP == 4) {
+        if (a.t_bf16) Elem<bf16>::load4(static_cast<const bf16*>(a.t) + at, t);
+        else Elem<float>::load4(static_cast<const float*>(a.t) + at, t);
+    } else {
+        t[0] = load_kept(a, at);
+    }
 }
 // what multiplies T * (M q - p ...) of a position; every lane of the wave has to call it
 __device__ __forceinline__ float grad_scale(const DistillArgs& a, int64_t position) {
@@ -179,6 +229,74 @@ __device__ __forceinline__ void for_kept(int cls, int phase, int g0, int lane, F
     }
 }
 
+// The kept entries of a row, one for each lane of a wave (cls: this lane's class or -1).
+struct Kept {
+    float p, lp, z;          // probability, its logarithm (base 2), the student's logit
+    float total;             // p of all entries with this class
+    float rest, mass;        // of the row: what the teacher gave to the other classes; sum of p and rest
+    float top, sum;          // of the row: the student's maximum over the kept classes and the sum of exp over it
+};
+template <typename T>
+__device__ __forceinline__ Kept kept_entries(const DistillArgs& a, int64_t row, const T* __restrict__ z, int cls, int lane, float c) {
+    Kept e;
+    e.p = 0.f;
+    e.lp = e.z = -INFINITY;
+    float t = -INFINITY;
+    if (cls >= 0) {
+        t = load_kept(a, row * a.k + lane);
+        e.z = Elem<T>::to_f(z[cls]);
+    }
+    if (a.tlse) {
+        e.lp = cls >= 0 ? fmaf(t, a.invT, -a.tlse[row]) * kLog2e : -INFINITY;
+        e.p = cls >= 0 ? fast_exp2(e.lp) : 0.f;
+    } else {
+        const float top = wave_max(t);
+        const float x = cls >= 0 && top != -INFINITY ? fast_exp2((t - top) * c) : 0.f;
+        const float sum = wave_sum(x);
+        e.p = sum == 0.f ? 0.f : x / sum;
+        e.lp = (t - top) * c - log2f(sum);
+    }
+    const float mass = wave_sum(e.p);
+    e.total = e.p;
+    bool first = cls >= 0;
+    for (int j = 0; j < a.k; ++j) {
+        const int cj = __builtin_amdgcn_readlane(cls, j);
+        const float pj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(e.p), j));
+        if (cj == cls && j != lane) {
+            e.total += pj;
+            if (j < lane) first = false;
+        }
+    }
+    const int distinct = __popcll(__ballot(first));
+    e.rest = a.tlse ? 1.f - mass : 0.f;
+    if (!(e.rest > kRestFloor) || distinct == a.V) e.rest = 0.f;
+    e.mass = mass + e.rest;
+    e.top = wave_max(first ? e.z : -INFINITY);
+    e.sum = wave_sum(first && e.top != -INFINITY ? exp_over(e.z, e.top, c) : 0.f);
+    return e;
+}
+// maximum and sum of exp over all classes, from those outside (ko, so) and those kept; share: exp of ko over the maximum
+struct Joined { float top, sum, share; };
+__device__ __forceinline__ Joined join(float ko, float so, float km, float sm, float c) {
+    Joined w;
+    w.top = fmaxf(ko, km);
+    w.share = rebase(ko, w.top, c);
+    w.sum = so * w.share + sm * rebase(km, w.top, c) + (so != so ? so : 0.f);      // a NaN among the logits reaches the row
+    return w;
+}
+// the row's loss in units of ln 2 T^2, for a whole wave
+__device__ __forceinline__ float kept_loss(const Kept& e, const Joined& w, float ko, float so, float c) {
+    const float ls = log2f(w.sum);
+    float l = e.p == 0.f ? 0.f : e.p * (e.lp - ((e.z - w.top) * c - ls));
+    l = wave_sum(l);
+    if (e.rest > 0.f) l += e.rest * (log2f(e.rest) - (log2f(so) + (ko - w.top) * c - ls));
+    return l;
+}
+// the gradient of a class outside is this times exp of its logit over ko
+__device__ __forceinline__ float outside_factor(const Joined& w, float so, float rest, float mass, float gs) {
+    return gs * (mass * w.share / w.sum - (rest > 0.f ? rest / so : 0.f));
+}
+
 // One workgroup per row; with NCH > 0 the row stays in registers (NCH pieces per thread), with NCH == 0 it is read twice.
 template <typename T, int NT, int NCH, bool GRAD>
 __global__ __launch_bounds__(NT) void distill_rows_kernel(const DistillArgs a) {
@@ -215,43 +333,13 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(const DistillArgs a) {
     }
 
     // ---- the kept entries, one for each lane of the first wave
-    float p = 0.f, lp = -INFINITY, zj = -INFINITY;
+    Kept e = {};
     if (wave == 0) {
-        float t = -INFINITY;
-        if (cls >= 0) {
-            t = load_kept(a, row * a.k + lane);
-            zj = Elem<T>::to_f(r.p[cls]);
-        }
-        if (a.tlse) {
-            lp = cls >= 0 ? fmaf(t, a.invT, -a.tlse[row]) * kLog2e : -INFINITY;
-            p = cls >= 0 ? fast_exp2(lp) : 0.f;
-        } else {
-            const float top = wave_max(t);
-            const float e = cls >= 0 && top != -INFINITY ? fast_exp2((t - top) * c) : 0.f;
-            const float sum = wave_sum(e);
-            p = sum == 0.f ? 0.f : e / sum;
-            lp = (t - top) * c - log2f(sum);
-        }
-        const float mass = wave_sum(p);
-        float total = p;                                  // of all entries with this class
-        bool first = cls >= 0;
-        for (int j = 0; j < a.k; ++j) {
-            const int cj = __builtin_amdgcn_readlane(cls, j);
-            const float pj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), j));
-            if (cj == cls && j != lane) {
-                total += pj;
-                if (j < lane) first = false;
-            }
-        }
-        const int distinct = __popcll(__ballot(first));
-        float rest = a.tlse ? 1.f - mass : 0.f;
-        if (!(rest > kRestFloor) || distinct == a.V) rest = 0.f;
-        const float zm = wave_max(first ? zj : -INFINITY);
-        const float sm = wave_sum(first && zm != -INFINITY ? exp_over(zj, zm, c) : 0.f);
+        e = kept_entries<T>(a, row, r.p, cls, lane, c);
         const float gs = GRAD ? grad_scale(a, row) : 0.f;
-        sh_p[lane] = total;
-        sh_z[lane] = zj;
-        if (lane == 0) { sh_x[0] = zm; sh_x[1] = sm; sh_x[2] = rest; sh_x[3] = mass + rest; sh_x[4] = gs; }
+        sh_p[lane] = e.total;
+        sh_z[lane] = e.z;
+        if (lane == 0) { sh_x[0] = e.top; sh_x[1] = e.sum; sh_x[2] = e.rest; sh_x[3] = e.mass; sh_x[4] = gs; }
     }
 
     // ---- maximum and sum of the classes that were not kept
@@ -313,22 +401,15 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(const DistillArgs a) {
     float so = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) so += sh_k[w] == -INFINITY ? sh_s[w] : sh_s[w] * exp_over(sh_k[w], ko, c);
-    const float km = sh_x[0], rest = sh_x[2], mass = sh_x[3], gs = sh_x[4];
-    const float kk = fmaxf(ko, km);
-    const float fo = rebase(ko, kk, c);
-    const float s = so * fo + sh_x[1] * rebase(km, kk, c) + (so != so ? so : 0.f);      // a NaN among the logits reaches the row
-
+    const Joined w = join(ko, so, sh_x[0], sh_x[1], c);
     if (wave == 0) {
-        const float ls = log2f(s);
-        float l = p == 0.f ? 0.f : p * (lp - ((zj - kk) * c - ls));
-        l = wave_sum(l);
-        if (rest > 0.f) l += rest * (log2f(rest) - (log2f(so) + (ko - kk) * c - ls));
+        const float l = kept_loss(e, w, ko, so, c);
         if (lane == 0) a.row_loss[row] = l * (kLn2 * a.T * a.T * a.weight);
     }
     if constexpr (GRAD) {
-        const float inv = 1.f / s;
-        const float gj = lane < a.k ? gs * (mass * exp_over(sh_z[lane], kk, c) * inv - sh_p[lane]) : 0.f;
-        const float b = gs * (mass * fo * inv - (rest > 0.f ? rest / so : 0.f));
+        const float gs = sh_x[4];
+        const float gj = lane < a.k ? gs * (sh_x[3] * exp_over(sh_z[lane], w.top, c) / w.sum - sh_p[lane]) : 0.f;
+        const float b = outside_factor(w, so, sh_x[2], sh_x[3], gs);
         const float base = ko == -INFINITY ? 0.f : ko;
         auto write = [&](const Piece<T>& y, int g0) {
             float f[VEC];
@@ -355,6 +436,153 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(const DistillArgs a) {
                 if (g0 + lane < r.pieces) y = r.load(g0 + lane);
                 write(y, g0);
             }
+        }
+    }
+}
+
+// Few long rows: a row is shared by S workgroups.  Maximum and sum of the classes outside, one pair for each share; one wave per row
+// joins them (loss, and what the gradient needs); the gradient of each share.
+constexpr int kShares = 64;
+constexpr int kRowFloats = 2 + kTopMax;      // of a joined row: maximum outside, factor outside, gradients of the kept entries
+
+template <typename T> struct Share {         // the pieces [lo, hi) of a row, whole groups of 64
+    int lo, hi;
+    __device__ __forceinline__ Share(const Row<T>& r) {
+        const int groups = (r.pieces + 63) / 64, per = (groups + gridDim.x - 1) / gridDim.x;
+        lo = (int)blockIdx.x * per * 64;
+        hi = lo + per * 64 < r.pieces ? lo + per * 64 : r.pieces;
+    }
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void distill_share_kernel(const DistillArgs a, float* __restrict__ parts) {
+    constexpr int VEC = Piece<T>::VEC, U = 4;
+    if (a.skip_if_one && a.upstream[0] == 1.f) return;
+    __shared__ float sh_k[4], sh_s[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t row = blockIdx.y;
+    const float c = a.invT * kLog2e;
+    const Row<T> r(static_cast<const T*>(a.z) + row * a.ld, a.V);
+    const Share<T> part(r);
+    const int cls = lane < a.k ? load_class(a, row * a.k + lane) : -1;
+    if (__ballot(cls >= 0) == 0) return;
+    float m = -INFINITY, s = 0.f;                        // of this lane
+    for (int g0 = part.lo + wave * 64; g0 < part.hi; g0 += 256 * U) {
+        Piece<T> y[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int g = g0 + u * 256 + lane;
+            if (g < part.hi) y[u] = r.load(g);
+            else
+#pragma unroll
+                for (int w = 0; w < 4; ++w) y[u].w[w] = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;
+        }
+        float top = m;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            for_kept<VEC>(cls, r.phase, g0 + u * 256, lane, [&](bool here, int v, int) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i)
+                    if (here && i == v) y[u].clear(i);
+            });
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) top = fmaxf(top, y[u].get(v));
+        }
+        s *= rebase(m, top, c);
+        m = top;
+        const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) s += exp_over(y[u].get(v), base, c);
+    }
+    const float k = wave_max(m);
+    s = wave_sum(m == -INFINITY ? s : s * exp_over(m, k, c));
+    if (lane == 0) { sh_k[wave] = k; sh_s[wave] = s; }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const float ko = fmaxf(fmaxf(sh_k[0], sh_k[1]), fmaxf(sh_k[2], sh_k[3]));
+        float so = 0.f;
+        for (int w = 0; w < 4; ++w) so += sh_k[w] == -INFINITY ? sh_s[w] : sh_s[w] * exp_over(sh_k[w], ko, c);
+        float* out = parts + (row * kShares + blockIdx.x) * 2;
+        out[0] = ko;
+        out[1] = so;
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(64) void distill_join_kernel(const DistillArgs a, const float* __restrict__ parts, int shares, float* __restrict__ joined) {
+    if (a.skip_if_one && a.upstream[0] == 1.f) return;
+    const int lane = threadIdx.x;
+    const int64_t row = blockIdx.x;
+    const float c = a.invT * kLog2e;
+    const T* z = static_cast<const T*>(a.z) + row * a.ld;
+    const int cls = lane < a.k ? load_class(a, row * a.k + lane) : -1;
+    if (__ballot(cls >= 0) == 0) {
+        if (lane == 0) a.row_loss[row] = 0.f;
+        return;
+    }
+    const float* in = parts + (row * kShares + lane) * 2;
+    const float k = lane < shares ? in[0] : -INFINITY, s = lane < shares ? in[1] : 0.f;
+    const float ko = wave_max(k), so = wave_sum(k == -INFINITY ? s : s * exp_over(k, ko, c));
+    const Kept e = kept_entries<T>(a, row, z, cls, lane, c);
+    const Joined w = join(ko, so, e.top, e.sum, c);
+    const float l = kept_loss(e, w, ko, so, c);
+    if (lane == 0) a.row_loss[row] = l * (kLn2 * a.T * a.T * a.weight);
+    if (joined) {
+        const float gs = grad_scale(a, row);
+        float* out = joined + row * kRowFloats;
+        if (lane == 0) {
+            out[0] = ko;
+            out[1] = outside_factor(w, so, e.rest, e.mass, gs);
+        }
+        out[2 + lane] = gs * (e.mass * exp_over(e.z, w.top, c) / w.sum - e.total);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void distill_share_grad_kernel(const DistillArgs a, const float* __restrict__ joined) {
+    constexpr int VEC = Piece<T>::VEC, U = 4;
+    if (a.skip_if_one && a.upstream[0] == 1.f) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t row = blockIdx.y;
+    const float c = a.invT * kLog2e;
+    const Row<T> r(static_cast<const T*>(a.z) + row * a.ld, a.V);
+    const Share<T> part(r);
+    T* dst = static_cast<T*>(a.dz) + row * a.ld_d;
+    const bool vec_ok = (reinterpret_cast<uintptr_t>(dst) / sizeof(T)) % VEC == (unsigned)r.phase;
+    const int cls = lane < a.k ? load_class(a, row * a.k + lane) : -1;
+    const bool any = __ballot(cls >= 0) != 0;
+    const float* in = joined + row * kRowFloats;
+    const float ko = any ? in[0] : 0.f, b = any ? in[1] : 0.f, gj = any ? in[2 + lane] : 0.f;
+    const float base = ko == -INFINITY ? 0.f : ko;
+    for (int g0 = part.lo + wave * 64; g0 < part.hi; g0 += 256 * U) {
+        Piece<T> y[U];
+        if (any) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int g = g0 + u * 256 + lane;
+                if (g < part.hi) y[u] = r.load(g);
+                else
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) y[u].w[w] = 0;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float f[VEC] = {};
+            if (any) {
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) f[v] = b * exp_over(y[u].get(v), base, c);
+                for_kept<VEC>(cls, r.phase, g0 + u * 256, lane, [&](bool here, int v, int j) {
+                    const float gv = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(gj), j));
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i)
+                        if (here && i == v) f[i] = gv;
+                });
+            }
+            const int g = g0 + u * 256 + lane;
+            if (g < part.hi) store_piece<T>(dst, vec_ok, g * VEC - r.phase, a.V, f);
         }
     }
 }
@@ -387,39 +615,43 @@ __global__ __launch_bounds__(256) void distill_pixels_kernel(const DistillArgs a
         }
         float e[CM][VP], top[VP], sum[VP], plogp[VP], lse[VP];
         uint32_t kept[VP];
+        if constexpr (VP == 4) {
+            if (a.tlse) Elem<float>::load4(a.tlse + o * a.inner + i0, lse);
+        } else if (a.tlse) lse[0] = a.tlse[o * a.inner + i0];
 #pragma unroll
         for (int v = 0; v < VP; ++v) {
             top[v] = -INFINITY;
             sum[v] = plogp[v] = 0.f;
             kept[v] = 0;
-            lse[v] = a.tlse ? a.tlse[o * a.inner + i0 + v] : 0.f;
 #pragma unroll
             for (int q = 0; q < CM; ++q) e[q][v] = 0.f;
         }
-        for (int j = 0; j < a.k; ++j)
+        const int64_t at = t0 + i0 * a.ts_p;
+        if (!a.tlse)                          // renormalised: the greatest of the kept logits first
+            for (int j = 0; j < a.k; ++j) {
+                int cj[VP];
+                float t[VP];
+                load_classes<VP>(a, at + j * a.ts_c, cj);
+                load_kepts<VP>(a, at + j * a.ts_c, t);
 #pragma unroll
-            for (int v = 0; v < VP; ++v) {
-                const int64_t at = t0 + j * a.ts_c + (i0 + v) * a.ts_p;
-                const int cj = load_class(a, at);
-                if (cj >= 0) {
-                    kept[v] |= 1u << cj;
-                    if (!a.tlse) top[v] = fmaxf(top[v], load_kept(a, at));
-                }
+                for (int v = 0; v < VP; ++v) top[v] = cj[v] >= 0 ? fmaxf(top[v], t[v]) : top[v];
             }
-        for (int j = 0; j < a.k; ++j)
+        for (int j = 0; j < a.k; ++j) {
+            int cj[VP];
+            float t[VP];
+            load_classes<VP>(a, at + j * a.ts_c, cj);
+            load_kepts<VP>(a, at + j * a.ts_c, t);
 #pragma unroll
             for (int v = 0; v < VP; ++v) {
-                const int64_t at = t0 + j * a.ts_c + (i0 + v) * a.ts_p;
-                const int cj = load_class(a, at);
-                if (cj < 0) continue;
-                const float t = load_kept(a, at);
-                const float lp = a.tlse ? fmaf(t, a.invT, -lse[v]) * kLog2e : (top[v] == -INFINITY ? -INFINITY : (t - top[v]) * c);
-                const float ej = fast_exp2(lp);
+                const float lp = a.tlse ? fmaf(t[v], a.invT, -lse[v]) * kLog2e : (top[v] == -INFINITY ? -INFINITY : (t[v] - top[v]) * c);
+                const float ej = cj[v] >= 0 ? fast_exp2(lp) : 0.f;
+                kept[v] |= cj[v] >= 0 ? 1u << cj[v] : 0u;
                 sum[v] += ej;
                 plogp[v] += ej == 0.f ? 0.f : ej * lp;
 #pragma unroll
-                for (int q = 0; q < CM; ++q) e[q][v] += q == cj ? ej : 0.f;
+                for (int q = 0; q < CM; ++q) e[q][v] += q == cj[v] ? ej : 0.f;
             }
+        }
 #pragma unroll
         for (int v = 0; v < VP; ++v) {
             const int64_t pos = o * a.inner + i0 + v;
@@ -493,21 +725,54 @@ __global__ __launch_bounds__(256) void distill_pixels_kernel(const DistillArgs a
     }
 }
 
-// positions with at least one kept logit: one partial count for each workgroup
-__global__ __launch_bounds__(256) void distill_count_kernel(const DistillArgs a, int64_t positions, int* __restrict__ counts) {
-    if (a.skip_if_one && a.upstream[0] == 1.f) return;
+// Positions with at least one kept logit: one partial count for each workgroup.
+// Rows: the entries of 64 / kp rows at a time, one for each lane, kp = k rounded up to a power of two.
+__global__ __launch_bounds__(256) void distill_count_rows_kernel(const DistillArgs a, int64_t rows, int log_kp, int* __restrict__ counts) {
     __shared__ int red[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int n = count_rows(a, rows, log_kp, (int64_t)blockIdx.x * 4 + wave, (int64_t)kCountBlocks * 4, lane);
+    if (lane == 0) red[wave] = n;
+    __syncthreads();
+    if (threadIdx.x == 0) counts[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+}
+// Planes: a thread takes 8 positions at a time and reads entry after entry until each has one (the first decides most of them); all
+// 8 loads of an entry are in flight together.
+__global__ __launch_bounds__(1024) void distill_count_planes_kernel(const DistillArgs a, int64_t positions, int* __restrict__ counts) {
+    __shared__ int red[16];
+    constexpr int U = 8;
     int n = 0;
-    for (int64_t p = (int64_t)blockIdx.x * 256 + threadIdx.x; p < positions; p += (int64_t)kCountBlocks * 256) {
-        const int64_t o = p / a.inner, i = p - o * a.inner;
-        int any = 0;
-        for (int j = 0; j < a.k && !any; ++j) any = load_class(a, o * a.k * a.inner + j * a.ts_c + i * a.ts_p) >= 0;
-        n += any;
+    const int64_t per = (positions + kCountBlocks - 1) / kCountBlocks, lo = per * blockIdx.x, hi = lo + per < positions ? lo + per : positions;
+    for (int64_t p = lo + threadIdx.x; p < hi; p += 1024 * U) {
+        int64_t at[U];
+        int c[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t pu = p + u * 1024 < hi ? p + u * 1024 : p;
+            const int64_t o = positions < (1ll << 31) ? (uint32_t)pu / (uint32_t)a.inner : pu / a.inner;
+            at[u] = o * a.k * a.inner + (pu - o * a.inner) * a.ts_p;
+            c[u] = -1;
+        }
+        for (int j = 0; j < a.k; ++j) {
+            int lowest = 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int d = load_class(a, at[u] + j * a.ts_c);
+                c[u] = d > c[u] ? d : c[u];
+                lowest = c[u] < lowest ? c[u] : lowest;
+            }
+            if (lowest >= 0) break;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) n += p + u * 1024 < hi && c[u] >= 0;
     }
     n = wave_sum_i(n);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = n;
     __syncthreads();
-    if (threadIdx.x == 0) counts[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+    if (threadIdx.x == 0) {
+        int t = 0;
+        for (int i = 0; i < 16; ++i) t += red[i];
+        counts[blockIdx.x] = t;
+    }
 }
 
 __device__ __forceinline__ double block_sum_1024(double s, double* red) {
@@ -824,8 +1089,10 @@ __global__ __launch_bounds__(256) void top_pixels_kernel(const T* __restrict__ z
 // ------------------------------------------------------------------------------------------------ host
 constexpr int kPixelClasses = 32;    // more classes than this: one workgroup (or wave) per row
 
-// `rows` launches with the tier of a row of V classes: (threads, pieces in registers per thread)
-template <typename T, typename F> static void row_tier(int64_t V, F&& f) {
+// Threads of a row's workgroup and pieces in registers per thread, by the row's length.  Rows of 16 to 64 KB: 512 threads with 8
+// pieces serve the loss, 256 with 16 the selection, whose search by the first wave leaves the others idle (4096 rows of 32000 bf16
+// logits: loss and gradient 103 against 107 us, selection 66 against 56).
+template <typename T, bool TOP, typename F> static void row_tier(int64_t V, F&& f) {
     constexpr int VEC = 16 / (int)sizeof(T);
     const int64_t pieces = (V + 2 * (VEC - 1)) / VEC;           // wherever the row begins
 #define SEGK_TIER(nt, nch) if (pieces <= (int64_t)(nt) * (nch)) return f(std::integral_constant<int, nt>{}, std::integral_constant<int, nch>{})
@@ -835,7 +1102,11 @@ template <typename T, typename F> static void row_tier(int64_t V, F&& f) {
     SEGK_TIER(64, 8);
     SEGK_TIER(256, 4);
     SEGK_TIER(256, 8);
-    SEGK_TIER(256, 16);
+    if constexpr (TOP) {
+        SEGK_TIER(256, 16);
+    } else {
+        SEGK_TIER(512, 8);
+    }
     SEGK_TIER(1024, 8);
     SEGK_TIER(1024, 16);
 #undef SEGK_TIER
@@ -904,7 +1175,7 @@ extern "C" int segk_top_logits(const void* logits, int dtype, int64_t outer, int
                                    px.s_p, px.inner, (int)C, (int)k, 1.f / temperature, (T*)values, indices, px.ts_c, px.ts_p, lse, px.blocks_each);
             });
         } else {
-            row_tier<T>(C, [&](auto nt, auto nch) {
+            row_tier<T, true>(C, [&](auto nt, auto nch) {
                 hipLaunchKernelGGL((top_rows_kernel<T, nt(), nch()>), dim3((unsigned)outer), dim3(nt()), 0, st, (const T*)logits, ld, (int)C, (int)k,
                                    1.f / temperature, (T*)values, indices, lse);
             });
@@ -914,10 +1185,22 @@ extern "C" int segk_top_logits(const void* logits, int dtype, int64_t outer, int
     return SEGK_OK;
 }
 
+// Workgroups that share a row (1: the row kernels).  The row kernels keep a row of up to 16384 pieces in registers and then read it
+// once; longer ones they read twice, and a few of them leave most of the chip idle.  Whole call for 131000 fp32 classes, shared / not,
+// forward and with gradient: 1 row 13/20, 17/34 us; 64 rows 17/30, 34/76; 128 rows 22/32, 54/82; 256 rows 35/35, 94/94.  For 131000
+// bf16 classes, in registers of one CU: 16 rows 14/18, 20/27; 128 rows 18/21, 35/31.  Below 8192 pieces one CU is as fast: 32000 fp32
+// classes, 16 rows 13/11, 19/15.
+static int shares_of(int64_t rows, int64_t C, int dtype) {
+    const int64_t pieces = C * (int64_t)esize(dtype) / 16;
+    if (rows > (pieces > 16384 ? 128 : 16) || pieces <= 8192) return 1;
+    int64_t s = pieces / 1024;
+    if (s > 1024 / rows) s = 1024 / rows;
+    return (int)(s > kShares ? kShares : s < 1 ? 1 : s);
+}
 static constexpr int kCollect = 256;
 // floats of the workspace: partial counts, level-1 sums, then one sum per row or workgroup
 static size_t distill_partials(int64_t outer, int64_t C, int64_t inner) {
-    if (!few(C, inner)) return (size_t)outer;
+    if (!few(C, inner)) return (size_t)outer * (outer <= 128 ? 1 + 2 * kShares + kRowFloats : 1);
     return (size_t)(pixels(outer, C, inner, C * inner, 1, false).blocks);      // an upper bound for either vector width
 }
 extern "C" size_t segk_distill_workspace(int64_t outer, int64_t C, int64_t inner) {
@@ -942,7 +1225,7 @@ extern "C" int segk_distill(const void* logits, int dtype, int64_t outer, int64_
     SEGK_REQUIRE(workspace_bytes >= segk_distill_workspace(outer, C, inner), SEGK_EWORKSPACE, "distill: workspace too small");
     SEGK_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 4 == 0, SEGK_EALIGN, "distill: workspace must be 4-byte aligned");
     const bool pix = few(C, inner);
-    const bool vec = aligned16(logits) && (!dlogits || (aligned16(dlogits) && ld_d % 4 == 0));
+    const bool vec = aligned16(logits) && (!dlogits || (aligned16(dlogits) && ld_d % 4 == 0)) && aligned16(values) && aligned16(indices) && aligned16(teacher_lse);
     const Pixels px = pixels(outer, C, inner, ld, k, vec);
     SEGK_REQUIRE(!pix || px.blocks < (1ll << 31), SEGK_ESHAPE, "distill: too many positions");
     SEGK_USE_DEVICE(dev);
@@ -965,8 +1248,14 @@ extern "C" int segk_distill(const void* logits, int dtype, int64_t outer, int64_
         a.inner = 1; a.ts_c = 1; a.ts_p = k;
         a.row_loss = position_loss ? position_loss : partial;
     }
-    if (mean) {
-        hipLaunchKernelGGL(distill_count_kernel, dim3(kCountBlocks), dim3(256), 0, st, a, outer * inner, counts);
+    if (mean && !skip) {
+        if (inner == 1) {
+            int log_kp = 0;
+            while ((1 << log_kp) < k) ++log_kp;
+            hipLaunchKernelGGL(distill_count_rows_kernel, dim3(kCountBlocks), dim3(256), 0, st, a, outer, log_kp, counts);
+        } else {
+            hipLaunchKernelGGL(distill_count_planes_kernel, dim3(kCountBlocks), dim3(1024), 0, st, a, outer * inner, counts);
+        }
         SEGK_LAUNCH_CHECK();
     }
     int64_t n = pix ? px.blocks : outer;
@@ -976,8 +1265,13 @@ extern "C" int segk_distill(const void* logits, int dtype, int64_t outer, int64_
                 if (dlogits) hipLaunchKernelGGL((distill_pixels_kernel<T, cm(), vp(), true>), dim3((unsigned)n), dim3(256), 0, st, a, px.blocks_each);
                 else hipLaunchKernelGGL((distill_pixels_kernel<T, cm(), vp(), false>), dim3((unsigned)n), dim3(256), 0, st, a, px.blocks_each);
             });
+        } else if (const int shares = shares_of(outer, C, dtype); shares > 1) {
+            float *parts = partial + outer, *joined = parts + outer * 2 * kShares;
+            hipLaunchKernelGGL((distill_share_kernel<T>), dim3(shares, (unsigned)outer), dim3(256), 0, st, a, parts);
+            hipLaunchKernelGGL((distill_join_kernel<T>), dim3((unsigned)outer), dim3(64), 0, st, a, parts, shares, dlogits ? joined : nullptr);
+            if (dlogits) hipLaunchKernelGGL((distill_share_grad_kernel<T>), dim3(shares, (unsigned)outer), dim3(256), 0, st, a, joined);
         } else {
-            row_tier<T>(C, [&](auto nt, auto nch) {
+            row_tier<T, false>(C, [&](auto nt, auto nch) {
                 if (dlogits) hipLaunchKernelGGL((distill_rows_kernel<T, nt(), nch(), true>), dim3((unsigned)n), dim3(nt()), 0, st, a);
                 else hipLaunchKernelGGL((distill_rows_kernel<T, nt(), nch(), false>), dim3((unsigned)n), dim3(nt()), 0, st, a);
             });

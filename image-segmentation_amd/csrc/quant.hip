@@ -78,6 +78,28 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
     return v > o ? v : o;
 }
 
+// The codes of values c0 .. c0 + 7 of a row (zeros beyond its end) and the scale byte of their block; the four lanes of a block, which
+// are neighbours, have to call it together.
+template <typename T> __device__ __forceinline__ uint32_t pack_eight(const T* __restrict__ row, int c0, int cols, uint32_t& byte) {
+    float v[8];
+    const T* p = row + c0;
+    if (c0 + 8 <= cols) load8_any<T>(p, v);
+    else
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = c0 + j < cols ? Elem<T>::to_f(p[j]) : 0.f;
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t b = __float_as_uint(v[j]) & 0x7FFFFFFFu;
+        top = top > b ? top : b;
+    }
+    byte = scale_byte(quad_max(top));
+    const float inv = scale_inverse(byte);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = byte == 255u ? 0.f : v[j] * inv;
+    return pack_codes(v);
+}
+
 // One thread for 8 values, four neighbouring threads for a block, sixteen for a slice of a row: 16 bytes (bf16) read and 4 written
 // per thread, both coalesced.
 template <typename T>
@@ -89,23 +111,8 @@ __global__ __launch_bounds__(256) void mxfp4_quantize_kernel(const T* __restrict
     const uint32_t r = per_row(item), i = item - r * per_row.d;
     const int64_t row = row0 + r;
     const int c0 = (int)i * 8;
-    float v[8];
-    const T* p = x + row * ld + c0;
-    if (c0 + 8 <= cols) load8_any<T>(p, v);
-    else
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = c0 + j < cols ? Elem<T>::to_f(p[j]) : 0.f;
-    uint32_t top = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const uint32_t b = __float_as_uint(v[j]) & 0x7FFFFFFFu;
-        top = top > b ? top : b;
-    }
-    const uint32_t byte = scale_byte(quad_max(top));
-    const float inv = scale_inverse(byte);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = byte == 255u ? 0.f : v[j] * inv;
-    codes[row * per_row.d + i] = pack_codes(v);
+    uint32_t byte;
+    codes[row * per_row.d + i] = pack_eight<T>(x + row * ld, c0, cols, byte);
     const int lane = threadIdx.x & 63;
     const uint32_t b1 = __shfl(byte, (lane & 48) + 4, 64), b2 = __shfl(byte, (lane & 48) + 8, 64), b3 = __shfl(byte, (lane & 48) + 12, 64);
     if ((i & 15u) == 0) scales[(int64_t)(i >> 4) * scale_rows + row] = byte | (b1 << 8) | (b2 << 16) | (b3 << 24);
@@ -205,25 +212,70 @@ __device__ __forceinline__ void store_rows(const LinearArgs& a, int64_t m, int64
     for (int i = 0; i < TN; ++i) store_outputs<TO>(a, m, n + i * 16 + 4 * q, acc[i][j]);
 }
 
-// Few rows: a workgroup computes 16 outputs of 16 rows, its four waves share the slices.  Operands go straight from memory to the
-// matrix instruction: lane l holds the 32 values (16 bytes) of row l % 16 in the block l / 16 of the slice.
-template <typename TO>
-__global__ __launch_bounds__(256) void mxfp4_rows_kernel(const LinearArgs a) {
+// Few rows: a workgroup computes 16 outputs of 16 rows, its waves share the slices.  Weights go straight from memory to the matrix
+// instruction, AHEAD slices of a wave at a time: lane l holds the 32 values (16 bytes) of row l % 16 in the block l / 16 of the slice.
+// FUSED: up to kFusedRows rows of x are packed by every workgroup for itself while its first weights are on their way, which
+// saves a launch; the packed rows stay in LDS.  Both in the same call, 8192 x 8192: one row 9.2 against 11.1 us with a launch of its
+// own, two 10.4 / 11.1, four 17.7 / 14.9.
+constexpr int kFusedRows = 2, kFusedBytes = 32768;
+
+template <typename TO, typename TX, int WAVES, int AHEAD, bool FUSED>
+__global__ __launch_bounds__(WAVES * 64) void mxfp4_rows_kernel(const LinearArgs a, const TX* __restrict__ xm, int64_t ldx, int cols) {
+    extern __shared__ __align__(16) char lds[];
+    __shared__ f32x4 part[WAVES][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
     const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * 16;
     const int64_t n = n0 + r < a.N ? n0 + r : a.N - 1, m = m0 + r < a.M ? m0 + r : a.M - 1;
     const uint8_t *wp = a.w + n * a.ldc + q * 16, *xp = a.x + m * a.ldc + q * 16;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int s = wave; s < a.slices; s += 4) {
-        const u32x4 wv = *reinterpret_cast<const u32x4*>(wp + (int64_t)s * 64), xv = *reinterpret_cast<const u32x4*>(xp + (int64_t)s * 64);
-        const uint32_t sw = a.ws[(int64_t)s * a.N + n] >> (8 * q), sx = a.xs[(int64_t)s * a.xs_rows + m] >> (8 * q);
-        acc = mfma_fp4(wv, xv, acc, sw, sx);
+    u32x4 wv[AHEAD];
+    uint32_t sw[AHEAD];
+    auto fetch = [&](int s0) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int s = s0 + u * WAVES < a.slices ? s0 + u * WAVES : a.slices - 1;
+            wv[u] = *reinterpret_cast<const u32x4*>(wp + (int64_t)s * 64);
+            sw[u] = a.ws[(int64_t)s * a.N + n];
+        }
+    };
+    fetch(wave);
+    uint32_t* xc = reinterpret_cast<uint32_t*>(lds);                               // packed rows, then their scales [slice][row]
+    uint32_t* xs = xc + (int)a.M * a.slices * 16;
+    if constexpr (FUSED) {
+        const int per_row = a.slices * 16, items = (int)a.M * per_row;
+        for (int item = threadIdx.x; item < items; item += WAVES * 64) {           // groups of 16 lanes stay together
+            const int row = item / per_row, i = item - row * per_row;
+            uint32_t byte;
+            xc[item] = pack_eight<TX>(xm + row * ldx, i * 8, cols, byte);
+            const uint32_t b1 = __shfl(byte, (lane & 48) + 4, 64), b2 = __shfl(byte, (lane & 48) + 8, 64), b3 = __shfl(byte, (lane & 48) + 12, 64);
+            if ((i & 15) == 0) xs[(i >> 4) * (int)a.M + row] = byte | (b1 << 8) | (b2 << 16) | (b3 << 24);
+        }
+        __syncthreads();
     }
-    __shared__ f32x4 part[4][64];
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = wave; s0 < a.slices; s0 += AHEAD * WAVES) {
+        if (s0 != wave) fetch(s0);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int s = s0 + u * WAVES;
+            if (s >= a.slices) break;
+            u32x4 xv;
+            uint32_t sx;
+            if constexpr (FUSED) {
+                xv = *reinterpret_cast<const u32x4*>(lds + (int)m * a.slices * 64 + s * 64 + q * 16);
+                sx = xs[s * (int)a.M + (int)m];
+            } else {
+                xv = *reinterpret_cast<const u32x4*>(xp + (int64_t)s * 64);
+                sx = a.xs[(int64_t)s * a.xs_rows + m];
+            }
+            acc = mfma_fp4(wv[u], xv, acc, sw[u] >> (8 * q), sx >> (8 * q));
+        }
+    }
     part[wave][lane] = acc;
     __syncthreads();
     if (wave == 0) {
-        acc = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+        acc = part[0][lane];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) acc += part[w][lane];
         store_outputs<TO>(a, m0 + r, n0 + 4 * q, acc);
     }
 }
@@ -390,6 +442,7 @@ __global__ __launch_bounds__(WM * WN * 64, (WM * WN * 64 >= 512 ? 2 : 0)) void m
 
 // ------------------------------------------------------------------------------------------------ host
 static int64_t slices_of(int64_t cols) { return (cols + kSlice - 1) / kSlice; }
+static bool fused(int64_t M, int64_t K) { return M <= kFusedRows && M * slices_of(K) * 68 <= kFusedBytes; }
 
 static int check_matrix(const char* who, int dtype, const void* x, int64_t ld, int64_t rows, int64_t cols) {
     SEGK_REQUIRE(x, SEGK_EINVAL, "%s: null pointer", who);
@@ -477,6 +530,7 @@ extern "C" int segk_mxfp4_dequantize(int dtype, const void* codes, const void* s
 
 extern "C" size_t segk_mxfp4_linear_workspace(int64_t M, int64_t K, int64_t N) {
     (void)N;
+    if (fused(M, K)) return 0;
     return align_up(segk_mxfp4_codes_bytes(M, K), 16) + segk_mxfp4_scales_bytes((int64_t)align_up(M > 0 ? M : 0, 4), K);
 }
 
@@ -489,30 +543,48 @@ extern "C" int segk_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const 
     if (const int rc = check_packed("mxfp4_linear", w_codes, w_scales)) return rc;
     if (x) {
         if (const int rc = check_matrix("mxfp4_linear", x_dtype, x, ldx, M, K)) return rc;
-        SEGK_REQUIRE(workspace && workspace_bytes >= segk_mxfp4_linear_workspace(M, K, N), SEGK_EWORKSPACE, "mxfp4_linear: workspace too small");
+        SEGK_REQUIRE(fused(M, K) || (workspace && workspace_bytes >= segk_mxfp4_linear_workspace(M, K, N)), SEGK_EWORKSPACE, "mxfp4_linear: workspace too small");
         SEGK_REQUIRE(aligned16(workspace), SEGK_EALIGN, "mxfp4_linear: workspace must be 16-byte aligned");
     } else if (const int rc = check_packed("mxfp4_linear", x_codes, x_scales)) return rc;
     SEGK_REQUIRE((M + 15) / 16 < 65536, SEGK_ESHAPE, "mxfp4_linear: too many rows");
     SEGK_USE_DEVICE(dev);
     hipStream_t st = (hipStream_t)stream;
-    if (x) {
+    const bool pack_inside = x && fused(M, K);
+    if (x && !pack_inside) {
         x_codes = workspace;
         x_scales = (const uint8_t*)workspace + align_up(segk_mxfp4_codes_bytes(M, K), 16);
         if (const int rc = quantize(x_dtype, x, ldx, M, K, workspace, const_cast<void*>(x_scales), (int64_t)align_up(M, 4), st)) return rc;
     }
     LinearArgs a = {};
     a.w = (const uint8_t*)w_codes; a.ws = (const uint32_t*)w_scales; a.x = (const uint8_t*)x_codes; a.xs = (const uint32_t*)x_scales;
-    a.bias = bias; a.y = y; a.M = M; a.N = N; a.xs_rows = x ? (int64_t)align_up(M, 4) : M; a.ldc = slices_of(K) * 64; a.ldy = ldy; a.slices = (int)slices_of(K);
+    a.bias = bias; a.y = y; a.M = M; a.N = N; a.xs_rows = x && !pack_inside ? (int64_t)align_up(M, 4) : M; a.ldc = slices_of(K) * 64; a.ldy = ldy; a.slices = (int)slices_of(K);
     for (int v : {4, 8})
         if (reinterpret_cast<uintptr_t>(y) % (v * esize(y_dtype)) == 0 && ldy % v == 0) a.vec = v;
-    const int choice = pick_tile(M, N);
+    const int choice = pack_inside ? 16 : pick_tile(M, N);
     const bool wide = N % 4 == 0 && a.xs_rows % 4 == 0 && aligned16(w_scales) && aligned16(x_scales);
     SEGK_DISPATCH_DTYPE(y_dtype, TO, {
         if (choice == 256 && wide) return launch_tile<TO, 256, 256, 2, 4, true>(a, st);
         if (choice == 256) return launch_tile<TO, 256, 256, 2, 4, false>(a, st);
         if (choice == 128) return launch_tile<TO, 128, 128, 2, 2, false>(a, st);
         if (choice == 64) return launch_tile<TO, 64, 64, 2, 2, false>(a, st);
-        hipLaunchKernelGGL((mxfp4_rows_kernel<TO>), dim3((unsigned)((N + 15) / 16), (unsigned)((M + 15) / 16)), dim3(256), 0, st, a);
+        const dim3 grid((unsigned)((N + 15) / 16), (unsigned)((M + 15) / 16));
+        // Up to 4096 outputs there are few workgroups, and 16 waves share the slices of each; beyond, 8 waves, with 8 slices in flight
+        // if they are many.  One row of packed x, 8192 outputs from 8192 values: (8 waves, 8 ahead) 8.8, (8, 4) 9.6, (4, 8) 12.2,
+        // (16, 8) 13.5 us; from 512 values: (8, 4) 3.3, (8, 8) 4.1 us; 512 outputs from 8192: (16, 4) 4.7, (16, 8) 6.6 us.
+        auto launch = [&](auto waves, auto ahead) {
+            if (pack_inside) {
+                const unsigned bytes = (unsigned)(M * a.slices * 68);
+                if (x_dtype == SEGK_BF16)
+                    hipLaunchKernelGGL((mxfp4_rows_kernel<TO, bf16, waves(), ahead(), true>), grid, dim3(waves() * 64), bytes, st, a, (const bf16*)x, ldx, (int)K);
+                else
+                    hipLaunchKernelGGL((mxfp4_rows_kernel<TO, float, waves(), ahead(), true>), grid, dim3(waves() * 64), bytes, st, a, (const float*)x, ldx, (int)K);
+            } else {
+                hipLaunchKernelGGL((mxfp4_rows_kernel<TO, float, waves(), ahead(), false>), grid, dim3(waves() * 64), 0, st, a, (const float*)nullptr, (int64_t)0, 0);
+            }
+        };
+        if (N <= 4096) launch(std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
+        else if (a.slices > 32) launch(std::integral_constant<int, 8>{}, std::integral_constant<int, 8>{});
+        else launch(std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{});
     });
     SEGK_LAUNCH_CHECK();
     return SEGK_OK;

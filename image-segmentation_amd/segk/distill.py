@@ -110,16 +110,17 @@ class _DistillFn(torch.autograd.Function):
         each = reduction == "none"
         out = torch.empty(rest if each else (), dtype=torch.float32, device=z.device)
         dz = torch.empty((outer, C, inner), dtype=z.dtype, device=z.device) if want_grad and not each else None
-        _DistillFn._launch(ctx.meta, z, values, indices, lse, None, MEAN if reduction == "mean" else 0, None if each else out, out if each else None, dz)
-        ctx.save_for_backward(z, values, indices, lse)
-        ctx.dz = dz
+        # a workspace of its own for every call: launches on other streams and replays of captured graphs never share one
+        ws = torch.empty(query("segk_distill_workspace", outer, C, inner), dtype=torch.uint8, device=z.device)
+        _DistillFn._launch(ctx.meta, z, values, indices, lse, None, MEAN if reduction == "mean" else 0, None if each else out, out if each else None, dz, ws)
+        if want_grad:
+            ctx.save_for_backward(z, values, indices, lse)
+            ctx.dz, ctx.ws = dz, ws
         return out
 
     @staticmethod
-    def _launch(meta, z, values, indices, lse, upstream, flags, loss, each, dz):
+    def _launch(meta, z, values, indices, lse, upstream, flags, loss, each, dz, ws):
         outer, C, inner, ld, moved, k, dim, T, weight, reduction, shape, in_dtype = meta
-        # a buffer of its own for every call: launches on other streams and replays of captured graphs never share one
-        ws = torch.empty(query("segk_distill_workspace", outer, C, inner), dtype=torch.uint8, device=z.device)
         p = ops._p
         dev, st = _env(z)
         with ops._streamed("distillation loss", z.numel() * z.element_size() * (2 if dz is not None else 1)):
@@ -132,13 +133,14 @@ class _DistillFn(torch.autograd.Function):
     def backward(ctx, g):
         z, values, indices, lse = ctx.saved_tensors
         outer, C, inner, ld, moved, k, dim, T, weight, reduction, shape, in_dtype = ctx.meta
-        dz, ctx.dz = ctx.dz, None               # handed over once; a second backward pass computes its own
+        dz, ctx.dz, ws, ctx.ws = ctx.dz, None, ctx.ws, None      # handed over once; a second backward pass computes its own
         flags = EACH if reduction == "none" else MEAN if reduction == "mean" else 0
         if dz is None:
             dz = torch.empty((outer, C, inner), dtype=z.dtype, device=z.device)
+            ws = torch.empty(query("segk_distill_workspace", outer, C, inner), dtype=torch.uint8, device=z.device)
         else:
             flags |= SKIP
-        _DistillFn._launch(ctx.meta, z, values, indices, lse, g.float().contiguous(), flags, None, None, dz)
+        _DistillFn._launch(ctx.meta, z, values, indices, lse, g.float().contiguous(), flags, None, None, dz, ws)
         return (_restore(dz, shape, dim, C, moved).to(in_dtype),) + (None,) * 8
 
 

@@ -133,12 +133,13 @@ def mxfp4_linear(x, w, bias=None, out_dtype=None):
         return (y if bias is None else y + bias).to(out_dtype).reshape(lead + (N,))
     y = torch.empty((M, N), dtype=torch.float32 if out_dtype == torch.float16 else out_dtype, device=w.device)
     if M and N:
-        ws = None if packed else torch.empty(query("segk_mxfp4_linear_workspace", M, K, N), dtype=torch.uint8, device=w.device)
+        nbytes = 0 if packed else query("segk_mxfp4_linear_workspace", M, K, N)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=w.device) if nbytes else None     # one for every call: nothing is shared
         dev, st = _env(w.codes)
         with ops._streamed("4-bit linear", M * K * (0.53125 if packed else x.element_size()) + N * K * 0.53125 + M * N * y.element_size()):
             call("segk_mxfp4_linear", None if packed else x.data_ptr(), 0 if packed else dt(x.dtype), 0 if packed else ld,
                  x.codes.data_ptr() if packed else None, x.scales.data_ptr() if packed else None, M, K, w.codes.data_ptr(), w.scales.data_ptr(), N,
-                 ops._p(bias), y.data_ptr(), dt(y.dtype), N, ops._p(ws), 0 if ws is None else ws.numel(), dev, st)
+                 ops._p(bias), y.data_ptr(), dt(y.dtype), N, ops._p(ws), nbytes, dev, st)
     return y.to(out_dtype).reshape(lead + (N,))
 
 

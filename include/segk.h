@@ -125,8 +125,9 @@ int segk_top_logits(const void* logits, int dtype, int64_t outer, int64_t C, int
  *   position_loss (optional) fp32 [outer][inner]
  *   dlogits       (optional) gradient of `loss` times *upstream (1 if NULL); element (o, c, i) at o*ld_d + c*inner + i, dtype of
  *                 logits.  flags bit1: upstream has one value per position (not with bit0): gradient of position_loss.
- * flags bit2 (upstream and dlogits given, no other output): dlogits already holds the gradient for an upstream of 1, and the
- * call leaves it as it is if *upstream is 1 -- a backward pass that finds the gradient of the forward pass still right.
+ * flags bit2 (upstream and dlogits given, no other output): dlogits already holds the gradient for an upstream of 1, written by a
+ * call with the same arguments, and the call leaves it as it is if *upstream is 1 -- a backward pass that finds the gradient of
+ * the forward pass still right.  `workspace` has to be that call's, with its contents.
  * values_dtype fp32 or bf16, index_bytes 4 or 8 (int32 / int64).  Deterministic. */
 size_t segk_distill_workspace(int64_t outer, int64_t C, int64_t inner);
 int segk_distill(const void* logits, int dtype, int64_t outer, int64_t C, int64_t inner, int64_t ld, const void* values, int values_dtype,

@@ -66,6 +66,23 @@ def test_rows(V, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [4100, 8193, 16385, 32769, 65537, 131073])
+def test_many_long_rows(V, dtype):
+    """Rows that one workgroup each works on (few rows are shared by several): every row of a group of five again and again."""
+    z, values, indices, lse = problem(5, V, 6, seed=V, dtype=dtype, T=2.0)
+    indices[3] = -1
+    loss, grad, counted, lerr, gerr = loss_and_gradient(z, values, indices, lse, 2.0)
+    again = lambda t: t.repeat(40, *([1] * (t.dim() - 1))).cuda()   # noqa: E731
+    x = again(z).requires_grad_()
+    got = distill_loss_topk(x, TopLogits(again(values), again(indices), again(lse)), temperature=2.0, reduction="none")
+    got.sum().backward()
+    assert bool(((got.detach().double().cpu().view(40, 5) - loss).abs() <= lerr + 2.0 ** -23 * loss).all())
+    # (rows of odd length begin at other places of a 16-byte piece and add up in another order: within the bounds, not to the bit)
+    bound, grad = (gerr + (half_step(dtype) + 2.0 ** -21) * grad.abs()).cuda(), grad.cuda()
+    assert bool(((x.grad.view(40, 5, V).double() - grad).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("V,k", [(70, 64), (64, 64), (5000, 64), (40, 40), (6, 6)])
 def test_many_entries(V, k, dtype):
     z, values, indices, lse = problem(6, V, k, seed=k, dtype=dtype, T=1.5)

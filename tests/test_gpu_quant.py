@@ -65,7 +65,8 @@ def test_non_finite_values_and_zeros():
 
 SHAPES = [(1, 1, 1), (1, 128, 16), (1, 1664, 1000), (1, 8192, 512), (2, 100, 33), (4, 513, 80), (5, 640, 1030), (8, 4096, 250), (15, 129, 17), (16, 256, 64),
           (17, 300, 65), (33, 1000, 127), (37, 1664, 1000), (64, 384, 128), (65, 2000, 129), (100, 77, 300), (128, 512, 128), (129, 1280, 255), (200, 3000, 100),
-          (255, 640, 257), (256, 896, 256), (257, 1152, 513), (300, 64, 2000), (1000, 32, 90), (513, 2048, 512), (2049, 130, 130), (1, 20000, 40), (520, 8192, 300)]
+          (255, 640, 257), (256, 896, 256), (257, 1152, 513), (300, 64, 2000), (1000, 32, 90), (513, 2048, 512), (2049, 130, 130), (1, 20000, 40), (520, 8192, 300), (4, 20000, 50),
+          (2, 300, 5000), (20, 1100, 4500), (3, 2500, 4097)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])

@@ -104,8 +104,8 @@ def test_c_entry_points_refuse_bad_arguments_without_a_gpu():
             _lib.call("segk_mxfp4_dequantize", o["dt"], o["c"], o["s"], o["rows"], o["cols"], o["x"], o["ld"], 0, None)
     base = dict(x=4096, dt=BF16, ld=64, xc=None, xs=None, M=4, K=64, wc=4096, ws=4096, N=8, b=None, y=4096, ydt=F32, ldy=8, ws_=4096, wsb=1 << 20, d=0, st=None)
     for kw, text in ((dict(x=None), "either"), (dict(xc=4096), "either"), (dict(M=0), "shape"), (dict(K=0), "shape"), (dict(N=0), "shape"), (dict(wc=None), "null"),
-                     (dict(wc=4100), "16-byte"), (dict(y=None), "null"), (dict(ydt=3), "dtype"), (dict(ldy=7), "ld"), (dict(wsb=16), "SEGK_EWORKSPACE"),
-                     (dict(ws_=None), "SEGK_EWORKSPACE"), (dict(ws_=4104), "16-byte"), (dict(x=None, xc=4096), "null"), (dict(dt=2), "dtype"), (dict(ld=10), "ld")):
+                     (dict(wc=4100), "16-byte"), (dict(y=None), "null"), (dict(ydt=3), "dtype"), (dict(ldy=7), "ld"), (dict(M=5, wsb=16), "SEGK_EWORKSPACE"),
+                     (dict(M=5, ws_=None), "SEGK_EWORKSPACE"), (dict(M=5, ws_=4104), "16-byte"), (dict(x=None, xc=4096), "null"), (dict(dt=2), "dtype"), (dict(ld=10), "ld")):
         with pytest.raises(_lib.SegkError, match=text):
             _lib.call("segk_mxfp4_linear", *{**base, **kw}.values())
     assert _lib.query("segk_mxfp4_codes_bytes", 3, 129) == 3 * 128 and _lib.query("segk_mxfp4_scales_bytes", 3, 129) == 24
