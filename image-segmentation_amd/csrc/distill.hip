@@ -36,7 +36,8 @@ struct DistillArgs {
     float T, invT, weight;
     const float* upstream;     // gradient that reaches the loss: none (1), one value, or one for each position
     int up_each, skip_if_one;
-    const int* counts;         // partial counts of the positions with a kept logit (mean), or none (sum)
+    int* counts;               // partial counts of the positions with a kept logit (mean), or none (sum)
+    int count_here, log_kp;    // few rows: so many rows are counted by whoever needs the number (0: counts hold it)
     float* row_loss;           // loss of each position
     float* partial;            // sums that the finalize kernel adds (thread-per-position kernel)
     void* dz;
@@ -45,20 +46,34 @@ struct DistillArgs {
 
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
+// Reductions over a wave with data moved between lanes by the ALU (DPP): six dependent instructions, where shuffles through LDS
+// take several hundred cycles.  The result is the same in every lane.
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t lanes(uint32_t other, uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)other, (int)v, CTRL, ROWS, 0xF, false);
 }
-__device__ __forceinline__ int wave_sum_i(int v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
+template <typename V, typename F> __device__ __forceinline__ V wave_all(V v, V nothing, F&& f) {
+    const uint32_t none = __builtin_bit_cast(uint32_t, nothing);
+    auto step = [&](uint32_t moved) { v = f(v, __builtin_bit_cast(V, moved)); };
+    step(lanes<0x111, 0xF>(none, __builtin_bit_cast(uint32_t, v)));       // from 1, 2, 4, 8 lanes below, within 16
+    step(lanes<0x112, 0xF>(none, __builtin_bit_cast(uint32_t, v)));
+    step(lanes<0x114, 0xF>(none, __builtin_bit_cast(uint32_t, v)));
+    step(lanes<0x118, 0xF>(none, __builtin_bit_cast(uint32_t, v)));
+    step(lanes<0x142, 0xA>(none, __builtin_bit_cast(uint32_t, v)));       // lane 15 into the next 16, lane 31 into the upper half
+    step(lanes<0x143, 0xC>(none, __builtin_bit_cast(uint32_t, v)));
+    return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
+__device__ __forceinline__ float wave_max(float v) { return wave_all(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); }); }
+__device__ __forceinline__ float sum_wave(float v) { return wave_all(v, 0.f, [](float a, float b) { return a + b; }); }
+__device__ __forceinline__ int wave_sum_i(int v) { return wave_all(v, 0, [](int a, int b) { return a + b; }); }
 
 // the class of a kept logit; -1 where it is none of [0, V): such an entry does not exist
 __device__ __forceinline__ int load_class(const DistillArgs& a, int64_t at) {
     const int64_t i = a.idx64 ? static_cast<const int64_t*>(a.idx)[at] : (int64_t) static_cast<const int32_t*>(a.idx)[at];
+    return i >= 0 && i < a.V ? (int)i : -1;
+}
+// the same with the type known: a branch on it between two loads would make the second wait for the first
+template <typename I> __device__ __forceinline__ int load_class_as(const DistillArgs& a, int64_t at) {
+    const I i = static_cast<const I*>(a.idx)[at];
     return i >= 0 && i < a.V ? (int)i : -1;
 }
 __device__ __forceinline__ float load_kept(const DistillArgs& a, int64_t at) {
@@ -66,7 +81,7 @@ __device__ __forceinline__ float load_kept(const DistillArgs& a, int64_t at) {
 }
 // Rows (of k contiguous entries) with at least one kept logit among every `step`-th group of 64 / kp rows from `first` on, for a
 // whole wave, four groups in flight
-__device__ __forceinline__ int count_rows(const DistillArgs& a, int64_t rows, int log_kp, int64_t first, int64_t step, int lane) {
+template <typename I> __device__ __forceinline__ int count_rows_as(const DistillArgs& a, int64_t rows, int log_kp, int64_t first, int64_t step, int lane) {
     const int per = 64 >> log_kp, j = lane & ((1 << log_kp) - 1);
     const int64_t groups = (rows + per - 1) / per;
     int n = 0;
@@ -75,7 +90,7 @@ __device__ __forceinline__ int count_rows(const DistillArgs& a, int64_t rows, in
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const int64_t row = (g + u * step) * per + (lane >> log_kp);
-            have[u] = j < a.k && row < rows && load_class(a, row * a.k + j) >= 0;
+            have[u] = load_class_as<I>(a, (row < rows ? row : 0) * a.k + (j < a.k ? j : 0)) >= 0 && j < a.k && row < rows;
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
@@ -87,12 +102,20 @@ __device__ __forceinline__ int count_rows(const DistillArgs& a, int64_t rows, in
     return wave_sum_i(n);
 }
 
-// the sum of the partial counts, at least 1; every lane of the wave has to call it
-__device__ __forceinline__ int count_of(const int* __restrict__ counts) {
+__device__ __forceinline__ int count_rows(const DistillArgs& a, int64_t rows, int log_kp, int64_t first, int64_t step, int lane) {
+    return a.idx64 ? count_rows_as<int64_t>(a, rows, log_kp, first, step, lane) : count_rows_as<int32_t>(a, rows, log_kp, first, step, lane);
+}
+
+// the number of positions with a kept logit, at least 1; every lane of the wave has to call it
+__device__ __forceinline__ int count_of(const DistillArgs& a) {
     int n = 0;
+    if (a.count_here) {
+        n = count_rows(a, a.count_here, a.log_kp, 0, 1, threadIdx.x & 63);
+    } else {
 #pragma unroll
-    for (int i = 0; i < kCountBlocks / 64; ++i) n += counts[i * 64 + (threadIdx.x & 63)];
-    n = wave_sum_i(n);
+        for (int i = 0; i < kCountBlocks / 64; ++i) n += a.counts[i * 64 + (threadIdx.x & 63)];
+        n = wave_sum_i(n);
+    }
     return n > 0 ? n : 1;
 }
 // the same for VP neighbouring positions: 16-byte loads for four of them
@@ -125,7 +148,7 @@ template <int VP> __device__ __forceinline__ void load_kepts(const DistillArgs& 
 // what multiplies T * (M q - p ...) of a position; every lane of the wave has to call it
 __device__ __forceinline__ float grad_scale(const DistillArgs& a, int64_t position) {
     float g = a.weight * a.T;
-    if (a.counts) g /= (float)count_of(a.counts);
+    if (a.counts) g /= (float)count_of(a);
     if (a.upstream) g *= a.upstream[a.up_each ? position : 0];
     return g;
 }
@@ -252,11 +275,11 @@ __device__ __forceinline__ Kept kept_entries(const DistillArgs& a, int64_t row, 
     } else {
         const float top = wave_max(t);
         const float x = cls >= 0 && top != -INFINITY ? fast_exp2((t - top) * c) : 0.f;
-        const float sum = wave_sum(x);
+        const float sum = sum_wave(x);
         e.p = sum == 0.f ? 0.f : x / sum;
         e.lp = (t - top) * c - log2f(sum);
     }
-    const float mass = wave_sum(e.p);
+    const float mass = sum_wave(e.p);
     e.total = e.p;
     bool first = cls >= 0;
     for (int j = 0; j < a.k; ++j) {
@@ -272,7 +295,7 @@ __device__ __forceinline__ Kept kept_entries(const DistillArgs& a, int64_t row, 
     if (!(e.rest > kRestFloor) || distinct == a.V) e.rest = 0.f;
     e.mass = mass + e.rest;
     e.top = wave_max(first ? e.z : -INFINITY);
-    e.sum = wave_sum(first && e.top != -INFINITY ? exp_over(e.z, e.top, c) : 0.f);
+    e.sum = sum_wave(first && e.top != -INFINITY ? exp_over(e.z, e.top, c) : 0.f);
     return e;
 }
 // maximum and sum of exp over all classes, from those outside (ko, so) and those kept; share: exp of ko over the maximum
@@ -288,7 +311,7 @@ __device__ __forceinline__ Joined join(float ko, float so, float km, float sm, f
 __device__ __forceinline__ float kept_loss(const Kept& e, const Joined& w, float ko, float so, float c) {
     const float ls = log2f(w.sum);
     float l = e.p == 0.f ? 0.f : e.p * (e.lp - ((e.z - w.top) * c - ls));
-    l = wave_sum(l);
+    l = sum_wave(l);
     if (e.rest > 0.f) l += e.rest * (log2f(e.rest) - (log2f(so) + (ko - w.top) * c - ls));
     return l;
 }
@@ -363,7 +386,7 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(const DistillArgs a) {
         for (int i = 0; i < NCH; ++i)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) sw += exp_over(x[i].get(v), base, c);
-        sw = wave_sum(sw);
+        sw = sum_wave(sw);
         kw = m;
     } else {
         float m = -INFINITY;                              // of this lane
@@ -390,7 +413,7 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(const DistillArgs a) {
             for (int v = 0; v < VEC; ++v) sw += exp_over(y.get(v), base, c);
         }
         kw = wave_max(m);
-        sw = wave_sum(m == -INFINITY ? sw : sw * exp_over(m, kw, c));      // sw of an empty lane is 0 (or NaN, which stays)
+        sw = sum_wave(m == -INFINITY ? sw : sw * exp_over(m, kw, c));      // sw of an empty lane is 0 (or NaN, which stays)
     }
     if (lane == 0) { sh_k[wave] = kw; sh_s[wave] = sw; }
     __syncthreads();
@@ -497,7 +520,7 @@ __global__ __launch_bounds__(256) void distill_share_kernel(const DistillArgs a,
             for (int v = 0; v < VEC; ++v) s += exp_over(y[u].get(v), base, c);
     }
     const float k = wave_max(m);
-    s = wave_sum(m == -INFINITY ? s : s * exp_over(m, k, c));
+    s = sum_wave(m == -INFINITY ? s : s * exp_over(m, k, c));
     if (lane == 0) { sh_k[wave] = k; sh_s[wave] = s; }
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -524,7 +547,7 @@ __global__ __launch_bounds__(64) void distill_join_kernel(const DistillArgs a, c
     }
     const float* in = parts + (row * kShares + lane) * 2;
     const float k = lane < shares ? in[0] : -INFINITY, s = lane < shares ? in[1] : 0.f;
-    const float ko = wave_max(k), so = wave_sum(k == -INFINITY ? s : s * exp_over(k, ko, c));
+    const float ko = wave_max(k), so = sum_wave(k == -INFINITY ? s : s * exp_over(k, ko, c));
     const Kept e = kept_entries<T>(a, row, z, cls, lane, c);
     const Joined w = join(ko, so, e.top, e.sum, c);
     const float l = kept_loss(e, w, ko, so, c);
@@ -718,7 +741,7 @@ __global__ __launch_bounds__(256) void distill_pixels_kernel(const DistillArgs a
         }
     }
     if (a.partial) {
-        block = wave_sum(block);
+        block = sum_wave(block);
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = block;
         __syncthreads();
         if (threadIdx.x == 0) a.partial[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
@@ -735,28 +758,33 @@ __global__ __launch_bounds__(256) void distill_count_rows_kernel(const DistillAr
     __syncthreads();
     if (threadIdx.x == 0) counts[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
 }
-// Planes: a thread takes 8 positions at a time and reads entry after entry until each has one (the first decides most of them); all
-// 8 loads of an entry are in flight together.
-__global__ __launch_bounds__(1024) void distill_count_planes_kernel(const DistillArgs a, int64_t positions, int* __restrict__ counts) {
+// Planes: a thread takes 16 positions at a time and reads entry after entry until each has one (the first decides most of them); all
+// 16 loads of an entry are in flight together.
+template <typename I> __global__ __launch_bounds__(1024) void distill_count_planes_kernel(const DistillArgs a, int64_t positions, int* __restrict__ counts) {
     __shared__ int red[16];
-    constexpr int U = 8;
+    constexpr int U = 16;
     int n = 0;
     const int64_t per = (positions + kCountBlocks - 1) / kCountBlocks, lo = per * blockIdx.x, hi = lo + per < positions ? lo + per : positions;
     for (int64_t p = lo + threadIdx.x; p < hi; p += 1024 * U) {
-        int64_t at[U];
+        int64_t at[U], o = p / a.inner, i = p - o * a.inner;
         int c[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int64_t pu = p + u * 1024 < hi ? p + u * 1024 : p;
-            const int64_t o = positions < (1ll << 31) ? (uint32_t)pu / (uint32_t)a.inner : pu / a.inner;
-            at[u] = o * a.k * a.inner + (pu - o * a.inner) * a.ts_p;
+            at[u] = p + u * 1024 < hi ? o * a.k * a.inner + i * a.ts_p : at[0];
             c[u] = -1;
+            i += 1024;
+            if (a.inner >= 1024) {
+                if (i >= a.inner) { i -= a.inner; ++o; }
+            } else {
+                o += i / a.inner;
+                i %= a.inner;
+            }
         }
         for (int j = 0; j < a.k; ++j) {
             int lowest = 0;
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int d = load_class(a, at[u] + j * a.ts_c);
+                const int d = load_class_as<I>(a, at[u] + j * a.ts_c);
                 c[u] = d > c[u] ? d : c[u];
                 lowest = c[u] < lowest ? c[u] : lowest;
             }
@@ -793,10 +821,9 @@ __global__ __launch_bounds__(1024) void distill_collect_kernel(const float* __re
     s = block_sum_1024(s, red);
     if (threadIdx.x == 0) out[blockIdx.x] = (float)s;
 }
-__global__ __launch_bounds__(1024) void distill_finalize_kernel(const float* __restrict__ v, int n, const int* __restrict__ counts,
-                                                                float* __restrict__ loss) {
+__global__ __launch_bounds__(1024) void distill_finalize_kernel(const DistillArgs a, const float* __restrict__ v, int n, float* __restrict__ loss) {
     __shared__ double red[16];
-    const int m = counts ? count_of(counts) : 1;
+    const int m = a.counts ? count_of(a) : 1;
     double s = 0.0;
     for (int i = threadIdx.x; i < n; i += 1024) s += (double)v[i];
     s = block_sum_1024(s, red);
@@ -853,7 +880,7 @@ __global__ __launch_bounds__(NT) void top_rows_kernel(const T* __restrict__ z, i
         for (int i = 0; i < NCH; ++i)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) sw += exp_over(x[i].get(v), base, c);
-        sw = wave_sum(sw);
+        sw = sum_wave(sw);
     } else {
         for (int g = threadIdx.x; g < r.pieces; g += NT) {
             const Piece<T> y = r.load(g);
@@ -869,7 +896,7 @@ __global__ __launch_bounds__(NT) void top_rows_kernel(const T* __restrict__ z, i
             for (int v = 0; v < VEC; ++v) sw += exp_over(y.get(v), base, c);
         }
         kw = wave_max(m);
-        sw = wave_sum(m == -INFINITY ? sw : sw * exp_over(m, kw, c));
+        sw = sum_wave(m == -INFINITY ? sw : sw * exp_over(m, kw, c));
     }
     sh_m[threadIdx.x] = m;
     if (lane == 0) { sh_k[wave] = kw; sh_s[wave] = sw; }
@@ -1248,13 +1275,15 @@ extern "C" int segk_distill(const void* logits, int dtype, int64_t outer, int64_
         a.inner = 1; a.ts_c = 1; a.ts_p = k;
         a.row_loss = position_loss ? position_loss : partial;
     }
-    if (mean && !skip) {
+    while ((1 << a.log_kp) < k) ++a.log_kp;
+    // up to 1024 entries (16 loads of a wave, all in flight) are counted where the number is needed instead of in a launch of their own
+    if (mean && inner == 1 && outer << a.log_kp <= 1024) a.count_here = (int)outer;
+    if (mean && !skip && !a.count_here) {
         if (inner == 1) {
-            int log_kp = 0;
-            while ((1 << log_kp) < k) ++log_kp;
-            hipLaunchKernelGGL(distill_count_rows_kernel, dim3(kCountBlocks), dim3(256), 0, st, a, outer, log_kp, counts);
+            hipLaunchKernelGGL(distill_count_rows_kernel, dim3(kCountBlocks), dim3(256), 0, st, a, outer, a.log_kp, counts);
         } else {
-            hipLaunchKernelGGL(distill_count_planes_kernel, dim3(kCountBlocks), dim3(1024), 0, st, a, outer * inner, counts);
+            if (a.idx64) hipLaunchKernelGGL(distill_count_planes_kernel<int64_t>, dim3(kCountBlocks), dim3(1024), 0, st, a, outer * inner, counts);
+            else hipLaunchKernelGGL(distill_count_planes_kernel<int32_t>, dim3(kCountBlocks), dim3(1024), 0, st, a, outer * inner, counts);
         }
         SEGK_LAUNCH_CHECK();
     }
@@ -1286,7 +1315,7 @@ extern "C" int segk_distill(const void* logits, int dtype, int64_t outer, int64_
             v = collected;
             n = kCollect;
         }
-        hipLaunchKernelGGL(distill_finalize_kernel, dim3(1), dim3(1024), 0, st, v, (int)n, (const int*)a.counts, loss);
+        hipLaunchKernelGGL(distill_finalize_kernel, dim3(1), dim3(1024), 0, st, a, v, (int)n, loss);
         SEGK_LAUNCH_CHECK();
     }
     return SEGK_OK;

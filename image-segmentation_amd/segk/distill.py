@@ -54,17 +54,12 @@ def _canonical(x, dim):
     moved = inner > 1 and C > PLANE_CLASSES
     if moved:
         x, outer, inner = x.movedim(dim, -1), outer * inner, 1
+    if x.is_contiguous():
+        return x, outer, C, inner, C * inner, moved
     x = x.reshape(outer, C, inner)
     if (C > 1 and x.stride(1) != inner) or (inner > 1 and x.stride(2) != 1) or (outer > 1 and x.stride(0) < C * inner):
         x = x.contiguous()
     return x, outer, C, inner, (x.stride(0) if outer > 1 else C * inner), moved
-
-
-def _restore(y, shape, dim, n, moved):
-    """The kernels' [outer][n][inner] (or [outer * inner][n] if the classes were moved) in the caller's order of dimensions."""
-    if moved:
-        return y.reshape(shape[:dim] + shape[dim + 1:] + (n,)).movedim(-1, dim)
-    return y.reshape(shape[:dim] + (n,) + shape[dim + 1:])
 
 
 def top_logits(logits, k, dim=1, temperature=1.0):
@@ -78,19 +73,23 @@ def top_logits(logits, k, dim=1, temperature=1.0):
     C = logits.shape[dim]
     if not 1 <= k <= min(MAX_K, C):
         raise ValueError(f"k has to be between 1 and min({MAX_K}, {C} classes), got {k}")
-    z = logits.detach()
-    rest = z.shape[:dim] + z.shape[dim + 1:]
+    z = logits.detach() if logits.requires_grad else logits
+    shape = z.shape
+    rest = shape[:dim] + shape[dim + 1:]
     if not z.is_cuda or z.numel() == 0:
         return _host_top(z, k, dim, temperature)
     z, outer, C, inner, ld, moved = _canonical(z.float() if z.dtype == torch.float16 else z, dim)
-    values = torch.empty((outer, k, inner), dtype=z.dtype, device=z.device)
-    indices = torch.empty((outer, k, inner), dtype=torch.int32, device=z.device)
+    kept = rest + (k,) if moved else shape[:dim] + (k,) + shape[dim + 1:]
+    values = torch.empty(kept, dtype=z.dtype, device=z.device)
+    indices = torch.empty(kept, dtype=torch.int32, device=z.device)
     lse = torch.empty(rest, dtype=torch.float32, device=z.device)
     dev, st = _env(z)
     with ops._streamed("top logits", z.numel() * z.element_size()):
         call("segk_top_logits", z.data_ptr(), dt(z.dtype), outer, C, inner, ld, k, temperature, values.data_ptr(), indices.data_ptr(),
              lse.data_ptr(), dev, st)
-    return TopLogits(_restore(values, logits.shape, dim, k, moved).to(logits.dtype), _restore(indices, logits.shape, dim, k, moved), lse)
+    if moved:
+        values, indices = values.movedim(-1, dim), indices.movedim(-1, dim)
+    return TopLogits(values if z.dtype == logits.dtype else values.to(logits.dtype), indices, lse)
 
 
 class _DistillFn(torch.autograd.Function):
@@ -103,13 +102,14 @@ class _DistillFn(torch.autograd.Function):
         k = values.shape[dim]
         if moved:
             values, indices = values.movedim(dim, -1), indices.movedim(dim, -1)
-        values, indices = values.contiguous(), indices.contiguous()
-        lse = None if lse is None else lse.contiguous()
+        values = values if values.is_contiguous() else values.contiguous()
+        indices = indices if indices.is_contiguous() else indices.contiguous()
+        lse = lse if lse is None or lse.is_contiguous() else lse.contiguous()
         ctx.meta = (outer, C, inner, ld, moved, k, dim, float(temperature), float(weight), reduction, logits.shape, logits.dtype)
         rest = logits.shape[:dim] + logits.shape[dim + 1:]
         each = reduction == "none"
         out = torch.empty(rest if each else (), dtype=torch.float32, device=z.device)
-        dz = torch.empty((outer, C, inner), dtype=z.dtype, device=z.device) if want_grad and not each else None
+        dz = _DistillFn._gradient(ctx.meta, z) if want_grad and not each else None
         # a workspace of its own for every call: launches on other streams and replays of captured graphs never share one
         ws = torch.empty(query("segk_distill_workspace", outer, C, inner), dtype=torch.uint8, device=z.device)
         _DistillFn._launch(ctx.meta, z, values, indices, lse, None, MEAN if reduction == "mean" else 0, None if each else out, out if each else None, dz, ws)
@@ -117,6 +117,12 @@ class _DistillFn(torch.autograd.Function):
             ctx.save_for_backward(z, values, indices, lse)
             ctx.dz, ctx.ws = dz, ws
         return out
+
+    @staticmethod
+    def _gradient(meta, z):
+        """Memory for dlogits, [outer][C][inner] (rows with the classes last if they were moved), in the caller's shape."""
+        moved, dim, shape = meta[4], meta[6], meta[10]
+        return torch.empty(shape[:dim] + shape[dim + 1:] + (shape[dim],) if moved else shape, dtype=z.dtype, device=z.device)
 
     @staticmethod
     def _launch(meta, z, values, indices, lse, upstream, flags, loss, each, dz, ws):
@@ -136,12 +142,14 @@ class _DistillFn(torch.autograd.Function):
         dz, ctx.dz, ws, ctx.ws = ctx.dz, None, ctx.ws, None      # handed over once; a second backward pass computes its own
         flags = EACH if reduction == "none" else MEAN if reduction == "mean" else 0
         if dz is None:
-            dz = torch.empty((outer, C, inner), dtype=z.dtype, device=z.device)
+            dz = _DistillFn._gradient(ctx.meta, z)
             ws = torch.empty(query("segk_distill_workspace", outer, C, inner), dtype=torch.uint8, device=z.device)
         else:
             flags |= SKIP
-        _DistillFn._launch(ctx.meta, z, values, indices, lse, g.float().contiguous(), flags, None, None, dz, ws)
-        return (_restore(dz, shape, dim, C, moved).to(in_dtype),) + (None,) * 8
+        _DistillFn._launch(ctx.meta, z, values, indices, lse, g if g.dtype == torch.float32 and g.is_contiguous() else g.float().contiguous(), flags, None, None, dz, ws)
+        if moved:
+            dz = dz.movedim(-1, dim)
+        return (dz if dz.dtype == in_dtype else dz.to(in_dtype),) + (None,) * 8
 
 
 def distill_loss_topk(pred, target, temperature=1.0, reduction="mean", dim=1, weight=1.0):
@@ -186,7 +194,9 @@ def distill_loss_topk(pred, target, temperature=1.0, reduction="mean", dim=1, we
         values = values.float()
     dt(torch.float32 if pred.dtype == torch.float16 else pred.dtype), dt(values.dtype)       # refuses what the kernels do not read
     want_grad = torch.is_grad_enabled() and pred.requires_grad
-    return _DistillFn.apply(pred, values, indices, None if lse is None else lse.float(), dim, temperature, weight, reduction, want_grad)
+    if lse is not None and lse.dtype != torch.float32:
+        lse = lse.float()
+    return _DistillFn.apply(pred, values, indices, lse, dim, temperature, weight, reduction, want_grad)
 
 
 # ------------------------------------------------------------------------------------ host tensors

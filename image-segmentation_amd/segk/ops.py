@@ -66,9 +66,12 @@ class Act:
         return Act(x.permute(0, 2, 3, 1).contiguous().to(dtype or x.dtype))
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
 def _env(t):
     dev = t.device.index if t.device.index is not None else torch.cuda.current_device()
-    return dev, torch.cuda.current_stream(dev).cuda_stream
+    return dev, _raw_stream(dev)         # the handle itself: a torch.cuda.Stream object costs 2 us per call
 
 
 _workspaces = {}

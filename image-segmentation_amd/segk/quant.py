@@ -55,11 +55,13 @@ def _rows(x, what):
         raise ValueError(f"{what} has no columns")
     if torch.is_grad_enabled() and x.requires_grad:
         raise RuntimeError(f"{what} requires a gradient and 4-bit rounding has none: call under torch.no_grad() or detach it")
-    x = x.detach()
+    if x.requires_grad:
+        x = x.detach()
     if x.dtype == torch.float16:
         x = x.float()
     dt(x.dtype)
-    x = x.reshape(-1, x.shape[-1])
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
     if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
         x = x.contiguous()
     return x, (x.stride(0) if x.shape[0] > 1 else x.shape[1])
@@ -126,7 +128,8 @@ def mxfp4_linear(x, w, bias=None, out_dtype=None):
             raise ValueError(f"bias has to be a floating point tensor [{N}] on the device of w")
         if torch.is_grad_enabled() and bias.requires_grad:
             raise RuntimeError("bias requires a gradient: call under torch.no_grad() or detach it")
-        bias = bias.detach().float().contiguous()
+        if bias.dtype != torch.float32 or bias.requires_grad or not bias.is_contiguous():
+            bias = bias.detach().float().contiguous()
     if w.codes.device.type != "cuda":
         xq = _host_dequantize(x if packed else MXFP4(*_host_quantize(x), K))
         y = xq @ _host_dequantize(w).t()
@@ -140,7 +143,9 @@ def mxfp4_linear(x, w, bias=None, out_dtype=None):
             call("segk_mxfp4_linear", None if packed else x.data_ptr(), 0 if packed else dt(x.dtype), 0 if packed else ld,
                  x.codes.data_ptr() if packed else None, x.scales.data_ptr() if packed else None, M, K, w.codes.data_ptr(), w.scales.data_ptr(), N,
                  ops._p(bias), y.data_ptr(), dt(y.dtype), N, ops._p(ws), nbytes, dev, st)
-    return y.to(out_dtype).reshape(lead + (N,))
+    if y.dtype != out_dtype:
+        y = y.to(out_dtype)
+    return y if len(lead) == 1 else y.reshape(lead + (N,))
 
 
 # ------------------------------------------------------------------------------------ host tensors

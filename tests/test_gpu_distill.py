@@ -196,7 +196,9 @@ def test_strides_offsets_and_dimensions(V, dtype):
     one = z[:1].expand(6, V).cuda()                                                              # stride 0
     same = TopLogits(target.values[:1].expand(6, 3), target.indices[:1].expand(6, 3), target.lse[:1].expand(6))
     alone = distill_loss_topk(one[:1], TopLogits(target.values[:1], target.indices[:1], target.lse[:1]), reduction="none")
-    assert torch.equal(distill_loss_topk(one, same, reduction="none"), alone.expand(6))
+    # the copies begin at other places of a 16-byte piece and add up in another order: either result is within lerr of the exact one
+    lerr = float(loss_and_gradient(z[:1], values[:1], indices[:1], lse[:1], 1.0)[3])
+    assert float((distill_loss_topk(one, same, reduction="none") - alone).abs().max()) <= 2 * lerr
 
 
 def test_half_precision_logits_and_values_types():
