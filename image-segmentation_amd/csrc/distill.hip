@@ -184,6 +184,44 @@ template <typename T, int N> __device__ __forceinline__ void stay_packed(Piece<T
     }
 }
 
+// The greatest element of a lane's pieces.  Pairs of bf16 are compared as 16-bit integers, which order positive floats as the floats
+// do and put all negative ones below them; a lane that has no positive element looks again, as floats.  (A quarter of the
+// instructions; 4096 rows of 32000, selection: 61.3 -> 60.0 us.)
+template <typename T, int N> __device__ __forceinline__ float lane_max(const Piece<T> (&x)[N]) {
+    float m = -INFINITY;
+    if constexpr (sizeof(T) == 2) {
+        typedef short s16x2 __attribute__((ext_vector_type(2)));
+        s16x2 best = {-32768, -32768};
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) best = __builtin_elementwise_max(best, __builtin_bit_cast(s16x2, x[i].w[w]));
+        const int top = best[0] > best[1] ? best[0] : best[1];
+        if (top >= 0) return __uint_as_float((uint32_t)top << 16);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int v = 0; v < Piece<T>::VEC; ++v) m = fmaxf(m, x[i].get(v));
+    return m;
+}
+// whether a piece may have an element of at least `bound` (certain for fp32; never a miss)
+template <typename T> __device__ __forceinline__ bool may_reach(const Piece<T>& x, float bound) {
+    if constexpr (sizeof(T) == 2) {
+        if (bound > 0.f) {
+            typedef short s16x2 __attribute__((ext_vector_type(2)));
+            const short b = (short)(__float_as_uint(bound) >> 16);
+            s16x2 best = __builtin_bit_cast(s16x2, x.w[0]);
+#pragma unroll
+            for (int w = 1; w < 4; ++w) best = __builtin_elementwise_max(best, __builtin_bit_cast(s16x2, x.w[w]));
+            return best[0] >= b || best[1] >= b;
+        }
+        return true;
+    } else {
+        return fmaxf(fmaxf(x.get(0), x.get(1)), fmaxf(x.get(2), x.get(3))) >= bound;
+    }
+}
+
 template <typename T> struct Row {
     const T* p;      // element 0
     int phase, V, pieces;
@@ -368,18 +406,14 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(const DistillArgs a) {
     // ---- maximum and sum of the classes that were not kept
     float kw = -INFINITY, sw = 0.f;
     if constexpr (NCH > 0) {
-        float m = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) {
+        for (int i = 0; i < NCH; ++i)
             for_kept<VEC>(cls, r.phase, i * NT + wave * 64, lane, [&](bool here, int v, int) {
 #pragma unroll
                 for (int u = 0; u < VEC; ++u)
                     if (here && u == v) x[i].clear(u);
             });
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) m = fmaxf(m, x[i].get(v));
-        }
-        m = wave_max(m);
+        const float m = wave_max(lane_max<T, NCH>(x));
         const float base = m == -INFINITY ? 0.f : m;
         stay_packed(x);
 #pragma unroll
@@ -868,10 +902,7 @@ __global__ __launch_bounds__(NT) void top_rows_kernel(const T* __restrict__ z, i
 #pragma unroll
                 for (int w = 0; w < 4; ++w) x[i].w[w] = sizeof(T) == 4 ? 0xFF800000u : 0xFF80FF80u;
         }
-#pragma unroll
-        for (int i = 0; i < NCH; ++i)
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) m = fmaxf(m, x[i].get(v));
+        m = lane_max<T, NCH>(x);
         const float mw = wave_max(m);
         kw = mw;
         const float base = mw == -INFINITY ? 0.f : mw;
@@ -955,6 +986,7 @@ __global__ __launch_bounds__(NT) void top_rows_kernel(const T* __restrict__ z, i
                 stay_packed(x);
 #pragma unroll
                 for (int i = 0; i < NCH; ++i) {
+                    if (!may_reach<T>(x[i], fb)) continue;
                     uint32_t hit = 0;
 #pragma unroll
                     for (int v = 0; v < VEC; ++v) hit |= x[i].get(v) >= fb ? 1u << v : 0u;
@@ -1144,12 +1176,13 @@ static int check_logits(const char* who, const void* z, int dtype, int64_t outer
                         float temperature) {
     SEGK_REQUIRE(z, SEGK_EINVAL, "%s: null pointer", who);
     SEGK_REQUIRE(dtype == SEGK_F32 || dtype == SEGK_BF16, SEGK_EINVAL, "%s: unknown dtype %d", who, dtype);
-    SEGK_REQUIRE(outer > 0 && C > 0 && inner > 0 && outer < (1ll << 31) && C < (1ll << 30) && inner < (1ll << 40), SEGK_ESHAPE, "%s: bad shape", who);
-    SEGK_REQUIRE(outer <= (1ll << 40) / inner, SEGK_ESHAPE, "%s: too many positions", who);
+    SEGK_REQUIRE(outer > 0 && C > 0 && inner > 0 && outer < (1ll << 31) && C < (1ll << 30) && inner < (1ll << 31), SEGK_ESHAPE, "%s: bad shape", who);
+    SEGK_REQUIRE(outer * inner < (1ll << 31), SEGK_ESHAPE, "%s: 2^31 positions and more", who);
     SEGK_REQUIRE(inner == 1 || C <= kPixelClasses, SEGK_ESHAPE, "%s: more than %d classes have to be the innermost dimension", who, kPixelClasses);
     SEGK_REQUIRE(ld >= C * inner, SEGK_ESHAPE, "%s: ld smaller than one row / image", who);
     SEGK_REQUIRE(k >= 1 && k <= kTopMax && k <= C, SEGK_ESHAPE, "%s: k must be between 1 and %d and at most the number of classes", who, kTopMax);
-    SEGK_REQUIRE(temperature > 0.f && temperature < INFINITY, SEGK_EINVAL, "%s: temperature must be positive and finite", who);
+    // so that neither 1 / T nor T^2 leaves the range of fp32
+    SEGK_REQUIRE(temperature >= 0x1p-40f && temperature <= 0x1p40f, SEGK_EINVAL, "%s: temperature must be between 2^-40 and 2^40", who);
     SEGK_REQUIRE(reinterpret_cast<uintptr_t>(z) % esize(dtype) == 0, SEGK_EALIGN, "%s: logits are not aligned to their type", who);
     return SEGK_OK;
 }

@@ -8,6 +8,7 @@
 //     scales [slices][rows][4 bytes]: the four scales of a row's slice are one dword, and those of neighbouring rows are
 //            neighbours, so a tile of rows gets its scales with coalesced loads
 #include "common.h"
+#include <atomic>
 #include <type_traits>
 
 namespace segk {
@@ -484,7 +485,15 @@ template <typename TO, int BM, int BN, int WM, int WN, bool WIDE> static int lau
     const int64_t tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN;
     SEGK_REQUIRE(tm * tn < (1ll << 31), SEGK_ESHAPE, "mxfp4_linear: too many tiles");
     auto kernel = mxfp4_tile_kernel<TO, BM, BN, WM, WN, WIDE>;
-    if (bytes > 65536) SEGK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if constexpr (bytes > 65536) {
+        static std::atomic<bool> allowed[64] = {};               // once per device
+        int dev = 0;
+        SEGK_HIP(hipGetDevice(&dev));
+        if (dev >= 64 || !allowed[dev].load(std::memory_order_acquire)) {
+            SEGK_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+            if (dev < 64) allowed[dev].store(true, std::memory_order_release);
+        }
+    }
     hipLaunchKernelGGL(kernel, dim3((unsigned)(tm * tn)), dim3(WM * WN * 64), bytes, st, a, (int)tm, (int)tn);
     SEGK_LAUNCH_CHECK();
     return SEGK_OK;
@@ -546,7 +555,6 @@ extern "C" int segk_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const 
         SEGK_REQUIRE(fused(M, K) || (workspace && workspace_bytes >= segk_mxfp4_linear_workspace(M, K, N)), SEGK_EWORKSPACE, "mxfp4_linear: workspace too small");
         SEGK_REQUIRE(aligned16(workspace), SEGK_EALIGN, "mxfp4_linear: workspace must be 16-byte aligned");
     } else if (const int rc = check_packed("mxfp4_linear", x_codes, x_scales)) return rc;
-    SEGK_REQUIRE((M + 15) / 16 < 65536, SEGK_ESHAPE, "mxfp4_linear: too many rows");
     SEGK_USE_DEVICE(dev);
     hipStream_t st = (hipStream_t)stream;
     const bool pack_inside = x && fused(M, K);

@@ -41,8 +41,8 @@ def _check(logits, dim, temperature):
         raise TypeError(f"logits of floating point type are expected, got {logits.dtype} with {logits.dim()} dimensions")
     if not -logits.dim() <= dim < logits.dim():
         raise IndexError(f"dimension {dim} is out of range for logits with {logits.dim()} dimensions")
-    if not (isinstance(temperature, (int, float)) and 0 < temperature < math.inf):
-        raise ValueError(f"temperature has to be positive and finite, got {temperature}")
+    if not (isinstance(temperature, (int, float)) and 2.0 ** -40 <= temperature <= 2.0 ** 40):
+        raise ValueError(f"temperature has to be a number between 2^-40 and 2^40, got {temperature}")
     return dim % logits.dim()
 
 
@@ -64,8 +64,8 @@ def _canonical(x, dim):
 
 def top_logits(logits, k, dim=1, temperature=1.0):
     """The k greatest logits along `dim` (1 <= k <= min(64, classes)) as TopLogits(values, indices int32, lse): descending, ties to
-    the lower class, NaN as the greatest; lse = logsumexp(logits / temperature) over all classes, fp32.  float32, bfloat16 and
-    float16 logits; values keep their type.  Not differentiable: a teacher's answer is data.
+    the lower class, NaN as the greatest; lse = logsumexp(logits / temperature) over all classes, fp32 (NaN where a logit is NaN or
+    +infinity).  float32, bfloat16 and float16 logits; values keep their type.  Not differentiable: a teacher's answer is data.
 
     The class dimension may stand anywhere: last (rows of any number of classes, read where they are) or in front of others as in
     [N, C, H, W] (up to 32 classes read where they are, more are copied once into rows)."""
@@ -164,7 +164,8 @@ def distill_loss_topk(pred, target, temperature=1.0, reduction="mean", dim=1, we
     `weight` scales loss and gradient; it costs nothing, where multiplying the returned loss costs another pass over the logits.
 
     pred: float32, bfloat16 or float16, any strides; target: TopLogits or a tuple (values, indices[, lse]) with float32 / bfloat16 /
-    float16 values and int32 / int64 indices.  Returns float32; the gradient has pred's type.  Sums run in float32."""
+    float16 values and int32 / int64 indices.  Returns float32; the gradient has pred's type.  Sums run in float32;
+    log p carries the rounding of the kept lse, 2^-24 |lse|, so logits / T of some thousands leave no exact probabilities."""
     dim = _check(pred, dim, temperature)
     if reduction not in ("mean", "sum", "none"):
         raise ValueError('Reduction parameter unknown.')
@@ -207,9 +208,10 @@ def _host_top(z, k, dim, temperature):
         return TopLogits(z.new_empty(shape), torch.empty(shape, dtype=torch.int32, device=z.device),
                          torch.empty(z.shape[:dim] + z.shape[dim + 1:], dtype=torch.float32, device=z.device))
     indices = torch.sort(w, dim=dim, descending=True, stable=True).indices.narrow(dim, 0, k)
+    lse = torch.logsumexp(w / temperature, dim)
     # two-byte types are gathered as integers: torch's gather on the CPU turns their NaNs into other ones
     raw = z.view(torch.int16) if z.element_size() == 2 else z
-    return TopLogits(torch.gather(raw, dim, indices).view(z.dtype), indices.to(torch.int32), torch.logsumexp(w / temperature, dim).float())
+    return TopLogits(torch.gather(raw, dim, indices).view(z.dtype), indices.to(torch.int32), lse.masked_fill(lse == math.inf, math.nan).float())
 
 
 def _host_distill(pred, values, indices, lse, dim, T, weight, reduction):

@@ -106,11 +106,13 @@ int segk_argmax_dice(const void* logits, int logits_dtype, const int64_t* labels
  * beside the losses above.  Logits are `outer` images (rows) of C classes x `inner` positions: element (o, c, i) at
  * logits[o*ld + c*inner + i], ld >= C*inner; inner = 1 gives rows [outer][C] with the classes innermost, C*inner = an NCHW image
  * otherwise (C <= 32 then).  fp32 or bf16, aligned to their type only.  Kept logits: `values` and `indices` [outer][k][inner],
- * contiguous, 1 <= k <= min(64, C); `lse` [outer][inner] fp32 = log(sum over the classes of exp(logit / temperature)).
+ * contiguous, 1 <= k <= min(64, C); `lse` [outer][inner] fp32 = log(sum over the classes of exp(logit / temperature)).  Fewer than
+ * 2^31 positions, 2^-40 <= temperature <= 2^40.
  * ---------------------------------------------------------------------------------------------- */
 
 /* The k greatest logits of every position in descending order (NaN counts as greatest; ties: the lower class first), the classes
- * they belong to (int32) and, if lse is not NULL, the logsumexp of all classes.  values have the dtype of logits.
+ * they belong to (int32) and, if lse is not NULL, the logsumexp of all classes (NaN where a logit is NaN or +inf).  values have the dtype of
+ * logits.
  * Outputs 16-byte aligned.  One pass over the logits. */
 int segk_top_logits(const void* logits, int dtype, int64_t outer, int64_t C, int64_t inner, int64_t ld, int64_t k, float temperature,
                     void* values, int32_t* indices, float* lse, int dev, void* stream);
@@ -577,7 +579,8 @@ int segk_mxfp4_dequantize(int dtype, const void* codes, const void* scales, int6
 /* y[M][N] = x[M][K] w[N][K]^T + bias with both operands in packed form on the scaled matrix instructions, fp32 accumulation in an
  * order fixed by the shape (deterministic), one rounding to y's type.  x is given as a matrix, packed by the call as above, or as
  * x_codes / x_scales (the other NULL).  bias: fp32 [N] or NULL.
- * workspace: segk_mxfp4_linear_workspace(M, K, N) bytes, 16-byte aligned; contents need not be cleared. */
+ * M, N < 2^28, K < 2^24.  workspace: segk_mxfp4_linear_workspace(M, K, N) bytes (0 for one or two rows), 16-byte aligned; contents
+ * need not be cleared. */
 size_t segk_mxfp4_linear_workspace(int64_t M, int64_t K, int64_t N);
 int segk_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const void* x_codes, const void* x_scales, int64_t M, int64_t K,
                       const void* w_codes, const void* w_scales, int64_t N, const float* bias, void* y, int y_dtype, int64_t ldy,

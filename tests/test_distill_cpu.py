@@ -51,7 +51,8 @@ def test_host_top_logits_order_and_ties():
     z = torch.tensor([[1.0, 3.0, 3.0, -math.inf, 0.0, -0.0, math.nan, math.inf], [0.0] * 8])
     values, indices, lse = top_logits(z, 6)
     assert indices.tolist() == [[6, 7, 1, 2, 0, 4], [0, 1, 2, 3, 4, 5]] and indices.dtype == torch.int32
-    assert abs(float(lse[1]) - math.log(8)) < 1e-6
+    assert abs(float(lse[1]) - math.log(8)) < 1e-6 and math.isnan(float(lse[0]))
+    assert math.isnan(float(top_logits(torch.tensor([[1.0, math.inf]]), 1).lse)) and float(top_logits(torch.full((1, 3), -math.inf), 1).lse) == -math.inf
     z = torch.randn(2, 5, 3, 4)
     values, indices, lse = top_logits(z, 2, dim=1)
     v, i = top(z.permute(0, 2, 3, 1).reshape(-1, 5), 2)
@@ -79,8 +80,9 @@ def test_refusals():
     z, target = problem(4, 9, 3)
     with pytest.raises(ValueError, match="temperature"):
         distill_loss_topk(z, target, temperature=0.0)
-    with pytest.raises(ValueError, match="temperature"):
-        top_logits(z, 2, temperature=math.inf)
+    for t in (math.inf, math.nan, -1.0, 1e-20, 1e20, "2"):
+        with pytest.raises(ValueError, match="temperature"):
+            top_logits(z, 2, temperature=t)
     with pytest.raises(ValueError, match="Reduction parameter unknown."):
         distill_loss_topk(z, target, reduction="batch")
     with pytest.raises(IndexError):
@@ -117,7 +119,8 @@ def test_c_entry_points_refuse_bad_arguments_without_a_gpu():
     for kw, text in ((dict(z=None), "null"), (dict(dt=7), "dtype"), (dict(o=0), "shape"), (dict(c=0), "shape"), (dict(c=1 << 30), "shape"), (dict(ld=79), "ld"),
                      (dict(k=0), "k must"), (dict(k=65), "k must"), (dict(k=9, c=8, ld=8), "k must"), (dict(t=0.0), "temperature"), (dict(t=math.inf), "temperature"),
                      (dict(t=math.nan), "temperature"), (dict(z=4097), "aligned"), (dict(v=None), "null"), (dict(v=4100), "16-byte"), (dict(i=4, ld=320), "innermost"),
-                     (dict(o=1 << 30, i=1 << 20, c=4, ld=4 << 20), "positions")):
+                     (dict(o=1 << 20, i=1 << 12, c=4, ld=4 << 12), "positions"), (dict(t=1e-20), "temperature"),
+                     (dict(t=1e20), "temperature")):
         with pytest.raises(_lib.SegkError, match=text):
             top_call(**kw)
     base = dict(z=4096, dt=BF16, o=4, c=80, i=1, ld=80, v=4096, vdt=F32, x=4096, xb=4, lse=None, k=8, t=1.0, w=1.0, f=1, up=None, loss=4096, each=None, dz=4096,

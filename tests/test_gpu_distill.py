@@ -286,7 +286,7 @@ def test_top_rows_where_order_is_hard(V, dtype):
         host = top_logits(z, k)
         assert torch.equal(indices.cpu(), host.indices)
         assert torch.equal(values.cpu().view(torch.int16 if dtype == BF16 else torch.int32), host.values.view(torch.int16 if dtype == BF16 else torch.int32))
-        assert float(lse[1]) == -math.inf and math.isnan(float(lse[6])) and abs(float(lse[0]) - math.log(V)) < 2.0 ** -20 * 12
+        assert float(lse[1]) == -math.inf and math.isnan(float(lse[6])) and math.isnan(float(lse[7])) and abs(float(lse[0]) - math.log(V)) < 2.0 ** -20 * 12
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -340,6 +340,27 @@ def test_other_stream_and_captured_graph():
             g.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(want, out))
+
+
+@pytest.mark.parametrize("T", [2.0 ** -40, 1e-3, 2.0 ** 40])
+def test_extreme_temperatures(T):
+    """At the ends of the range the softmax is one class, or uniform."""
+    for V in (6, 300):
+        z = torch.arange(V, dtype=F32).repeat(4, 1)
+        x = z.cuda().requires_grad_()
+        t = top_logits(x, 3, temperature=T)
+        assert t.indices.cpu().tolist() == [[V - 1, V - 2, V - 3]] * 4
+        loss = distill_loss_topk(x, t, temperature=T)
+        loss.backward()
+        assert torch.isfinite(t.lse).all() and torch.isfinite(loss) and torch.isfinite(x.grad).all()
+        # The student is the teacher: both give every class the same, up to rounding of probabilities, 2^-18.  The kept lse and
+        # z / T are of the size V / T in fp32: rounded at 1 / T, at its product with log2(e), at those with z and with lse, at
+        # lse as kept and at their difference, log p is off by d <= 8 * 2^-24 V / T (nothing is off where T is a power of two
+        # and z / T exact).  d weighs in p log p, and as a rest of up to d that the teacher seems to have left:
+        # d (log d - log R), log R >= -(3 + log V) / T; 1e-3 and 300: e^d - 1 < 1.1 d.
+        d = 0.0 if math.log2(T).is_integer() else 8 * 2.0 ** -24 * V / T
+        off = 2.0 ** -18 + 1.1 * d * (2 + (0 if d == 0 else abs(math.log(d)) + (3 + math.log(V)) / T))
+        assert abs(float(loss.detach())) <= T * T * off and float(x.grad.abs().max()) <= T * (2.0 ** -18 + 4 * d)
 
 
 def test_far_rows_of_a_large_tensor():

@@ -127,6 +127,35 @@ def test_rows_behind_the_last_stay_as_they_were():
     assert bool((z[M:] == 7).all()) and bool((z[:, K:] == 7).all()) and torch.equal(z[:M, :K], mxfp4_dequantize(q))
 
 
+def test_many_rows_few_outputs():
+    """More rows than a grid dimension of 65535 workgroups of 16 covers: pixels through a 1x1 layer."""
+    M, K, N = 1_200_000, 32, 24
+    x, w = matrix(64, K, BF16), matrix(N, K)
+    y = mxfp4_linear(x.cuda().repeat(M // 64, 1), mxfp4_quantize(w.cuda()))
+    want = four_bit(x) @ four_bit(w).t()
+    assert y.shape == (M, N) and bool((y.view(-1, 64, N) == y[:64]).all())
+    size = four_bit(x).abs() @ four_bit(w).abs().t()
+    assert bool(((y[:64].cpu().double() - want).abs() <= (K + 8) * 2.0 ** -24 * size + 2.0 ** -8 * want.abs() * (1 + 2.0 ** -10)).all())
+
+
+@pytest.mark.parametrize("M,K,N", [(2, 700, 900), (40, 700, 900), (2050, 256, 2052), (4096, 384, 4100)])
+def test_every_kernel_in_a_captured_graph(M, K, N):
+    """The kernels for few rows and every tile size, captured without a call before and replayed on new inputs."""
+    qw = mxfp4_quantize(matrix(N, K).cuda())
+    x = matrix(M, K, BF16).cuda()
+    side = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(g, stream=side):
+        y = mxfp4_linear(x, qw)
+    for seed in (1, 2, 3):
+        new = matrix(M, K, BF16, seed=seed).cuda()
+        x.copy_(new)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, mxfp4_linear(new, qw))
+
+
 def test_chain_other_stream_and_captured_graph():
     """Teacher's last layer in 4 bits -> its top logits -> loss and gradient of a student's logits, eager, on another stream and as
     two captured graphs."""
