@@ -38,6 +38,8 @@ struct DistillArgs {
     int up_each, skip_if_one;
     int* counts;               // partial counts of the positions with a kept logit (mean), or none (sum)
     int count_here, log_kp;    // few rows: so many rows are counted by whoever needs the number (0: counts hold it)
+    int count_losses;          // no gradient waits for the number: the row losses that are not -0 are counted with their final sum
+                               // (1: by the finalize kernel, 2: by the collect kernel into counts)
     float* row_loss;           // loss of each position
     float* partial;            // sums that the finalize kernel adds (thread-per-position kernel)
     void* dz;
@@ -75,6 +77,12 @@ __device__ __forceinline__ int load_class(const DistillArgs& a, int64_t at) {
 template <typename I> __device__ __forceinline__ int load_class_as(const DistillArgs& a, int64_t at) {
     const I i = static_cast<const I*>(a.idx)[at];
     return i >= 0 && i < a.V ? (int)i : -1;
+}
+// loss of a row; -0 says that it has no entry, where the final sum counts them, and no other row has that value
+__device__ __forceinline__ float loss_of_empty(const DistillArgs& a) { return a.count_losses ? -0.f : 0.f; }
+__device__ __forceinline__ float loss_of_row(const DistillArgs& a, float l) {
+    l *= kLn2 * a.T * a.T * a.weight;
+    return l == 0.f ? 0.f : l;
 }
 __device__ __forceinline__ float load_kept(const DistillArgs& a, int64_t at) {
     return a.t_bf16 ? (float)static_cast<const bf16*>(a.t)[at] : static_cast<const float*>(a.t)[at];
@@ -373,7 +381,7 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(const DistillArgs a) {
 
     const int cls = lane < a.k ? load_class(a, row * a.k + lane) : -1;
     if (__ballot(cls >= 0) == 0) {                       // nothing was kept here: no loss, no gradient, the row is not read
-        if (threadIdx.x == 0) a.row_loss[row] = 0.f;
+        if (threadIdx.x == 0) a.row_loss[row] = loss_of_empty(a);
         if constexpr (GRAD) {
             const float zero[VEC] = {};
             for (int g = threadIdx.x; g < r.pieces; g += NT) store_piece<T>(dst, vec_ok, g * VEC - r.phase, a.V, zero);
@@ -461,7 +469,7 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(const DistillArgs a) {
     const Joined w = join(ko, so, sh_x[0], sh_x[1], c);
     if (wave == 0) {
         const float l = kept_loss(e, w, ko, so, c);
-        if (lane == 0) a.row_loss[row] = l * (kLn2 * a.T * a.T * a.weight);
+        if (lane == 0) a.row_loss[row] = loss_of_row(a, l);
     }
     if constexpr (GRAD) {
         const float gs = sh_x[4];
@@ -576,7 +584,7 @@ __global__ __launch_bounds__(64) void distill_join_kernel(const DistillArgs a, c
     const T* z = static_cast<const T*>(a.z) + row * a.ld;
     const int cls = lane < a.k ? load_class(a, row * a.k + lane) : -1;
     if (__ballot(cls >= 0) == 0) {
-        if (lane == 0) a.row_loss[row] = 0.f;
+        if (lane == 0) a.row_loss[row] = loss_of_empty(a);
         return;
     }
     const float* in = parts + (row * kShares + lane) * 2;
@@ -585,7 +593,7 @@ __global__ __launch_bounds__(64) void distill_join_kernel(const DistillArgs a, c
     const Kept e = kept_entries<T>(a, row, z, cls, lane, c);
     const Joined w = join(ko, so, e.top, e.sum, c);
     const float l = kept_loss(e, w, ko, so, c);
-    if (lane == 0) a.row_loss[row] = l * (kLn2 * a.T * a.T * a.weight);
+    if (lane == 0) a.row_loss[row] = loss_of_row(a, l);
     if (joined) {
         const float gs = grad_scale(a, row);
         float* out = joined + row * kRowFloats;
@@ -792,8 +800,51 @@ __global__ __launch_bounds__(256) void distill_count_rows_kernel(const DistillAr
     __syncthreads();
     if (threadIdx.x == 0) counts[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
 }
-// Planes: a thread takes 16 positions at a time and reads entry after entry until each has one (the first decides most of them); all
-// 16 loads of an entry are in flight together.
+// Planes: a thread takes 16 loads of positions at a time and reads entry after entry until each has one (the first decides most of
+// them); all loads of an entry are in flight together.  Four neighbouring positions for each load where the plane allows it.
+__global__ __launch_bounds__(1024) void distill_count_planes4_kernel(const DistillArgs a, int64_t positions, int* __restrict__ counts) {
+    __shared__ int red[16];
+    constexpr int U = 6, STEP = 1024 * 4;
+    int n = 0;
+    const int64_t per = (positions / 4 + kCountBlocks - 1) / kCountBlocks * 4, lo = per * blockIdx.x, hi = lo + per < positions ? lo + per : positions;
+    for (int64_t p = lo + threadIdx.x * 4; p < hi; p += STEP * U) {
+        int64_t at[U];
+        int c[U][4];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t q = (uint32_t)(p + u * STEP < hi ? p + u * STEP : p), o = q / (uint32_t)a.inner;       // positions < 2^31
+            at[u] = (int64_t)o * a.k * a.inner + (q - o * (uint32_t)a.inner);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) c[u][v] = -1;
+        }
+        for (int j = 0; j < a.k; ++j) {
+            int lowest = 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int4 i = *reinterpret_cast<const int4*>(static_cast<const int32_t*>(a.idx) + at[u] + j * a.inner);
+                const int d[4] = {i.x, i.y, i.z, i.w};
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    c[u][v] = d[v] >= 0 && d[v] < a.V ? d[v] : c[u][v];
+                    lowest = c[u][v] < lowest ? c[u][v] : lowest;
+                }
+            }
+            if (lowest >= 0) break;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) n += p + u * STEP < hi && c[u][v] >= 0;
+    }
+    n = wave_sum_i(n);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = n;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        int t = 0;
+        for (int i = 0; i < 16; ++i) t += red[i];
+        counts[blockIdx.x] = t;
+    }
+}
 template <typename I> __global__ __launch_bounds__(1024) void distill_count_planes_kernel(const DistillArgs a, int64_t positions, int* __restrict__ counts) {
     __shared__ int red[16];
     constexpr int U = 16;
@@ -846,21 +897,46 @@ __device__ __forceinline__ double block_sum_1024(double s, double* red) {
         for (int i = 0; i < 16; ++i) t += red[i];
     return t;
 }
+__device__ __forceinline__ int block_sum_i(int n, double* red) {
+    n = wave_sum_i(n);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = (double)n;
+    __syncthreads();
+    int t = 0;
+    for (int i = 0; i < 16; ++i) t += (int)red[i];
+    return t;
+}
 // level 1 of the final sum (many positions): workgroup b adds its own range in double
-__global__ __launch_bounds__(1024) void distill_collect_kernel(const float* __restrict__ v, int64_t n, float* __restrict__ out) {
+__global__ __launch_bounds__(1024) void distill_collect_kernel(const DistillArgs a, const float* __restrict__ v, int64_t n, float* __restrict__ out) {
     __shared__ double red[16];
     const int64_t per = (n + gridDim.x - 1) / gridDim.x, lo = per * blockIdx.x, hi = lo + per < n ? lo + per : n;
     double s = 0.0;
-    for (int64_t i = lo + threadIdx.x; i < hi; i += 1024) s += (double)v[i];
+    int m = 0;
+    for (int64_t i = lo + threadIdx.x; i < hi; i += 1024) {
+        s += (double)v[i];
+        m += __float_as_uint(v[i]) != 0x80000000u;
+    }
     s = block_sum_1024(s, red);
     if (threadIdx.x == 0) out[blockIdx.x] = (float)s;
+    if (a.count_losses) {
+        m = block_sum_i(m, red);
+        if (threadIdx.x == 0) a.counts[blockIdx.x] = m;
+    }
 }
 __global__ __launch_bounds__(1024) void distill_finalize_kernel(const DistillArgs a, const float* __restrict__ v, int n, float* __restrict__ loss) {
     __shared__ double red[16];
-    const int m = a.counts ? count_of(a) : 1;
+    int m = a.counts && a.count_losses != 1 ? count_of(a) : 1;
+    int own = 0;
     double s = 0.0;
-    for (int i = threadIdx.x; i < n; i += 1024) s += (double)v[i];
+    for (int i = threadIdx.x; i < n; i += 1024) {
+        s += (double)v[i];
+        own += __float_as_uint(v[i]) != 0x80000000u;
+    }
     s = block_sum_1024(s, red);
+    if (a.count_losses == 1) {
+        own = block_sum_i(own, red);
+        m = own > 0 ? own : 1;
+    }
     if (threadIdx.x == 0) loss[0] = (float)(s / (double)m);
 }
 
@@ -1257,7 +1333,8 @@ static int shares_of(int64_t rows, int64_t C, int dtype) {
     if (s > 1024 / rows) s = 1024 / rows;
     return (int)(s > kShares ? kShares : s < 1 ? 1 : s);
 }
-static constexpr int kCollect = 256;
+static constexpr int kCollect = 256, kFinal = 16384;      // from more than kFinal values on the final sum has two levels
+static_assert(kCollect == kCountBlocks);
 // floats of the workspace: partial counts, level-1 sums, then one sum per row or workgroup
 static size_t distill_partials(int64_t outer, int64_t C, int64_t inner) {
     if (!few(C, inner)) return (size_t)outer * (outer <= 128 ? 1 + 2 * kShares + kRowFloats : 1);
@@ -1311,11 +1388,14 @@ extern "C" int segk_distill(const void* logits, int dtype, int64_t outer, int64_
     while ((1 << a.log_kp) < k) ++a.log_kp;
     // up to 1024 entries (16 loads of a wave, all in flight) are counted where the number is needed instead of in a launch of their own
     if (mean && inner == 1 && outer << a.log_kp <= 1024) a.count_here = (int)outer;
-    if (mean && !skip && !a.count_here) {
+    if (mean && !dlogits && !pix) a.count_losses = outer > kFinal ? 2 : 1;
+    if (a.count_losses) a.count_here = 0;
+    if (mean && !skip && !a.count_here && !a.count_losses) {
         if (inner == 1) {
             hipLaunchKernelGGL(distill_count_rows_kernel, dim3(kCountBlocks), dim3(256), 0, st, a, outer, a.log_kp, counts);
         } else {
-            if (a.idx64) hipLaunchKernelGGL(distill_count_planes_kernel<int64_t>, dim3(kCountBlocks), dim3(1024), 0, st, a, outer * inner, counts);
+            if (!a.idx64 && inner % 4 == 0 && aligned16(indices)) hipLaunchKernelGGL(distill_count_planes4_kernel, dim3(kCountBlocks), dim3(1024), 0, st, a, outer * inner, counts);
+            else if (a.idx64) hipLaunchKernelGGL(distill_count_planes_kernel<int64_t>, dim3(kCountBlocks), dim3(1024), 0, st, a, outer * inner, counts);
             else hipLaunchKernelGGL(distill_count_planes_kernel<int32_t>, dim3(kCountBlocks), dim3(1024), 0, st, a, outer * inner, counts);
         }
         SEGK_LAUNCH_CHECK();
@@ -1342,8 +1422,8 @@ extern "C" int segk_distill(const void* logits, int dtype, int64_t outer, int64_
     SEGK_LAUNCH_CHECK();
     if (loss) {
         const float* v = pix ? partial : a.row_loss;
-        if (n > 16384) {
-            hipLaunchKernelGGL(distill_collect_kernel, dim3(kCollect), dim3(1024), 0, st, v, n, collected);
+        if (n > kFinal) {
+            hipLaunchKernelGGL(distill_collect_kernel, dim3(kCollect), dim3(1024), 0, st, a, v, n, collected);
             SEGK_LAUNCH_CHECK();
             v = collected;
             n = kCollect;

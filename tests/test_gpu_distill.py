@@ -363,6 +363,59 @@ def test_extreme_temperatures(T):
         assert abs(float(loss.detach())) <= T * T * off and float(x.grad.abs().max()) <= T * (2.0 ** -18 + 4 * d)
 
 
+@pytest.mark.parametrize("weight", [1.0, -2.0])
+@pytest.mark.parametrize("P,V", [(1, 40), (70, 40), (1100, 40), (16384, 12), (16385, 12), (40000, 12), (20, 140000), (3, 300000)])
+def test_positions_counted_for_a_mean(P, V, weight):
+    """The mean with a gradient (counted before) and without (counted with the sum), over rows of loss 0 and rows without entries."""
+    z, values, indices, lse = problem(min(P, 100), V, 3, seed=P, ignored=0.2)
+    indices[0::3] = -1                                           # whole rows, and single entries of others
+    values[1::3], indices[1::3], lse[1::3] = 0.0, -1, 0.0
+    indices[1::3, 0] = 5                                         # p = 1 at class 5 ...
+    z[1::3] = -200.0
+    z[1::3, 5] = 200.0                                           # ... and the student agrees: loss 0
+    agreed = torch.arange(P) % len(z) % 3 == 1                    # where these rows are repeated to
+    n = -(-P // len(z))
+    z, values, indices, lse = (torch.cat([t] * n)[:P].cuda() for t in (z, values, indices, lse))
+    loss = distill_loss_topk(z, TopLogits(values, indices, lse), weight=weight, reduction="none")
+    zero, has = loss[agreed.cuda()], (indices >= 0).any(1)
+    assert not zero.any() and not loss[~has].any()
+    want = loss.double().sum() / max(1, int(has.sum()))
+    for idx in (indices, indices.long()):
+        x = z.clone().requires_grad_()
+        counted = distill_loss_topk(x, TopLogits(values, idx, lse), weight=weight)
+        with torch.no_grad():
+            plain = distill_loss_topk(z, TopLogits(values, idx, lse), weight=weight)
+        # both sum in double, over at most 256 parts that are rounded to fp32, and round the quotient
+        tol = 2.0 ** -23 * float(loss.abs().double().sum()) / max(1, int(has.sum()))
+        assert abs(float(counted) - float(want)) <= tol and float(plain) == float(counted)
+
+
+@pytest.mark.parametrize("N,side", [(3, 8), (2, 66), (1, 21), (5, 130), (1, 1700)])
+def test_positions_counted_in_planes(N, side):
+    """A constant loss per counted position: the mean gives the number away.  Entries behind the first decide some positions."""
+    g = torch.Generator().manual_seed(side)
+    indices = torch.randint(-1, 3, (N, 3, side, side), generator=g, dtype=torch.int32)
+    indices[:, :, : side // 2] = torch.where(torch.rand(N, 3, side // 2, side, generator=g) < 0.7, -1, 2).int()
+    z = torch.zeros(N, 3, side, side)
+    z[:, 1] = 1.0
+    values = torch.zeros(N, 3, side, side)
+    has = (indices >= 0).any(1)
+    flat = torch.empty(indices.numel() + 1, dtype=torch.int32, device="cuda")
+    odd = flat[1:].view(indices.shape).copy_(indices)             # not aligned to 16 bytes
+    x = z.cuda().requires_grad_()
+    for idx in (indices.cuda(), indices.long().cuda(), odd):
+        target = TopLogits(values.cuda(), idx, None)
+        total = distill_loss_topk(x, target, reduction="sum")
+        mean = distill_loss_topk(x, target)
+        n = float(total.detach().double() / mean.detach().double())
+        assert abs(n / int(has.sum()) - 1) <= 2.0 ** -22          # two roundings to fp32; the number has to be exact
+        ga, = torch.autograd.grad(total, x)
+        gb, = torch.autograd.grad(mean, x)
+        # the scale is rounded once and the product once, on both sides
+        assert bool(((gb.double() * int(has.sum()) - ga.double()).abs() <= 2.0 ** -21 * ga.double().abs()).all())
+        assert not gb.permute(0, 2, 3, 1)[~has.cuda()].any()
+
+
 def test_far_rows_of_a_large_tensor():
     """Element offsets beyond 2^31."""
     V, P = 131072, 16400
