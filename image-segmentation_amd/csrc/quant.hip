@@ -213,7 +213,7 @@ __device__ __forceinline__ void store_rows(const LinearArgs& a, int64_t m, int64
     for (int i = 0; i < TN; ++i) store_outputs<TO>(a, m, n + i * 16 + 4 * q, acc[i][j]);
 }
 
-// Few rows: a workgroup computes 16 outputs of 16 rows, its waves share the slices.  Weights go straight from memory to the matrix
+// Few outputs in all: a workgroup computes 16 outputs of 16 rows, its waves share the slices.  Weights go straight from memory to the matrix
 // instruction, AHEAD slices of a wave at a time: lane l holds the 32 values (16 bytes) of row l % 16 in the block l / 16 of the slice.
 // FUSED: up to kFusedRows rows of x are packed by every workgroup for itself while its first weights are on their way, which
 // saves a launch; the packed rows stay in LDS.  Both in the same call, 8192 x 8192: one row 9.2 against 11.1 us with a launch of its
@@ -281,7 +281,7 @@ __global__ __launch_bounds__(WAVES * 64) void mxfp4_rows_kernel(const LinearArgs
     }
 }
 
-// Many rows: a workgroup of WM x WN waves computes BM rows x BN outputs.  Two stages of LDS hold two slices (256 values, 128 bytes a
+// Many outputs: a workgroup of WM x WN waves computes BM rows x BN outputs.  Two stages of LDS hold two slices (256 values, 128 bytes a
 // row) of both operands and are filled by LDS DMA.  The eight 16-byte blocks of a row lie at block ^ (row % 8), which spreads the 16
 // rows of a fragment over all banks; the DMA writes LDS in lane order, so the permutation is applied to its source addresses.
 // Scales: LDS [slice of the stage][row] dwords, of which a lane reads the byte of its block.
@@ -443,7 +443,24 @@ __global__ __launch_bounds__(WM * WN * 64, (WM * WN * 64 >= 512 ? 2 : 0)) void m
 
 // ------------------------------------------------------------------------------------------------ host
 static int64_t slices_of(int64_t cols) { return (cols + kSlice - 1) / kSlice; }
-static bool fused(int64_t M, int64_t K) { return M <= kFusedRows && M * slices_of(K) * 68 <= kFusedBytes; }
+
+// The kernel for M rows and N outputs: 16 = the rows kernel, else the side of the square tile.
+// Rows kernel: while its workgroups of 16 x 16 outputs are few (two per CU), splitting the slices over 8 or 16 waves beats a tile that
+// walks them alone; beyond, the weights are read again for every 16 rows, or too many short-lived workgroups fetch them.  Rows kernel /
+// 64-tile, us, packed x: 8192 -> 512: 64 rows 6.3/13.5, 256 rows (512 workgroups) 10.5/13.7; 8192 -> 1000: 128 rows (504) 11.8/13.6;
+// 8192 -> 2048: 64 (512) 10.4/13.6, 100 (896) 17.5/13.8; 8192 -> 8192: 16 (512) 10.8/18.0, 33 (1536) 24.5/18.4; 2048 -> 131072, one
+// row (8192): 39/23; 1664 -> 1000: 33 rows 3.6/5.1, 128 rows 5.0/5.1; 512 -> 2048: 64 rows (512) 4.0/3.8.
+// Tiles: a larger one moves fewer bytes per product, if it does not leave CUs without work and its rows are not mostly empty.  64 /
+// 128 / 256, us: 2048 -> 131072: 64 rows 25.5/30.5/42, 65 rows 37.8/31.0/41, 129 rows 51.5/51.8/44.3; 8192 -> 32768 (256 tiles of 128
+// for 65 rows): 64 rows 23.5/30.8/44, 65 rows 38.4/30.5/44; 2048 -> 16384 (128 tiles of 128): 128 rows 7.5/10.1/15.3.
+static int kernel_of(int64_t M, int64_t N) {
+    if (((M + 15) / 16) * ((N + 15) / 16) <= 512) return 16;
+    for (int t : {256, 128}) {
+        if (M > t / 2 && ((M + t - 1) / t) * ((N + t - 1) / t) >= 256) return t;
+    }
+    return 64;
+}
+static bool packs_inside(int64_t M, int64_t K, int64_t N) { return M <= kFusedRows && M * slices_of(K) * 68 <= kFusedBytes && kernel_of(M, N) == 16; }
 
 static int check_matrix(const char* who, int dtype, const void* x, int64_t ld, int64_t rows, int64_t cols) {
     SEGK_REQUIRE(x, SEGK_EINVAL, "%s: null pointer", who);
@@ -499,13 +516,6 @@ template <typename TO, int BM, int BN, int WM, int WN, bool WIDE> static int lau
     return SEGK_OK;
 }
 
-static int pick_tile(int64_t M, int64_t N) {
-    if (M <= 32) return 16;
-    for (int t : {256, 128}) {
-        if (((M + t - 1) / t) * ((N + t - 1) / t) >= 256) return t;
-    }
-    return 64;
-}
 
 }  // namespace segk
 
@@ -538,8 +548,7 @@ extern "C" int segk_mxfp4_dequantize(int dtype, const void* codes, const void* s
 }
 
 extern "C" size_t segk_mxfp4_linear_workspace(int64_t M, int64_t K, int64_t N) {
-    (void)N;
-    if (fused(M, K)) return 0;
+    if (packs_inside(M, K, N)) return 0;
     return align_up(segk_mxfp4_codes_bytes(M, K), 16) + segk_mxfp4_scales_bytes((int64_t)align_up(M > 0 ? M : 0, 4), K);
 }
 
@@ -552,12 +561,12 @@ extern "C" int segk_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const 
     if (const int rc = check_packed("mxfp4_linear", w_codes, w_scales)) return rc;
     if (x) {
         if (const int rc = check_matrix("mxfp4_linear", x_dtype, x, ldx, M, K)) return rc;
-        SEGK_REQUIRE(fused(M, K) || (workspace && workspace_bytes >= segk_mxfp4_linear_workspace(M, K, N)), SEGK_EWORKSPACE, "mxfp4_linear: workspace too small");
+        SEGK_REQUIRE(packs_inside(M, K, N) || (workspace && workspace_bytes >= segk_mxfp4_linear_workspace(M, K, N)), SEGK_EWORKSPACE, "mxfp4_linear: workspace too small");
         SEGK_REQUIRE(aligned16(workspace), SEGK_EALIGN, "mxfp4_linear: workspace must be 16-byte aligned");
     } else if (const int rc = check_packed("mxfp4_linear", x_codes, x_scales)) return rc;
     SEGK_USE_DEVICE(dev);
     hipStream_t st = (hipStream_t)stream;
-    const bool pack_inside = x && fused(M, K);
+    const bool pack_inside = x && packs_inside(M, K, N);
     if (x && !pack_inside) {
         x_codes = workspace;
         x_scales = (const uint8_t*)workspace + align_up(segk_mxfp4_codes_bytes(M, K), 16);
@@ -568,7 +577,7 @@ extern "C" int segk_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const 
     a.bias = bias; a.y = y; a.M = M; a.N = N; a.xs_rows = x && !pack_inside ? (int64_t)align_up(M, 4) : M; a.ldc = slices_of(K) * 64; a.ldy = ldy; a.slices = (int)slices_of(K);
     for (int v : {4, 8})
         if (reinterpret_cast<uintptr_t>(y) % (v * esize(y_dtype)) == 0 && ldy % v == 0) a.vec = v;
-    const int choice = pack_inside ? 16 : pick_tile(M, N);
+    const int choice = kernel_of(M, N);
     const bool wide = N % 4 == 0 && a.xs_rows % 4 == 0 && aligned16(w_scales) && aligned16(x_scales);
     SEGK_DISPATCH_DTYPE(y_dtype, TO, {
         if (choice == 256 && wide) return launch_tile<TO, 256, 256, 2, 4, true>(a, st);

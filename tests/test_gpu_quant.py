@@ -66,7 +66,10 @@ def test_non_finite_values_and_zeros():
 SHAPES = [(1, 1, 1), (1, 128, 16), (1, 1664, 1000), (1, 8192, 512), (2, 100, 33), (4, 513, 80), (5, 640, 1030), (8, 4096, 250), (15, 129, 17), (16, 256, 64),
           (17, 300, 65), (33, 1000, 127), (37, 1664, 1000), (64, 384, 128), (65, 2000, 129), (100, 77, 300), (128, 512, 128), (129, 1280, 255), (200, 3000, 100),
           (255, 640, 257), (256, 896, 256), (257, 1152, 513), (300, 64, 2000), (1000, 32, 90), (513, 2048, 512), (2049, 130, 130), (1, 20000, 40), (520, 8192, 300), (4, 20000, 50),
-          (2, 300, 5000), (20, 1100, 4500), (3, 2500, 4097)]
+          (2, 300, 5000), (20, 1100, 4500), (3, 2500, 4097),
+          # the kernels' borders: more than 512 workgroups of 16 x 16, a side of 64, 128 or 256 with 256 tiles
+          (1, 260, 9000), (2, 129, 8200), (33, 300, 4100), (64, 513, 8197), (100, 1000, 1500), (150, 128, 1111), (300, 1100, 777), (512, 100, 256),
+          (513, 300, 256), (65, 400, 32773), (129, 200, 33000), (200, 384, 65540), (130, 100, 65283)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -138,7 +141,7 @@ def test_many_rows_few_outputs():
     assert bool(((y[:64].cpu().double() - want).abs() <= (K + 8) * 2.0 ** -24 * size + 2.0 ** -8 * want.abs() * (1 + 2.0 ** -10)).all())
 
 
-@pytest.mark.parametrize("M,K,N", [(2, 700, 900), (40, 700, 900), (2050, 256, 2052), (4096, 384, 4100)])
+@pytest.mark.parametrize("M,K,N", [(2, 700, 900), (40, 700, 900), (40, 700, 9000), (1, 300, 9000), (2050, 256, 2052), (4096, 384, 4100)])
 def test_every_kernel_in_a_captured_graph(M, K, N):
     """The kernels for few rows and every tile size, captured without a call before and replayed on new inputs."""
     qw = mxfp4_quantize(matrix(N, K).cuda())
