@@ -281,15 +281,15 @@ __global__ __launch_bounds__(WAVES * 64) void mxfp4_rows_kernel(const LinearArgs
     }
 }
 
-// Many outputs: a workgroup of WM x WN waves computes BM rows x BN outputs.  Two stages of LDS hold two slices (256 values, 128 bytes a
-// row) of both operands and are filled by LDS DMA.  The eight 16-byte blocks of a row lie at block ^ (row % 8), which spreads the 16
+// Many outputs: a workgroup of WM x WN waves computes BM rows x BN outputs.  Each stage of LDS holds two slices (256 values, 128 bytes
+// a row) of both operands and is filled by LDS DMA.  The eight 16-byte blocks of a row lie at block ^ (row % 8), which spreads the 16
 // rows of a fragment over all banks; the DMA writes LDS in lane order, so the permutation is applied to its source addresses.
 // Scales: LDS [slice of the stage][row] dwords, of which a lane reads the byte of its block.
 //
 // The loop is skewed: while the products of one slice run, every fragment register is refilled for the next slice as soon as its
 // last product has been issued, so the matrix pipe does not wait for LDS.  The one barrier of a stage stands between its two
 // slices: the second slice's fragments are in registers by then, so the stage may be overwritten behind it, and the next stage,
-// requested one stage earlier, has landed.  The transfers are spread over the products of the second slice.
+// requested STAGES - 1 stages earlier, has landed.  The transfers are spread over the products of the second slice.
 template <int BM, int BN> struct TileLds {
     static constexpr int kData = (BM + BN) * 128, kScale = (BM + BN) * 8, kStage = kData + kScale;
 };
@@ -304,8 +304,10 @@ __device__ __forceinline__ void dma4(const void* base, uint32_t off, uint32_t ld
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(lds_addr));
 }
 
-template <typename TO, int BM, int BN, int WM, int WN, bool WIDE>
-__global__ __launch_bounds__(WM * WN * 64, (WM * WN * 64 >= 512 ? 2 : 0)) void mxfp4_tile_kernel(const LinearArgs a, int tiles_m, int tiles_n) {
+// Two waves per SIMD in the launch bounds: with more registers to give away the accumulators went to the other half of the register
+// file and were moved about in the loop (128 tile, 8192 -> 8192, 256 rows: 29 -> 26 us).
+template <typename TO, int BM, int BN, int WM, int WN, bool WIDE, int STAGES>
+__global__ __launch_bounds__(WM * WN * 64, 2) void mxfp4_tile_kernel(const LinearArgs a, int tiles_m, int tiles_n) {
     constexpr int W = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16, kRows = BM + BN;
     constexpr int kStage = TileLds<BM, BN>::kStage, kData = TileLds<BM, BN>::kData;
     // WIDE: the scales of 256 rows of a slice in one transfer (their rows come in fours), else of 64 rows.  With fewer transfers than
@@ -351,7 +353,7 @@ __global__ __launch_bounds__(WM * WN * 64, (WM * WN * 64 >= 512 ? 2 : 0)) void m
     // piece i of this wave for the stage of slices 2 step and 2 step + 1
     auto fill = [&](int step, int i) {
         const int slice = 2 * step < last_slice ? 2 * step : last_slice;
-        const uint32_t at = lds0 + (step & 1) * kStage;
+        const uint32_t at = lds0 + step % STAGES * kStage;
         if (i < kLoads) {
             dma16((i * W * 8 < BN ? wp : xp) + slice * 64, off[i < kLoads ? i : 0], at + (i * W + wave) * 1024);
         } else {
@@ -367,8 +369,9 @@ __global__ __launch_bounds__(WM * WN * 64, (WM * WN * 64 >= 512 ? 2 : 0)) void m
     const int steps = (a.slices + 1) / 2;
     u32x4 fw[2][TN], fx[TM];
     uint32_t sw[2][TN], sx[TM];
-    auto publish = [&]() {       // this wave's transfers have landed and its reads are done; behind the barrier this holds for all waves
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    // All but the youngest `pending` stages of this wave have landed and its reads are done; behind the barrier this holds for all waves
+    auto publish = [&](auto pending) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(pending() * kPieces) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
@@ -376,8 +379,8 @@ __global__ __launch_bounds__(WM * WN * 64, (WM * WN * 64 >= 512 ? 2 : 0)) void m
     // `ahead` is requested.
     auto multiply = [&](auto h, int next, int half, auto request, int ahead) {
         // fragment rows are r modulo 16, so r modulo 8 decides the slot
-        const char* d = lds + (next & 1) * kStage + r * 128 + ((half * 4 + q) ^ (r & 7)) * 16;
-        const char* c = lds + (next & 1) * kStage + kData + half * kRows * 4 + r * 4 + q;
+        const char* d = lds + next % STAGES * kStage + r * 128 + ((half * 4 + q) ^ (r & 7)) * 16;
+        const char* c = lds + next % STAGES * kStage + kData + half * kRows * 4 + r * 4 + q;
 #pragma unroll
         for (int j = 0; j < TM; ++j) {
 #pragma unroll
@@ -399,17 +402,17 @@ __global__ __launch_bounds__(WM * WN * 64, (WM * WN * 64 >= 512 ? 2 : 0)) void m
     constexpr std::integral_constant<int, 0> first{};
     constexpr std::integral_constant<int, 1> second{};
     const bool odd = a.slices & 1;
+    constexpr std::integral_constant<int, 0> none{};
+    for (int s = 0; s < STAGES && s < steps; ++s) {
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) fill(0, i);
-    if (steps > 1) {
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i) fill(1, i);
+        for (int i = 0; i < kPieces; ++i) fill(s, i);
     }
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
         for (int j = 0; j < TM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    publish();
+    if (steps >= STAGES) publish(std::integral_constant<int, STAGES - 1>{});
+    else publish(none);
     {
         const char* d = lds + r * 128 + (q ^ (r & 7)) * 16;
         const char* c = lds + kData + r * 4 + q;
@@ -425,15 +428,15 @@ __global__ __launch_bounds__(WM * WN * 64, (WM * WN * 64 >= 512 ? 2 : 0)) void m
         }
     }
     int step = 0;
-    for (; step + 2 < steps; ++step) {
+    for (; step + STAGES < steps; ++step) {
         multiply(first, step, 1, std::false_type{}, 0);
-        publish();
-        multiply(second, step + 1, step + 2 == steps && odd ? 1 : 0, std::true_type{}, step + 2);
+        publish(std::integral_constant<int, STAGES - 2>{});
+        multiply(second, step + 1, step + 2 == steps && odd ? 1 : 0, std::true_type{}, step + STAGES);
     }
-    for (; step < steps; ++step) {       // the last two stages; what is read ahead of the end is not used
+    for (; step < steps; ++step) {       // the last stages; what is read ahead of the end is not used
         multiply(first, step, 1, std::false_type{}, 0);
         if (step + 1 == steps && odd) break;
-        publish();
+        publish(none);
         multiply(second, step + 1, step + 2 == steps && odd ? 1 : 0, std::false_type{}, 0);
     }
     const int64_t m = m0 + (wave / WN) * TM * 16 + r, n = n0 + (wave % WN) * TN * 16;
@@ -447,12 +450,12 @@ static int64_t slices_of(int64_t cols) { return (cols + kSlice - 1) / kSlice; }
 // The kernel for M rows and N outputs: 16 = the rows kernel, else the side of the square tile.
 // Rows kernel: while its workgroups of 16 x 16 outputs are few (two per CU), splitting the slices over 8 or 16 waves beats a tile that
 // walks them alone; beyond, the weights are read again for every 16 rows, or too many short-lived workgroups fetch them.  Rows kernel /
-// 64-tile, us, packed x: 8192 -> 512: 64 rows 6.3/13.5, 256 rows (512 workgroups) 10.5/13.7; 8192 -> 1000: 128 rows (504) 11.8/13.6;
-// 8192 -> 2048: 64 (512) 10.4/13.6, 100 (896) 17.5/13.8; 8192 -> 8192: 16 (512) 10.8/18.0, 33 (1536) 24.5/18.4; 2048 -> 131072, one
-// row (8192): 39/23; 1664 -> 1000: 33 rows 3.6/5.1, 128 rows 5.0/5.1; 512 -> 2048: 64 rows (512) 4.0/3.8.
+// 64-tile, us, packed x: 8192 -> 512: 64 rows 6.3/11.5, 256 rows (512 workgroups) 10.5/11.7; 8192 -> 2048: 64 (512) 10.4/11.7, 100
+// (896) 17.5/11.9; 8192 -> 8192: 16 (512) 10.8/12.0, 33 (1536) 24.5/12.1; 2048 -> 131072, one row (8192): 39/23; 1664 -> 1000: 33 rows
+// 3.6/4.8, 128 rows (504) 5.0/4.9; 512 -> 2048: 64 rows (512) 4.0/3.8.
 // Tiles: a larger one moves fewer bytes per product, if it does not leave CUs without work and its rows are not mostly empty.  64 /
-// 128 / 256, us: 2048 -> 131072: 64 rows 25.5/30.5/42, 65 rows 37.8/31.0/41, 129 rows 51.5/51.8/44.3; 8192 -> 32768 (256 tiles of 128
-// for 65 rows): 64 rows 23.5/30.8/44, 65 rows 38.4/30.5/44; 2048 -> 16384 (128 tiles of 128): 128 rows 7.5/10.1/15.3.
+// 128 / 256, us: 8192 -> 32768: 64 rows 24/29/46, 128 rows (256 tiles of 128) 32/31/46, 1000 rows (512 tiles of 256) 224/155/121;
+// 8192 -> 8192: 256 rows (128 tiles of 128) 19/26/44, 1000 rows (512 of 128, 128 of 256) 61/41/50.
 static int kernel_of(int64_t M, int64_t N) {
     if (((M + 15) / 16) * ((N + 15) / 16) <= 512) return 16;
     for (int t : {256, 128}) {
@@ -497,11 +500,11 @@ static int quantize(int dtype, const void* x, int64_t ld, int64_t rows, int64_t 
     });
 }
 
-template <typename TO, int BM, int BN, int WM, int WN, bool WIDE> static int launch_tile(const LinearArgs& a, hipStream_t st) {
-    constexpr int bytes = 2 * TileLds<BM, BN>::kStage;
+template <typename TO, int BM, int BN, int WM, int WN, bool WIDE, int STAGES> static int launch_tile(const LinearArgs& a, hipStream_t st) {
+    constexpr int bytes = STAGES * TileLds<BM, BN>::kStage;
     const int64_t tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN;
     SEGK_REQUIRE(tm * tn < (1ll << 31), SEGK_ESHAPE, "mxfp4_linear: too many tiles");
-    auto kernel = mxfp4_tile_kernel<TO, BM, BN, WM, WN, WIDE>;
+    auto kernel = mxfp4_tile_kernel<TO, BM, BN, WM, WN, WIDE, STAGES>;
     if constexpr (bytes > 65536) {
         static std::atomic<bool> allowed[64] = {};               // once per device
         int dev = 0;
@@ -580,10 +583,13 @@ extern "C" int segk_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const 
     const int choice = kernel_of(M, N);
     const bool wide = N % 4 == 0 && a.xs_rows % 4 == 0 && aligned16(w_scales) && aligned16(x_scales);
     SEGK_DISPATCH_DTYPE(y_dtype, TO, {
-        if (choice == 256 && wide) return launch_tile<TO, 256, 256, 2, 4, true>(a, st);
-        if (choice == 256) return launch_tile<TO, 256, 256, 2, 4, false>(a, st);
-        if (choice == 128) return launch_tile<TO, 128, 128, 2, 2, false>(a, st);
-        if (choice == 64) return launch_tile<TO, 64, 64, 2, 2, false>(a, st);
+        if (choice == 256 && wide) return launch_tile<TO, 256, 256, 2, 4, true, 2>(a, st);
+        if (choice == 256) return launch_tile<TO, 256, 256, 2, 4, false, 2>(a, st);
+        if (choice == 128) return launch_tile<TO, 128, 128, 2, 2, false, 2>(a, st);
+        // Up to two tiles per CU wait for memory rather than for each other: four stages instead of the room for four workgroups per
+        // CU.  2 / 4 stages, us: 8192 -> 8192, 64 rows (128 tiles) 18.9/12.2, 256 rows (512) 21.0/18.8, 1000 rows (2048) 61/67.
+        if (choice == 64 && ((M + 63) / 64) * ((N + 63) / 64) <= 512) return launch_tile<TO, 64, 64, 2, 2, false, 4>(a, st);
+        if (choice == 64) return launch_tile<TO, 64, 64, 2, 2, false, 2>(a, st);
         const dim3 grid((unsigned)((N + 15) / 16), (unsigned)((M + 15) / 16));
         // Up to 4096 outputs there are few workgroups, and 16 waves share the slices of each; beyond, 8 waves, with 8 slices in flight
         // if they are many.  One row of packed x, 8192 outputs from 8192 values: (8 waves, 8 ahead) 8.8, (8, 4) 9.6, (4, 8) 12.2,
