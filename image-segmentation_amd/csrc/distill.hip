@@ -367,6 +367,10 @@ __device__ __forceinline__ float outside_factor(const Joined& w, float so, float
 }
 
 // One workgroup per row; with NCH > 0 the row stays in registers (NCH pieces per thread), with NCH == 0 it is read twice.
+// In registers the forward pass and the gradient cost one read and one write of the logits, and memory bounds it: 4096 rows of 32000
+// bf16 logits, 32 kept: 524 MB in 101 us, 5.2 TB/s (a copy of that size: 5.4).  The first wave handles the kept entries, one for
+// each lane, while the others wait for their pieces; their classes are taken out of the registers, so the two groups of classes have
+// separate maxima without a second pass.
 template <typename T, int NT, int NCH, bool GRAD>
 __global__ __launch_bounds__(NT) void distill_rows_kernel(const DistillArgs a) {
     constexpr int VEC = Piece<T>::VEC, NW = NT / 64;
@@ -655,6 +659,8 @@ __global__ __launch_bounds__(256) void distill_share_grad_kernel(const DistillAr
 // ------------------------------------------------------------------------------------------------ one thread per position
 // Few classes (up to 32), all of them in the registers of one thread, VP neighbouring positions per thread: the class planes of
 // [N, C, ...] logits are read with coalesced 16-byte loads (VP = 4), class-last rows with strided ones (VP = 1).
+// Memory bounds it: 32 x 4 x 384 x 384 fp32 logits with 2 kept entries, loss and gradient: 245 MB in 52 us, 4.7 TB/s (a copy: 5.4).
+// With scalar loads of the kept entries all kernels of that call took 168 us instead of 97.
 template <typename T, int CM, int VP, bool GRAD>
 __global__ __launch_bounds__(256) void distill_pixels_kernel(const DistillArgs a, int blocks_each) {
     if (a.skip_if_one && a.upstream[0] == 1.f) return;
@@ -801,7 +807,8 @@ __global__ __launch_bounds__(256) void distill_count_rows_kernel(const DistillAr
     if (threadIdx.x == 0) counts[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
 }
 // Planes: a thread takes 16 loads of positions at a time and reads entry after entry until each has one (the first decides most of
-// them); all loads of an entry are in flight together.  Four neighbouring positions for each load where the plane allows it.
+// them); all loads of an entry are in flight together.  Four neighbouring positions for each load where the plane allows it (4.7
+// million positions, 2 entries, a tenth without: 12 us; one position for each load 16 us).
 __global__ __launch_bounds__(1024) void distill_count_planes4_kernel(const DistillArgs a, int64_t positions, int* __restrict__ counts) {
     __shared__ int red[16];
     constexpr int U = 6, STEP = 1024 * 4;
@@ -948,23 +955,44 @@ __device__ __forceinline__ uint32_t order_key(float f) {
     return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 
-constexpr int kCandidates = 1024;
+constexpr int kMostCandidates = 1024;
+
+// Rows of one wave: four of them share a workgroup while their lists are short, and do not wait for each other.  A million rows of 80
+// (300) fp32 logits: 645 -> 455 (761 -> 537) us, 8000 rows of 80: 7.9 -> 7.0.  With the lists of longer rows fewer waves fit a CU: 32000
+// rows of 1000 logits 34 -> 39.
+constexpr int rows_per_group(int nt, int nch) { return nt == 64 && nch <= 2 ? 4 : 1; }
+template <int R> __device__ __forceinline__ void sync_row() {
+    if constexpr (R > 1) {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");       // one wave: LDS serves it in order
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    } else {
+        __syncthreads();
+    }
+}
 
 // Selection in three steps.  (1) Every thread takes the maximum of its part of the row (and the row's logsumexp is formed).
 // (2) The first wave finds a value that at least k of these maxima reach, by a binary search over the bits with ballots: at least
 // k elements of the row reach it, and hardly more than k in unordered data.  (3) The elements that reach it are collected in LDS
-// and ranked by counting; ties go to the lower index.  Where more than kCandidates reach it (many ties) or a NaN is in the row,
+// and ranked by counting; ties go to the lower index.  Where more than the list holds reach it (many ties) or a NaN is in the row,
 // the exact k-th key and then the last index that still belongs are found by binary searches over the whole row.
+// The row is read once: 4096 rows of 32000 bf16 logits, 32 kept: 262 MB in 60 us, 4.4 TB/s (the read alone: 48).  What is left are
+// the search of (2), during which one wave works, and the exponentials; other rows on the CU cover most of both.
 template <typename T, int NT, int NCH>
-__global__ __launch_bounds__(NT) void top_rows_kernel(const T* __restrict__ z, int64_t ld, int V, int k, float invT, T* __restrict__ values,
+__global__ __launch_bounds__(NT * rows_per_group(NT, NCH)) void top_rows_kernel(const T* __restrict__ z, int64_t rows, int64_t ld, int V, int k, float invT, T* __restrict__ values,
                                                       int32_t* __restrict__ indices, float* __restrict__ lse) {
-    constexpr int VEC = Piece<T>::VEC, NW = NT / 64;
-    __shared__ float sh_m[NT], sh_k[NW], sh_s[NW];
-    __shared__ uint32_t ck[kCandidates];
-    __shared__ int ci[kCandidates], sh_n[NW], sh_count, sh_slow;
-    __shared__ uint32_t sh_bound;
+    constexpr int VEC = Piece<T>::VEC, NW = NT / 64, R = rows_per_group(NT, NCH);
+    constexpr int kCandidates = NCH > 0 && NT * NCH * VEC < kMostCandidates ? NT * NCH * VEC : kMostCandidates;
+    __shared__ struct {
+        float m[NT], k[NW], s[NW];
+        uint32_t ck[kCandidates], bound;
+        int ci[kCandidates], n[NW], count, slow;
+    } shared[R];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t row = blockIdx.x;
+    const int of = R == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.y);
+    const int64_t row = (int64_t)blockIdx.x * R + of;
+    if (R > 1 && row >= rows) return;
+    auto& sh = shared[of];
     const float c = invT * kLog2e;
     const Row<T> r(z + row * ld, V);
     Piece<T> x[NCH > 0 ? NCH : 1];
@@ -1005,20 +1033,20 @@ __global__ __launch_bounds__(NT) void top_rows_kernel(const T* __restrict__ z, i
         kw = wave_max(m);
         sw = sum_wave(m == -INFINITY ? sw : sw * exp_over(m, kw, c));
     }
-    sh_m[threadIdx.x] = m;
-    if (lane == 0) { sh_k[wave] = kw; sh_s[wave] = sw; }
-    if (threadIdx.x == 0) sh_count = 0;
-    __syncthreads();
+    sh.m[threadIdx.x] = m;
+    if (lane == 0) { sh.k[wave] = kw; sh.s[wave] = sw; }
+    if (threadIdx.x == 0) sh.count = 0;
+    sync_row<R>();
     if (wave == 0) {
-        float kk = sh_k[0], s = 0.f;
+        float kk = sh.k[0], s = 0.f;
 #pragma unroll
-        for (int w = 1; w < NW; ++w) kk = fmaxf(kk, sh_k[w]);
+        for (int w = 1; w < NW; ++w) kk = fmaxf(kk, sh.k[w]);
 #pragma unroll
-        for (int w = 0; w < NW; ++w) s += sh_k[w] == -INFINITY ? sh_s[w] : sh_s[w] * exp_over(sh_k[w], kk, c);
+        for (int w = 0; w < NW; ++w) s += sh.k[w] == -INFINITY ? sh.s[w] : sh.s[w] * exp_over(sh.k[w], kk, c);
         if (lane == 0 && lse) lse[row] = (kk == -INFINITY && s == 0.f) ? -INFINITY : kk * invT + log2f(s) * kLn2;
         uint32_t key[NW];
 #pragma unroll
-        for (int w = 0; w < NW; ++w) key[w] = order_key(sh_m[w * 64 + lane]);
+        for (int w = 0; w < NW; ++w) key[w] = order_key(sh.m[w * 64 + lane]);
         uint32_t bound = 0;
         for (int bit = 31; bit >= (sizeof(T) == 2 ? 16 : 0); --bit) {
             const uint32_t cand = bound | (1u << bit);
@@ -1031,15 +1059,15 @@ __global__ __launch_bounds__(NT) void top_rows_kernel(const T* __restrict__ z, i
             }
         }
         if (lane == 0) {
-            sh_bound = bound;
-            sh_slow = s != s;
+            sh.bound = bound;
+            sh.slow = s != s;
         }
     }
-    __syncthreads();
+    sync_row<R>();
 
     auto take = [&](uint32_t key, int e) {
-        const int at = atomicAdd(&sh_count, 1);
-        if (at < kCandidates) { ck[at] = key; ci[at] = e; }
+        const int at = atomicAdd(&sh.count, 1);
+        if (at < kCandidates) { sh.ck[at] = key; sh.ci[at] = e; }
     };
     auto each_in_memory = [&](auto&& f) {
         for (int g = threadIdx.x; g < r.pieces; g += NT) {
@@ -1051,8 +1079,8 @@ __global__ __launch_bounds__(NT) void top_rows_kernel(const T* __restrict__ z, i
             }
         }
     };
-    const uint32_t bound = sh_bound;
-    bool slow = sh_slow != 0;
+    const uint32_t bound = sh.bound;
+    bool slow = sh.slow != 0;
     if (!slow) {
         // the bound as a float: keys of floats order as the floats do, so the elements are compared unconverted
         const float fb = bound <= 0x007FFFFFu ? -INFINITY      // no key lies between 0 and that of -inf: everything belongs
@@ -1083,19 +1111,19 @@ __global__ __launch_bounds__(NT) void top_rows_kernel(const T* __restrict__ z, i
                     if (f >= fb) take(order_key(f), e);
                 });
         }
-        __syncthreads();
-        slow = sh_count > kCandidates;
+        sync_row<R>();
+        slow = sh.count > kCandidates;
     }
     if (slow) {
         auto count = [&](auto&& pred) {
             int n = 0;
             each_in_memory([&](float f, int e) { n += pred(order_key(f), e) ? 1 : 0; });
             n = wave_sum_i(n);
-            __syncthreads();
-            if (lane == 0) sh_n[wave] = n;
-            __syncthreads();
+            sync_row<R>();
+            if (lane == 0) sh.n[wave] = n;
+            sync_row<R>();
             int t = 0;
-            for (int w = 0; w < NW; ++w) t += sh_n[w];
+            for (int w = 0; w < NW; ++w) t += sh.n[w];
             return t;
         };
         uint32_t kth = 0;
@@ -1109,21 +1137,21 @@ __global__ __launch_bounds__(NT) void top_rows_kernel(const T* __restrict__ z, i
             const int cand = last | (1 << bit);
             if (cand < V && count([&](uint32_t q, int e) { return q == kth && e < cand; }) < need) last = cand;
         }
-        __syncthreads();
-        if (threadIdx.x == 0) sh_count = 0;
-        __syncthreads();
+        sync_row<R>();
+        if (threadIdx.x == 0) sh.count = 0;
+        sync_row<R>();
         each_in_memory([&](float f, int e) {
             const uint32_t q = order_key(f);
             if (q > kth || (q == kth && e <= last)) take(q, e);
         });
-        __syncthreads();
+        sync_row<R>();
     }
-    const int n = sh_count < kCandidates ? sh_count : kCandidates;
+    const int n = sh.count < kCandidates ? sh.count : kCandidates;
     for (int i = threadIdx.x; i < n; i += NT) {
-        const uint32_t q = ck[i];
-        const int e = ci[i];
+        const uint32_t q = sh.ck[i];
+        const int e = sh.ci[i];
         int rank = 0;
-        for (int j = 0; j < n; ++j) rank += (ck[j] > q || (ck[j] == q && ci[j] < e)) ? 1 : 0;
+        for (int j = 0; j < n; ++j) rank += (sh.ck[j] > q || (sh.ck[j] == q && sh.ci[j] < e)) ? 1 : 0;
         if (rank < k) {
             indices[row * k + rank] = e;
             values[row * k + rank] = r.p[e];
@@ -1150,7 +1178,8 @@ __device__ __forceinline__ void store_same4(bf16* p, const float (&v)[4]) {
                                               (__float_as_uint(v[2]) >> 16) | (__float_as_uint(v[3]) & 0xFFFF0000u));
 }
 
-// one thread per position, up to 32 classes in its registers: k rounds of "greatest that is left"
+// one thread per position, up to 32 classes in its registers: k rounds of "greatest that is left".  32 x 4 x 384 x 384 fp32 logits,
+// the best 2: 170 MB in 32 us, 5.3 TB/s, bound by memory.
 template <typename T, int CM, int VP>
 __global__ __launch_bounds__(256) void top_pixels_kernel(const T* __restrict__ z, int64_t ld, int64_t s_c, int64_t s_p, int64_t inner, int V,
                                                          int k, float invT, T* __restrict__ values, int32_t* __restrict__ indices,
@@ -1281,7 +1310,11 @@ static Pixels pixels(int64_t outer, int64_t C, int64_t inner, int64_t ld, int64_
     p.blocks = p.outer * p.blocks_each;
     return p;
 }
-static bool few(int64_t C, int64_t inner) { return C <= kPixelClasses && (inner > 1 || C <= 8); }
+// One thread per position: class planes of up to 32 classes, and rows of so few classes.  Rows of 9 to 32 classes go to a wave each
+// while they are too few to fill the chip with threads.  Thread / wave for each row, fp32, selection and loss with gradient, us: 8000
+// rows of 4 classes 3.2/11.4, 8.7/15.2, of 16 6.3/7.5, 12.7/15.1, of 32 9.4/7.5, 18.6/15.3; 32000 of 32 9.6/18.4, 20.7/30.4; 1000 of 9
+// 4.1/5.1, 9.9/9.5, of 32 9.3/5.1, 18.0/9.4.
+static bool few(int64_t outer, int64_t C, int64_t inner) { return C <= kPixelClasses && (inner > 1 || C <= 8 || outer >= 512 * C); }
 
 template <typename F> static void class_tier(int64_t C, int vp, F&& f) {
     if (C <= 4) return vp == 4 ? f(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{}) : f(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
@@ -1299,7 +1332,7 @@ extern "C" int segk_top_logits(const void* logits, int dtype, int64_t outer, int
     if (const int rc = check_logits("top_logits", logits, dtype, outer, C, inner, ld, k, temperature)) return rc;
     SEGK_REQUIRE(values && indices, SEGK_EINVAL, "top_logits: null output");
     SEGK_REQUIRE(aligned16(values) && aligned16(indices) && aligned16(lse), SEGK_EALIGN, "top_logits: outputs must be 16-byte aligned");
-    const bool pix = few(C, inner);
+    const bool pix = few(outer, C, inner);
     const Pixels px = pixels(outer, C, inner, ld, k, aligned16(logits));
     SEGK_REQUIRE(!pix || px.blocks < (1ll << 31), SEGK_ESHAPE, "top_logits: too many positions");
     SEGK_USE_DEVICE(dev);
@@ -1312,7 +1345,8 @@ extern "C" int segk_top_logits(const void* logits, int dtype, int64_t outer, int
             });
         } else {
             row_tier<T, true>(C, [&](auto nt, auto nch) {
-                hipLaunchKernelGGL((top_rows_kernel<T, nt(), nch()>), dim3((unsigned)outer), dim3(nt()), 0, st, (const T*)logits, ld, (int)C, (int)k,
+                constexpr int r = rows_per_group(nt(), nch());
+                hipLaunchKernelGGL((top_rows_kernel<T, nt(), nch()>), dim3((unsigned)((outer + r - 1) / r)), dim3(nt(), r), 0, st, (const T*)logits, outer, ld, (int)C, (int)k,
                                    1.f / temperature, (T*)values, indices, lse);
             });
         }
@@ -1337,7 +1371,7 @@ static constexpr int kCollect = 256, kFinal = 16384;      // from more than kFin
 static_assert(kCollect == kCountBlocks);
 // floats of the workspace: partial counts, level-1 sums, then one sum per row or workgroup
 static size_t distill_partials(int64_t outer, int64_t C, int64_t inner) {
-    if (!few(C, inner)) return (size_t)outer * (outer <= 128 ? 1 + 2 * kShares + kRowFloats : 1);
+    if (!few(outer, C, inner)) return (size_t)outer * (outer <= 128 ? 1 + 2 * kShares + kRowFloats : 1);
     return (size_t)(pixels(outer, C, inner, C * inner, 1, false).blocks);      // an upper bound for either vector width
 }
 extern "C" size_t segk_distill_workspace(int64_t outer, int64_t C, int64_t inner) {
@@ -1361,7 +1395,7 @@ extern "C" int segk_distill(const void* logits, int dtype, int64_t outer, int64_
     SEGK_REQUIRE(!dlogits || (ld_d >= C * inner && reinterpret_cast<uintptr_t>(dlogits) % esize(dtype) == 0), SEGK_ESHAPE, "distill: bad dlogits");
     SEGK_REQUIRE(workspace_bytes >= segk_distill_workspace(outer, C, inner), SEGK_EWORKSPACE, "distill: workspace too small");
     SEGK_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 4 == 0, SEGK_EALIGN, "distill: workspace must be 4-byte aligned");
-    const bool pix = few(C, inner);
+    const bool pix = few(outer, C, inner);
     const bool vec = aligned16(logits) && (!dlogits || (aligned16(dlogits) && ld_d % 4 == 0)) && aligned16(values) && aligned16(indices) && aligned16(teacher_lse);
     const Pixels px = pixels(outer, C, inner, ld, k, vec);
     SEGK_REQUIRE(!pix || px.blocks < (1ll << 31), SEGK_ESHAPE, "distill: too many positions");

@@ -363,6 +363,18 @@ def test_extreme_temperatures(T):
         assert abs(float(loss.detach())) <= T * T * off and float(x.grad.abs().max()) <= T * (2.0 ** -18 + 4 * d)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("P,V", [(4607, 9), (4608, 9), (8191, 16), (8192, 16), (16384, 32), (16383, 32), (5, 200), (1027, 80)])
+def test_many_short_rows(P, V, dtype):
+    """Both sides of the border between a thread and a wave for each row, and rows that do not fill the last workgroup."""
+    z, values, indices, lse = problem(P, V, 3, seed=V, dtype=dtype, ignored=0.1)
+    got = top_logits(z.cuda(), 3)
+    want = torch.topk(z.double(), 3, 1)
+    assert torch.equal(got.values.cpu().double(), want.values)
+    assert torch.equal(z.gather(1, got.indices.cpu().long()), got.values.cpu())
+    check(z, values, indices, lse, 1.0)
+
+
 @pytest.mark.parametrize("weight", [1.0, -2.0])
 @pytest.mark.parametrize("P,V", [(1, 40), (70, 40), (1100, 40), (16384, 12), (16385, 12), (40000, 12), (20, 140000), (3, 300000)])
 def test_positions_counted_for_a_mean(P, V, weight):
