@@ -308,7 +308,7 @@ __device__ __forceinline__ void dma4(const void* base, uint32_t off, uint32_t ld
 }
 
 // 256 x 256 tiles by eight waves (128 x 64 outputs each) reach 4.4 PFLOP/s at 8192^3 (250 us); a loop of these matrix instructions
-// alone runs at 7.2.  The matrix units are busy 58 % of the time.  Without the transfers the loop is 19 % faster, with half the
+// alone runs at 7.2.  The matrix units are busy 63 % of the time.  Without the transfers the loop is 19 % faster, with half the
 // fragment reads 9 %, without the scales 6 %; bank conflicts are 0; the width of the stripes, wave priorities and a 4 x 2 layout of
 // the waves change nothing.
 // Two waves per SIMD in the launch bounds: with more registers to give away the accumulators went to the other half of the register
