@@ -524,9 +524,10 @@ template <typename T> struct Share {         // the pieces [lo, hi) of a row, wh
 };
 
 template <typename T>
-__global__ __launch_bounds__(256) void distill_share_kernel(const DistillArgs a, float* __restrict__ parts) {
+__global__ __launch_bounds__(256) void distill_share_kernel(const DistillArgs a, float* __restrict__ parts, int* __restrict__ rows_done) {
     constexpr int VEC = Piece<T>::VEC, U = 4;
     if (a.skip_if_one && a.upstream[0] == 1.f) return;
+    if (rows_done && (blockIdx.x | blockIdx.y | threadIdx.x) == 0) *rows_done = 0;
     __shared__ float sh_k[4], sh_s[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t row = blockIdx.y;
@@ -579,8 +580,37 @@ __global__ __launch_bounds__(256) void distill_share_kernel(const DistillArgs a,
     }
 }
 
+// The loss of a joined row.  Whichever wave is the last of all adds the rows' losses, in their order (a launch less: 61 rows of 128011
+// fp32 classes 24 -> 21 us).  The counter only says who is last; the losses pass between the XCDs' caches as atomic accesses.
+__device__ __forceinline__ void deliver(const DistillArgs& a, int64_t row, float l, int* __restrict__ rows_done, float* __restrict__ loss, int lane) {
+    if (!rows_done) {
+        if (lane == 0) a.row_loss[row] = l;
+        return;
+    }
+    int before = 0;
+    if (lane == 0) {
+        __hip_atomic_store(a.row_loss + row, l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        before = __hip_atomic_fetch_add(rows_done, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    const int rows = (int)gridDim.x;
+    if (__builtin_amdgcn_readfirstlane(before) != rows - 1) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    int m = a.counts && !a.count_losses ? count_of(a) : 1, own = 0;
+    double s = 0.0;
+    for (int i = lane; i < rows; i += 64) {
+        const float v = __hip_atomic_load(a.row_loss + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        s += (double)v;
+        own += __float_as_uint(v) != 0x80000000u;
+    }
+    s = wave_sum_d(s);
+    own = wave_sum_i(own);
+    if (a.count_losses) m = own > 0 ? own : 1;
+    if (lane == 0) loss[0] = (float)(s / (double)m);
+}
+
 template <typename T>
-__global__ __launch_bounds__(64) void distill_join_kernel(const DistillArgs a, const float* __restrict__ parts, int shares, float* __restrict__ joined) {
+__global__ __launch_bounds__(64) void distill_join_kernel(const DistillArgs a, const float* __restrict__ parts, int shares, float* __restrict__ joined,
+                                                          int* __restrict__ rows_done, float* __restrict__ loss) {
     if (a.skip_if_one && a.upstream[0] == 1.f) return;
     const int lane = threadIdx.x;
     const int64_t row = blockIdx.x;
@@ -588,7 +618,7 @@ __global__ __launch_bounds__(64) void distill_join_kernel(const DistillArgs a, c
     const T* z = static_cast<const T*>(a.z) + row * a.ld;
     const int cls = lane < a.k ? load_class(a, row * a.k + lane) : -1;
     if (__ballot(cls >= 0) == 0) {
-        if (lane == 0) a.row_loss[row] = loss_of_empty(a);
+        deliver(a, row, loss_of_empty(a), rows_done, loss, lane);
         return;
     }
     const float* in = parts + (row * kShares + lane) * 2;
@@ -597,7 +627,6 @@ __global__ __launch_bounds__(64) void distill_join_kernel(const DistillArgs a, c
     const Kept e = kept_entries<T>(a, row, z, cls, lane, c);
     const Joined w = join(ko, so, e.top, e.sum, c);
     const float l = kept_loss(e, w, ko, so, c);
-    if (lane == 0) a.row_loss[row] = loss_of_row(a, l);
     if (joined) {
         const float gs = grad_scale(a, row);
         float* out = joined + row * kRowFloats;
@@ -607,6 +636,7 @@ __global__ __launch_bounds__(64) void distill_join_kernel(const DistillArgs a, c
         }
         out[2 + lane] = gs * (e.mass * exp_over(e.z, w.top, c) / w.sum - e.total);
     }
+    deliver(a, row, loss_of_row(a, l), rows_done, loss, lane);
 }
 
 template <typename T>
@@ -1371,7 +1401,7 @@ static constexpr int kCollect = 256, kFinal = 16384;      // from more than kFin
 static_assert(kCollect == kCountBlocks);
 // floats of the workspace: partial counts, level-1 sums, then one sum per row or workgroup
 static size_t distill_partials(int64_t outer, int64_t C, int64_t inner) {
-    if (!few(outer, C, inner)) return (size_t)outer * (outer <= 128 ? 1 + 2 * kShares + kRowFloats : 1);
+    if (!few(outer, C, inner)) return (size_t)outer * (outer <= 128 ? 1 + 2 * kShares + kRowFloats : 1) + 1;
     return (size_t)(pixels(outer, C, inner, C * inner, 1, false).blocks);      // an upper bound for either vector width
 }
 extern "C" size_t segk_distill_workspace(int64_t outer, int64_t C, int64_t inner) {
@@ -1435,6 +1465,7 @@ extern "C" int segk_distill(const void* logits, int dtype, int64_t outer, int64_
         SEGK_LAUNCH_CHECK();
     }
     int64_t n = pix ? px.blocks : outer;
+    bool summed = false;
     SEGK_DISPATCH_DTYPE(dtype, T, {
         if (pix) {
             class_tier(C, px.vp, [&](auto cm, auto vp) {
@@ -1443,8 +1474,10 @@ extern "C" int segk_distill(const void* logits, int dtype, int64_t outer, int64_
             });
         } else if (const int shares = shares_of(outer, C, dtype); shares > 1) {
             float *parts = partial + outer, *joined = parts + outer * 2 * kShares;
-            hipLaunchKernelGGL((distill_share_kernel<T>), dim3(shares, (unsigned)outer), dim3(256), 0, st, a, parts);
-            hipLaunchKernelGGL((distill_join_kernel<T>), dim3((unsigned)outer), dim3(64), 0, st, a, parts, shares, dlogits ? joined : nullptr);
+            int* rows_done = loss ? reinterpret_cast<int*>(joined + outer * kRowFloats) : nullptr;
+            summed = loss;
+            hipLaunchKernelGGL((distill_share_kernel<T>), dim3(shares, (unsigned)outer), dim3(256), 0, st, a, parts, rows_done);
+            hipLaunchKernelGGL((distill_join_kernel<T>), dim3((unsigned)outer), dim3(64), 0, st, a, parts, shares, dlogits ? joined : nullptr, rows_done, loss);
             if (dlogits) hipLaunchKernelGGL((distill_share_grad_kernel<T>), dim3(shares, (unsigned)outer), dim3(256), 0, st, a, joined);
         } else {
             row_tier<T, false>(C, [&](auto nt, auto nch) {
@@ -1454,7 +1487,7 @@ extern "C" int segk_distill(const void* logits, int dtype, int64_t outer, int64_
         }
     });
     SEGK_LAUNCH_CHECK();
-    if (loss) {
+    if (loss && !summed) {
         const float* v = pix ? partial : a.row_loss;
         if (n > kFinal) {
             hipLaunchKernelGGL(distill_collect_kernel, dim3(kCollect), dim3(1024), 0, st, a, v, n, collected);

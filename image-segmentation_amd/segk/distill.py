@@ -112,10 +112,10 @@ class _DistillFn(torch.autograd.Function):
         dz = _DistillFn._gradient(ctx.meta, z) if want_grad and not each else None
         # a workspace of its own for every call: launches on other streams and replays of captured graphs never share one
         ws = torch.empty(query("segk_distill_workspace", outer, C, inner), dtype=torch.uint8, device=z.device)
-        _DistillFn._launch(ctx.meta, z, values, indices, lse, None, MEAN if reduction == "mean" else 0, None if each else out, out if each else None, dz, ws)
+        args = _DistillFn._launch(ctx.meta, z, values, indices, lse, None, MEAN if reduction == "mean" else 0, None if each else out, out if each else None, dz, ws)
         if want_grad:
             ctx.save_for_backward(z, values, indices, lse)
-            ctx.dz, ctx.ws = dz, ws
+            ctx.dz, ctx.ws, ctx.args = dz, ws, args
         return out
 
     @staticmethod
@@ -129,10 +129,11 @@ class _DistillFn(torch.autograd.Function):
         outer, C, inner, ld, moved, k, dim, T, weight, reduction, shape, in_dtype = meta
         p = ops._p
         dev, st = _env(z)
+        args = [z.data_ptr(), dt(z.dtype), outer, C, inner, ld, values.data_ptr(), dt(values.dtype), indices.data_ptr(), indices.element_size(),
+                p(lse), k, T, weight, flags, p(upstream), p(loss), p(each), p(dz), C * inner, ws.data_ptr(), ws.numel(), dev, st]
         with ops._streamed("distillation loss", z.numel() * z.element_size() * (2 if dz is not None else 1)):
-            call("segk_distill", z.data_ptr(), dt(z.dtype), outer, C, inner, ld, values.data_ptr(), dt(values.dtype), indices.data_ptr(),
-                 indices.element_size(), p(lse), k, T, weight, flags, p(upstream), p(loss), p(each), p(dz), C * inner, ws.data_ptr(), ws.numel(),
-                 dev, st)
+            call("segk_distill", *args)
+        return args
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -140,13 +141,18 @@ class _DistillFn(torch.autograd.Function):
         z, values, indices, lse = ctx.saved_tensors
         outer, C, inner, ld, moved, k, dim, T, weight, reduction, shape, in_dtype = ctx.meta
         dz, ctx.dz, ws, ctx.ws = ctx.dz, None, ctx.ws, None      # handed over once; a second backward pass computes its own
-        flags = EACH if reduction == "none" else MEAN if reduction == "mean" else 0
+        if g.dtype != torch.float32 or not g.is_contiguous():
+            g = g.float().contiguous()
         if dz is None:
             dz = _DistillFn._gradient(ctx.meta, z)
             ws = torch.empty(query("segk_distill_workspace", outer, C, inner), dtype=torch.uint8, device=z.device)
+            _DistillFn._launch(ctx.meta, z, values, indices, lse, g, EACH if reduction == "none" else MEAN if reduction == "mean" else 0, None, None, dz, ws)
         else:
-            flags |= SKIP
-        _DistillFn._launch(ctx.meta, z, values, indices, lse, g if g.dtype == torch.float32 and g.is_contiguous() else g.float().contiguous(), flags, None, None, dz, ws)
+            # the forward pass's arguments once more: this runs in autograd's thread, where every line costs several times its usual time
+            args = ctx.args
+            args[14] |= SKIP
+            args[15], args[16], args[23] = g.data_ptr(), None, _env(z)[1]
+            call("segk_distill", *args)
         if moved:
             dz = dz.movedim(-1, dim)
         return (dz if dz.dtype == in_dtype else dz.to(in_dtype),) + (None,) * 8
