@@ -50,6 +50,8 @@ def _canonical(x, dim):
     """(tensor, outer, C, inner, ld, moved): x as `outer` images of C x `inner`, in place where its strides allow it.  More than
     PLANE_CLASSES classes in front of other dimensions are moved to the end (a copy)."""
     shape = x.shape
+    if dim == 1 and len(shape) == 2 and x.is_contiguous():            # the usual rows, for the sake of a short call
+        return x, shape[0], shape[1], 1, shape[1], False
     C, outer, inner = shape[dim], math.prod(shape[:dim]), math.prod(shape[dim + 1:])
     moved = inner > 1 and C > PLANE_CLASSES
     if moved:
@@ -74,15 +76,15 @@ def top_logits(logits, k, dim=1, temperature=1.0):
     if not 1 <= k <= min(MAX_K, C):
         raise ValueError(f"k has to be between 1 and min({MAX_K}, {C} classes), got {k}")
     z = logits.detach() if logits.requires_grad else logits
-    shape = z.shape
-    rest = shape[:dim] + shape[dim + 1:]
     if not z.is_cuda or z.numel() == 0:
         return _host_top(z, k, dim, temperature)
+    before, behind = z.shape[:dim], z.shape[dim + 1:]
     z, outer, C, inner, ld, moved = _canonical(z.float() if z.dtype == torch.float16 else z, dim)
-    kept = rest + (k,) if moved else shape[:dim] + (k,) + shape[dim + 1:]
-    values = torch.empty(kept, dtype=z.dtype, device=z.device)
-    indices = torch.empty(kept, dtype=torch.int32, device=z.device)
-    lse = torch.empty(rest, dtype=torch.float32, device=z.device)
+    device, rest = z.device, before + behind
+    kept = rest + (k,) if moved else before + (k,) + behind
+    values = torch.empty(kept, dtype=z.dtype, device=device)
+    indices = torch.empty(kept, dtype=torch.int32, device=device)
+    lse = torch.empty(rest, dtype=torch.float32, device=device)
     dev, st = _env(z)
     with ops._streamed("top logits", z.numel() * z.element_size()):
         call("segk_top_logits", z.data_ptr(), dt(z.dtype), outer, C, inner, ld, k, temperature, values.data_ptr(), indices.data_ptr(),
@@ -105,17 +107,17 @@ class _DistillFn(torch.autograd.Function):
         values = values if values.is_contiguous() else values.contiguous()
         indices = indices if indices.is_contiguous() else indices.contiguous()
         lse = lse if lse is None or lse.is_contiguous() else lse.contiguous()
-        ctx.meta = (outer, C, inner, ld, moved, k, dim, float(temperature), float(weight), reduction, logits.shape, logits.dtype)
-        rest = logits.shape[:dim] + logits.shape[dim + 1:]
+        shape = logits.shape
+        meta = (outer, C, inner, ld, moved, k, dim, float(temperature), float(weight), reduction, shape, logits.dtype)
         each = reduction == "none"
-        out = torch.empty(rest if each else (), dtype=torch.float32, device=z.device)
-        dz = _DistillFn._gradient(ctx.meta, z) if want_grad and not each else None
+        out = torch.empty(shape[:dim] + shape[dim + 1:] if each else (), dtype=torch.float32, device=z.device)
+        dz = _DistillFn._gradient(meta, z) if want_grad and not each else None
         # a workspace of its own for every call: launches on other streams and replays of captured graphs never share one
         ws = torch.empty(query("segk_distill_workspace", outer, C, inner), dtype=torch.uint8, device=z.device)
-        args = _DistillFn._launch(ctx.meta, z, values, indices, lse, None, MEAN if reduction == "mean" else 0, None if each else out, out if each else None, dz, ws)
+        args = _DistillFn._launch(meta, z, values, indices, lse, None, MEAN if reduction == "mean" else 0, None if each else out, out if each else None, dz, ws)
         if want_grad:
             ctx.save_for_backward(z, values, indices, lse)
-            ctx.dz, ctx.ws, ctx.args = dz, ws, args
+            ctx.meta, ctx.dz, ctx.ws, ctx.args = meta, dz, ws, args
         return out
 
     @staticmethod
@@ -136,8 +138,12 @@ class _DistillFn(torch.autograd.Function):
         return args
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        # the wrapper only matters where somebody may differentiate again
+        return _once(ctx, g) if torch.is_grad_enabled() else _DistillFn._gradients(ctx, g)
+
+    @staticmethod
+    def _gradients(ctx, g):
         z, values, indices, lse = ctx.saved_tensors
         outer, C, inner, ld, moved, k, dim, T, weight, reduction, shape, in_dtype = ctx.meta
         dz, ctx.dz, ws, ctx.ws = ctx.dz, None, ctx.ws, None      # handed over once; a second backward pass computes its own
@@ -158,6 +164,9 @@ class _DistillFn(torch.autograd.Function):
         return (dz if dz.dtype == in_dtype else dz.to(in_dtype),) + (None,) * 8
 
 
+_once = torch.autograd.function.once_differentiable(_DistillFn._gradients)
+
+
 def distill_loss_topk(pred, target, temperature=1.0, reduction="mean", dim=1, weight=1.0):
     """Distillation loss of the student's logits `pred` against a teacher's top logits.
 
@@ -175,8 +184,7 @@ def distill_loss_topk(pred, target, temperature=1.0, reduction="mean", dim=1, we
     dim = _check(pred, dim, temperature)
     if reduction not in ("mean", "sum", "none"):
         raise ValueError('Reduction parameter unknown.')
-    target = TopLogits(*target)
-    values, indices, lse = target
+    values, indices, lse = target if isinstance(target, TopLogits) else TopLogits(*target)
     shape, C = pred.shape, pred.shape[dim]
     k = values.shape[dim] if values.dim() == pred.dim() else 0
     want = shape[:dim] + (k,) + shape[dim + 1:]
@@ -191,9 +199,10 @@ def distill_loss_topk(pred, target, temperature=1.0, reduction="mean", dim=1, we
         raise TypeError(f"values of floating point type are expected, got {values.dtype}")
     if lse is not None and (lse.shape != shape[:dim] + shape[dim + 1:] or not lse.dtype.is_floating_point):
         raise ValueError(f"lse has to have the logits' shape without dimension {dim} and a floating point type, got {tuple(lse.shape)} {lse.dtype}")
-    if any(t is not None and t.device != pred.device for t in target):
+    device = pred.device
+    if values.device != device or indices.device != device or (lse is not None and lse.device != device):
         raise ValueError("logits and target have to be on the same device")
-    if any(t is not None and t.requires_grad for t in target):
+    if values.requires_grad or (lse is not None and lse.requires_grad):
         raise ValueError("the target is data: detach the teacher's logits")
     if not pred.is_cuda or pred.numel() == 0:
         return _host_distill(pred, values, indices, lse, dim, temperature, weight, reduction)
@@ -203,7 +212,9 @@ def distill_loss_topk(pred, target, temperature=1.0, reduction="mean", dim=1, we
     want_grad = torch.is_grad_enabled() and pred.requires_grad
     if lse is not None and lse.dtype != torch.float32:
         lse = lse.float()
-    return _DistillFn.apply(pred, values, indices, lse, dim, temperature, weight, reduction, want_grad)
+    if not want_grad:                                        # no node to be made (3 us)
+        return _DistillFn.forward(None, pred, values, indices, lse, dim, temperature, weight, reduction, False)
+    return _DistillFn.apply(pred, values, indices, lse, dim, temperature, weight, reduction, True)
 
 
 # ------------------------------------------------------------------------------------ host tensors

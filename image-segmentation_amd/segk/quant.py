@@ -32,6 +32,13 @@ class MXFP4:
             raise ValueError("codes have to be 16-byte aligned and scales 4-byte aligned")
         self.codes, self.scales, self.cols = codes, scales, int(cols)
 
+    @classmethod
+    def _of(cls, codes, scales, cols):
+        """What mxfp4_quantize allocated: its shapes need no check."""
+        q = object.__new__(cls)
+        q.codes, q.scales, q.cols = codes, scales, cols
+        return q
+
     rows = property(lambda s: s.codes.shape[0])
     shape = property(lambda s: (s.codes.shape[0], s.cols))
     device = property(lambda s: s.codes.device)
@@ -53,18 +60,21 @@ def _rows(x, what):
         raise TypeError(f"{what} has to be a floating point tensor with at least one dimension")
     if x.shape[-1] < 1:
         raise ValueError(f"{what} has no columns")
-    if torch.is_grad_enabled() and x.requires_grad:
-        raise RuntimeError(f"{what} requires a gradient and 4-bit rounding has none: call under torch.no_grad() or detach it")
     if x.requires_grad:
+        if torch.is_grad_enabled():
+            raise RuntimeError(f"{what} requires a gradient and 4-bit rounding has none: call under torch.no_grad() or detach it")
         x = x.detach()
     if x.dtype == torch.float16:
         x = x.float()
     dt(x.dtype)
     if x.dim() != 2:
         x = x.reshape(-1, x.shape[-1])
-    if x.shape[1] > 1 and x.stride(1) != 1 or x.shape[0] > 1 and x.stride(0) < x.shape[1]:
+    rows, cols = x.shape
+    if x.is_contiguous():
+        return x, cols
+    if cols > 1 and x.stride(1) != 1 or rows > 1 and x.stride(0) < cols:
         x = x.contiguous()
-    return x, (x.stride(0) if x.shape[0] > 1 else x.shape[1])
+    return x, (x.stride(0) if rows > 1 else cols)
 
 
 def mxfp4_quantize(x):
@@ -75,14 +85,14 @@ def mxfp4_quantize(x):
     rows, cols = x.shape
     if not x.is_cuda:
         return MXFP4(*_host_quantize(x), cols)
-    slices = -(-cols // SLICE)
-    codes = torch.empty((rows, slices * (SLICE // 2)), dtype=torch.uint8, device=x.device)
-    scales = torch.empty((slices, rows, 4), dtype=torch.uint8, device=x.device)
+    slices, device = -(-cols // SLICE), x.device
+    codes = torch.empty((rows, slices * (SLICE // 2)), dtype=torch.uint8, device=device)
+    scales = torch.empty((slices, rows, 4), dtype=torch.uint8, device=device)
     if rows:
         dev, st = _env(x)
         with ops._streamed("4-bit packing", x.numel() * (x.element_size() + 0.53125)):
             call("segk_mxfp4_quantize", dt(x.dtype), x.data_ptr(), ld, rows, cols, codes.data_ptr(), scales.data_ptr(), dev, st)
-    return MXFP4(codes, scales, cols)
+    return MXFP4._of(codes, scales, cols)
 
 
 def mxfp4_dequantize(q, dtype=torch.float32):
@@ -90,9 +100,9 @@ def mxfp4_dequantize(q, dtype=torch.float32):
     if dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"float32 or bfloat16 hold these values exactly, not {dtype}")
     rows, cols = q.shape
-    if q.codes.device.type != "cuda":
+    if not q.codes.is_cuda:
         return _host_dequantize(q).to(dtype)
-    y = torch.empty((rows, cols), dtype=dtype, device=q.device)
+    y = torch.empty((rows, cols), dtype=dtype, device=q.codes.device)
     if rows:
         dev, st = _env(q.codes)
         with ops._streamed("4-bit unpacking", y.numel() * (y.element_size() + 0.53125)):
@@ -121,23 +131,24 @@ def mxfp4_linear(x, w, bias=None, out_dtype=None):
         M = x.shape[0]
     if kx != K:
         raise ValueError(f"x has {kx} columns and w {K}")
-    if x.device != w.device:
+    device = w.codes.device
+    if x.device != device:
         raise ValueError("x and w have to be on the same device")
     if bias is not None:
-        if bias.shape != (N,) or bias.device != w.device or not bias.dtype.is_floating_point:
+        if bias.shape != (N,) or bias.device != device or not bias.dtype.is_floating_point:
             raise ValueError(f"bias has to be a floating point tensor [{N}] on the device of w")
-        if torch.is_grad_enabled() and bias.requires_grad:
+        if bias.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("bias requires a gradient: call under torch.no_grad() or detach it")
         if bias.dtype != torch.float32 or bias.requires_grad or not bias.is_contiguous():
             bias = bias.detach().float().contiguous()
-    if w.codes.device.type != "cuda":
+    if not w.codes.is_cuda:
         xq = _host_dequantize(x if packed else MXFP4(*_host_quantize(x), K))
         y = xq @ _host_dequantize(w).t()
         return (y if bias is None else y + bias).to(out_dtype).reshape(lead + (N,))
-    y = torch.empty((M, N), dtype=torch.float32 if out_dtype == torch.float16 else out_dtype, device=w.device)
+    y = torch.empty((M, N), dtype=torch.float32 if out_dtype == torch.float16 else out_dtype, device=device)
     if M and N:
         nbytes = 0 if packed else query("segk_mxfp4_linear_workspace", M, K, N)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=w.device) if nbytes else None     # one for every call: nothing is shared
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None     # one for every call: nothing is shared
         dev, st = _env(w.codes)
         with ops._streamed("4-bit linear", M * K * (0.53125 if packed else x.element_size()) + N * K * 0.53125 + M * N * y.element_size()):
             call("segk_mxfp4_linear", None if packed else x.data_ptr(), 0 if packed else dt(x.dtype), 0 if packed else ld,

@@ -240,6 +240,21 @@ def test_upstream_gradients_and_a_second_backward_pass(shape):
     torch.testing.assert_close(x.grad, g * w.unsqueeze(1), rtol=2.0 ** -20, atol=2 * 2 * 4 * 2.0 ** -24 * 2)
 
 
+def test_a_second_differentiation_is_refused():
+    z, values, indices, lse = problem(4, 50, 3)
+    x = z.cuda().requires_grad_()
+    loss = distill_loss_topk(x, TopLogits(values.cuda(), indices.cuda(), lse.cuda()))
+    want, = torch.autograd.grad(loss, x, retain_graph=True)
+    g, = torch.autograd.grad(loss, x, create_graph=True)
+    assert torch.equal(g.detach(), want)
+    with pytest.raises(RuntimeError, match="does not require grad"):           # torch's upstream gradient, a constant 1
+        torch.autograd.grad(g.sum(), x)
+    g, = torch.autograd.grad(loss2 := distill_loss_topk(x, TopLogits(values.cuda(), indices.cuda(), lse.cuda())) ** 2, x, create_graph=True)
+    assert torch.allclose(g.detach(), 2 * loss.detach() * want, rtol=2.0 ** -20) and loss2.requires_grad
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+
+
 def test_gradient_against_differences_of_the_definition():
     z, values, indices, lse = problem(5, 400, 7, T=1.5)
     x = z.cuda().requires_grad_()
@@ -399,7 +414,7 @@ def test_positions_counted_for_a_mean(P, V, weight):
             plain = distill_loss_topk(z, TopLogits(values, idx, lse), weight=weight)
         # both sum in double, over at most 256 parts that are rounded to fp32, and round the quotient
         tol = 2.0 ** -23 * float(loss.abs().double().sum()) / max(1, int(has.sum()))
-        assert abs(float(counted) - float(want)) <= tol and float(plain) == float(counted)
+        assert abs(float(counted.detach()) - float(want)) <= tol and float(plain) == float(counted.detach())
 
 
 @pytest.mark.parametrize("N,side", [(3, 8), (2, 66), (1, 21), (5, 130), (1, 1700)])
