@@ -989,7 +989,7 @@ constexpr int kMostCandidates = 1024;
 
 // Rows of one wave: four of them share a workgroup while their lists are short, and do not wait for each other.  A million rows of 80
 // (300) fp32 logits: 645 -> 455 (761 -> 537) us, 8000 rows of 80: 7.9 -> 7.0.  With the lists of longer rows fewer waves fit a CU: 32000
-// rows of 1000 logits 34 -> 39.
+// rows of 1000 logits 34 -> 39.  (Lists of 512 entries: 100000 rows of 600 bf16 logits 131 -> 81 us.)
 constexpr int rows_per_group(int nt, int nch) { return nt == 64 && nch <= 2 ? 4 : 1; }
 template <int R> __device__ __forceinline__ void sync_row() {
     if constexpr (R > 1) {
@@ -1009,10 +1009,10 @@ template <int R> __device__ __forceinline__ void sync_row() {
 // The row is read once: 4096 rows of 32000 bf16 logits, 32 kept: 262 MB in 60 us, 4.4 TB/s (the read alone: 48).  What is left are
 // the search of (2), during which one wave works, and the exponentials; other rows on the CU cover most of both.
 template <typename T, int NT, int NCH>
-__global__ __launch_bounds__(NT * rows_per_group(NT, NCH)) void top_rows_kernel(const T* __restrict__ z, int64_t rows, int64_t ld, int V, int k, float invT, T* __restrict__ values,
+__global__ __launch_bounds__(NT * rows_per_group(NT, NCH), NT * NCH == 4096 ? 6 : 1) void top_rows_kernel(const T* __restrict__ z, int64_t rows, int64_t ld, int V, int k, float invT, T* __restrict__ values,
                                                       int32_t* __restrict__ indices, float* __restrict__ lse) {
     constexpr int VEC = Piece<T>::VEC, NW = NT / 64, R = rows_per_group(NT, NCH);
-    constexpr int kCandidates = NCH > 0 && NT * NCH * VEC < kMostCandidates ? NT * NCH * VEC : kMostCandidates;
+    constexpr int kMost = R > 1 ? kMostCandidates / 2 : kMostCandidates, kCandidates = NCH > 0 && NT * NCH * VEC < kMost ? NT * NCH * VEC : kMost;
     __shared__ struct {
         float m[NT], k[NW], s[NW];
         uint32_t ck[kCandidates], bound;
@@ -1074,15 +1074,23 @@ __global__ __launch_bounds__(NT * rows_per_group(NT, NCH)) void top_rows_kernel(
 #pragma unroll
         for (int w = 0; w < NW; ++w) s += sh.k[w] == -INFINITY ? sh.s[w] : sh.s[w] * exp_over(sh.k[w], kk, c);
         if (lane == 0 && lse) lse[row] = (kk == -INFINITY && s == 0.f) ? -INFINITY : kk * invT + log2f(s) * kLn2;
-        uint32_t key[NW];
+        // 64 to 256 groups of threads, whatever the workgroup's size: 1024 rows of 128011 bf16 (fp32) logits with up to 1024 groups 100 (234)
+        // us, with 256 85 (156)
+        constexpr int NG = NW < 4 ? NW : 4;
+        uint32_t key[NG];
 #pragma unroll
-        for (int w = 0; w < NW; ++w) key[w] = order_key(sh.m[w * 64 + lane]);
+        for (int g = 0; g < NG; ++g) {
+            float mg = sh.m[g * 64 + lane];
+#pragma unroll
+            for (int w = g + NG; w < NW; w += NG) mg = fmaxf(mg, sh.m[w * 64 + lane]);
+            key[g] = order_key(mg);
+        }
         uint32_t bound = 0;
         for (int bit = 31; bit >= (sizeof(T) == 2 ? 16 : 0); --bit) {
             const uint32_t cand = bound | (1u << bit);
             int n = 0;
 #pragma unroll
-            for (int w = 0; w < NW; ++w) n += __popcll(__ballot(key[w] >= cand));
+            for (int g = 0; g < NG; ++g) n += __popcll(__ballot(key[g] >= cand));
             if (n >= k) {
                 bound = cand;
                 if (n <= k + (k >> 2) + 2) break;
@@ -1285,10 +1293,12 @@ constexpr int kPixelClasses = 32;    // more classes than this: one workgroup (o
 
 // Threads of a row's workgroup and pieces in registers per thread, by the row's length.  Rows of 16 to 64 KB: 512 threads with 8
 // pieces serve the loss, 256 with 16 the selection, whose search by the first wave leaves the others idle (4096 rows of 32000 bf16
-// logits: loss and gradient 103 against 107 us, selection 66 against 56).
-template <typename T, bool TOP, typename F> static void row_tier(int64_t V, F&& f) {
+// logits: loss and gradient 103 against 107 us, selection 66 against 56; six waves of the latter per SIMD instead of five: 67 -> 63).
+template <typename T, bool TOP, typename F> static void row_tier(const void* z, int64_t ld, int64_t V, F&& f) {
     constexpr int VEC = 16 / (int)sizeof(T);
-    const int64_t pieces = (V + 2 * (VEC - 1)) / VEC;           // wherever the row begins
+    // Rows that begin between two pieces may touch one more.  (4096 rows of 16384 bf16 logits, 2048 pieces: selection 52 -> 39 us, loss with
+    // gradient 83 -> 62 since they are not taken for 2049.)
+    const int64_t pieces = (V + (aligned16(z) && ld % VEC == 0 ? VEC - 1 : 2 * (VEC - 1))) / VEC;
 #define SEGK_TIER(nt, nch) if (pieces <= (int64_t)(nt) * (nch)) return f(std::integral_constant<int, nt>{}, std::integral_constant<int, nch>{})
     SEGK_TIER(64, 1);
     SEGK_TIER(64, 2);
@@ -1374,7 +1384,7 @@ extern "C" int segk_top_logits(const void* logits, int dtype, int64_t outer, int
                                    px.s_p, px.inner, (int)C, (int)k, 1.f / temperature, (T*)values, indices, px.ts_c, px.ts_p, lse, px.blocks_each);
             });
         } else {
-            row_tier<T, true>(C, [&](auto nt, auto nch) {
+            row_tier<T, true>(logits, ld, C, [&](auto nt, auto nch) {
                 constexpr int r = rows_per_group(nt(), nch());
                 hipLaunchKernelGGL((top_rows_kernel<T, nt(), nch()>), dim3((unsigned)((outer + r - 1) / r)), dim3(nt(), r), 0, st, (const T*)logits, outer, ld, (int)C, (int)k,
                                    1.f / temperature, (T*)values, indices, lse);
@@ -1480,7 +1490,7 @@ extern "C" int segk_distill(const void* logits, int dtype, int64_t outer, int64_
             hipLaunchKernelGGL((distill_join_kernel<T>), dim3((unsigned)outer), dim3(64), 0, st, a, parts, shares, dlogits ? joined : nullptr, rows_done, loss);
             if (dlogits) hipLaunchKernelGGL((distill_share_grad_kernel<T>), dim3(shares, (unsigned)outer), dim3(256), 0, st, a, joined);
         } else {
-            row_tier<T, false>(C, [&](auto nt, auto nch) {
+            row_tier<T, false>(logits, ld, C, [&](auto nt, auto nch) {
                 if (dlogits) hipLaunchKernelGGL((distill_rows_kernel<T, nt(), nch(), true>), dim3((unsigned)n), dim3(nt()), 0, st, a);
                 else hipLaunchKernelGGL((distill_rows_kernel<T, nt(), nch(), false>), dim3((unsigned)n), dim3(nt()), 0, st, a);
             });

@@ -379,6 +379,26 @@ def test_extreme_temperatures(T):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [1024, 2048, 8192, 16384, 32768, 65536, 131072])
+def test_rows_that_fill_a_kernel_exactly(V, dtype):
+    """Lengths at which a row just fits the registers of a kernel, if it begins and ends with a 16-byte piece, and does not otherwise."""
+    z, values, indices, lse = problem(20, V, 7, seed=V, dtype=dtype)          # 20 rows: not shared by workgroups below 16384 pieces
+
+    def shifted(x):
+        flat = torch.empty(x.numel() + 1, dtype=x.dtype, device="cuda")
+        return flat[1:].view(x.shape).copy_(x)
+
+    def padded(x):
+        return torch.nn.functional.pad(x.cuda(), (0, 1))[:, :V]
+    want = torch.topk(z.double(), 7, 1).values
+    for form in (lambda x: x.cuda(), shifted, padded):
+        got = top_logits(form(z), 7)
+        assert torch.equal(got.values.cpu().double(), want) and torch.equal(z.gather(1, got.indices.cpu().long()), got.values.cpu())
+        assert bool(((got.lse.cpu().double() - torch.logsumexp(z.double(), 1)).abs() <= 2.0 ** -21 * (8 + 3 * z.double().abs().amax(1))).all())
+        check(z, values, indices, lse, 1.0, cuda=form)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("P,V", [(4607, 9), (4608, 9), (8191, 16), (8192, 16), (16384, 32), (16383, 32), (5, 200), (1027, 80)])
 def test_many_short_rows(P, V, dtype):
     """Both sides of the border between a thread and a wave for each row, and rows that do not fill the last workgroup."""
