@@ -1006,7 +1006,7 @@ template <int R> __device__ __forceinline__ void sync_row() {
 // k elements of the row reach it, and hardly more than k in unordered data.  (3) The elements that reach it are collected in LDS
 // and ranked by counting; ties go to the lower index.  Where more than the list holds reach it (many ties) or a NaN is in the row,
 // the exact k-th key and then the last index that still belongs are found by binary searches over the whole row.
-// The row is read once: 4096 rows of 32000 bf16 logits, 32 kept: 262 MB in 60 us, 4.4 TB/s (the read alone: 48).  What is left are
+// The row is read once: 4096 rows of 32000 bf16 logits, 32 kept: 262 MB in 57 us, 4.6 TB/s (the read alone: 48).  What is left are
 // the search of (2), during which one wave works, and the exponentials; other rows on the CU cover most of both.
 template <typename T, int NT, int NCH>
 __global__ __launch_bounds__(NT * rows_per_group(NT, NCH), NT * NCH == 4096 ? 6 : 1) void top_rows_kernel(const T* __restrict__ z, int64_t rows, int64_t ld, int V, int k, float invT, T* __restrict__ values,
@@ -1184,7 +1184,57 @@ __global__ __launch_bounds__(NT * rows_per_group(NT, NCH), NT * NCH == 4096 ? 6 
         });
         sync_row<R>();
     }
-    const int n = sh.count < kCandidates ? sh.count : kCandidates;
+    int n = sh.count < kCandidates ? sh.count : kCandidates;
+    // Many candidates (ties, k near the number of groups): the first wave keeps exactly k of them, so that the ranking, which compares
+    // each with all, stays short (20000 rows of 300 fp32 logits, 64 kept: 378 -> 72 us).
+    if (n > (NT == 64 ? 64 : 128)) {
+        if (wave == 0) {
+            // from LDS each time: in registers they would cost the whole kernel a wave per SIMD
+            auto count = [&](auto&& pred) {
+                int t = 0;
+                for (int j = 0; j < n; j += 64) {
+                    const int i = j + lane;
+                    t += __popcll(__ballot(i < n && pred(sh.ck[i < n ? i : 0], sh.ci[i < n ? i : 0])));
+                }
+                return t;
+            };
+            uint32_t kth = 0;
+            int reach = n;
+            for (int bit = 31; bit >= 0 && reach > k; --bit) {
+                const uint32_t cand = kth | (1u << bit);
+                const int t = count([&](uint32_t q, int) { return q >= cand; });
+                if (t >= k) {
+                    kth = cand;
+                    reach = t;
+                }
+            }
+            int last = 0x7FFFFFFF;                            // of the elements equal to the k-th, the index of the last that belongs
+            if (reach > k) {
+                const int need = k - count([&](uint32_t q, int) { return q > kth; });
+                last = 0;
+                for (int bit = 30; bit >= 0; --bit) {
+                    const int cand = last | (1 << bit);
+                    if (cand < V && count([&](uint32_t q, int e) { return q == kth && e < cand; }) < need) last = cand;
+                }
+            }
+            int to = 0;
+            for (int j = 0; j < n; j += 64) {                 // forward and never past what has been read
+                const int i = j + lane;
+                const uint32_t q = sh.ck[i < n ? i : 0];
+                const int e = sh.ci[i < n ? i : 0];
+                const bool keep = i < n && (q > kth || (q == kth && e <= last));
+                const uint64_t mask = __ballot(keep);
+                if (keep) {
+                    const int d = to + __popcll(mask & ((1ull << lane) - 1));
+                    sh.ck[d] = q;
+                    sh.ci[d] = e;
+                }
+                to += __popcll(mask);
+            }
+        }
+        n = k;
+        sync_row<R>();
+    }
     for (int i = threadIdx.x; i < n; i += NT) {
         const uint32_t q = sh.ck[i];
         const int e = sh.ci[i];
@@ -1294,16 +1344,20 @@ constexpr int kPixelClasses = 32;    // more classes than this: one workgroup (o
 // Threads of a row's workgroup and pieces in registers per thread, by the row's length.  Rows of 16 to 64 KB: 512 threads with 8
 // pieces serve the loss, 256 with 16 the selection, whose search by the first wave leaves the others idle (4096 rows of 32000 bf16
 // logits: loss and gradient 103 against 107 us, selection 66 against 56; six waves of the latter per SIMD instead of five: 67 -> 63).
-template <typename T, bool TOP, typename F> static void row_tier(const void* z, int64_t ld, int64_t V, F&& f) {
+template <typename T, bool TOP, typename F> static void row_tier(const void* z, int64_t ld, int64_t V, int64_t k, F&& f) {
     constexpr int VEC = 16 / (int)sizeof(T);
     // Rows that begin between two pieces may touch one more.  (4096 rows of 16384 bf16 logits, 2048 pieces: selection 52 -> 39 us, loss with
     // gradient 83 -> 62 since they are not taken for 2049.)
     const int64_t pieces = (V + (aligned16(z) && ld % VEC == 0 ? VEC - 1 : 2 * (VEC - 1))) / VEC;
 #define SEGK_TIER(nt, nch) if (pieces <= (int64_t)(nt) * (nch)) return f(std::integral_constant<int, nt>{}, std::integral_constant<int, nch>{})
     SEGK_TIER(64, 1);
-    SEGK_TIER(64, 2);
-    SEGK_TIER(64, 4);
-    SEGK_TIER(64, 8);
+    // The selection's bound lets few candidates through while k is well below the number of threads.  64 / 256 threads, 20000 rows of 2000
+    // bf16 logits: 24 kept 51/68 us, 32 kept 70/71, 64 kept 527/111; of 300 fp32 logits, all of which its list holds, 64 kept: 72/115.
+    if (!TOP || k <= 24 || V <= 512) SEGK_TIER(64, 2);
+    if (!TOP || k <= 24) {
+        SEGK_TIER(64, 4);
+        SEGK_TIER(64, 8);
+    }
     SEGK_TIER(256, 4);
     SEGK_TIER(256, 8);
     if constexpr (TOP) {
@@ -1384,7 +1438,7 @@ extern "C" int segk_top_logits(const void* logits, int dtype, int64_t outer, int
                                    px.s_p, px.inner, (int)C, (int)k, 1.f / temperature, (T*)values, indices, px.ts_c, px.ts_p, lse, px.blocks_each);
             });
         } else {
-            row_tier<T, true>(logits, ld, C, [&](auto nt, auto nch) {
+            row_tier<T, true>(logits, ld, C, k, [&](auto nt, auto nch) {
                 constexpr int r = rows_per_group(nt(), nch());
                 hipLaunchKernelGGL((top_rows_kernel<T, nt(), nch()>), dim3((unsigned)((outer + r - 1) / r)), dim3(nt(), r), 0, st, (const T*)logits, outer, ld, (int)C, (int)k,
                                    1.f / temperature, (T*)values, indices, lse);
@@ -1490,7 +1544,7 @@ extern "C" int segk_distill(const void* logits, int dtype, int64_t outer, int64_
             hipLaunchKernelGGL((distill_join_kernel<T>), dim3((unsigned)outer), dim3(64), 0, st, a, parts, shares, dlogits ? joined : nullptr, rows_done, loss);
             if (dlogits) hipLaunchKernelGGL((distill_share_grad_kernel<T>), dim3(shares, (unsigned)outer), dim3(256), 0, st, a, joined);
         } else {
-            row_tier<T, false>(logits, ld, C, [&](auto nt, auto nch) {
+            row_tier<T, false>(logits, ld, C, k, [&](auto nt, auto nch) {
                 if (dlogits) hipLaunchKernelGGL((distill_rows_kernel<T, nt(), nch(), true>), dim3((unsigned)n), dim3(nt()), 0, st, a);
                 else hipLaunchKernelGGL((distill_rows_kernel<T, nt(), nch(), false>), dim3((unsigned)n), dim3(nt()), 0, st, a);
             });

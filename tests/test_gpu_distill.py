@@ -379,6 +379,51 @@ def test_extreme_temperatures(T):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("P", [1, 3, 129])
+@pytest.mark.parametrize("V,k", [(16384, 64), (33793, 64), (40963, 5), (66049, 1), (131585, 33), (262147, 64)])
+def test_top_of_long_rows(V, k, P, dtype):
+    """Ties, NaN and infinities in long rows."""
+    g = torch.Generator().manual_seed(V)
+    base = 2 * torch.randn(3, V, generator=g)
+    base[1] = torch.randint(-2, 3, (V,), generator=g).float()                # ties everywhere
+    base[2] = -math.inf
+    base[2, ::V // 40] = base[0, ::V // 40]                                   # 40 or 41 finite logits: fewer than 64
+    for last in (None, math.nan, math.inf):
+        z = base.clone()
+        if last is not None:
+            z[0, V - 1] = last
+            z[1, V // 2] = last
+        z = z.to(dtype).repeat(-(-P // 3), 1)[:P]
+        host = top_logits(z[:3], k, temperature=2.0)
+        got = top_logits(z.cuda(), k, temperature=2.0)
+        for lo in range(0, P, 3):
+            n = min(3, P - lo)
+            same = got.values[lo:lo + n].cpu().eq(host.values[:n]) | (got.values[lo:lo + n].cpu().isnan() & host.values[:n].isnan())
+            assert bool(same.all()) and torch.equal(got.indices[lo:lo + n].cpu(), host.indices[:n])
+        want = torch.logsumexp(z[:3].double() / 2, 1)
+        for row in range(min(P, 3)):
+            lse = got.lse[row::3].cpu()
+            if not math.isfinite(want[row]):
+                assert lse.isnan().all()
+            else:
+                top = float(z[row][z[row].isfinite()].double().abs().max())
+                assert bool(((lse.double() - want[row]).abs() <= 2.0 ** -21 * (8 + 3 * top / 2)).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("V", [70, 500, 1000, 2000, 4000, 9000])
+def test_as_many_as_can_be_kept(V, dtype):
+    """k = 64 of rows whose threads are hardly more: many candidates, in order, in reverse, equal, or in runs."""
+    g = torch.Generator().manual_seed(V)
+    rows = [torch.randn(V, generator=g), torch.arange(V) / 64.0, -torch.arange(V) / 64.0, torch.zeros(V), torch.randint(0, 4, (V,), generator=g).float(),
+            (torch.arange(V) // 64).float(), torch.where(torch.arange(V) < V - 66, -math.inf, torch.randn(V, generator=g)), torch.arange(V).fmod(65.0)]
+    z = torch.stack(rows).to(dtype)
+    for k in (33, 63, 64):
+        host, got = top_logits(z, k), top_logits(z.cuda(), k)
+        assert torch.equal(got.values.cpu(), host.values) and torch.equal(got.indices.cpu(), host.indices)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("V", [1024, 2048, 8192, 16384, 32768, 65536, 131072])
 def test_rows_that_fill_a_kernel_exactly(V, dtype):
     """Lengths at which a row just fits the registers of a kernel, if it begins and ends with a 16-byte piece, and does not otherwise."""
