@@ -826,6 +826,150 @@ __global__ __launch_bounds__(256) void distill_pixels_kernel(const DistillArgs a
     }
 }
 
+// Class planes of 33 to 256 classes: one thread for a position again, but its classes do not fit its registers: they are read once for
+// the maximum and the sum of those outside (running, eight loads in flight) and once more for the gradient.  The kept classes are bits
+// of eight registers; their logits are gathered in the loops over the entries, and their gradients overwrite what the second pass
+// wrote there.  8 x 80 x 256 x 256 fp32 logits, 1 (8) kept, with
+// gradient: 126 (320) us, 4.0 (1.6) TB/s of three passes; copied into rows first 553 (829).  With many entries their gathers bound it.
+constexpr int kPlaneClasses = 256, kPlaneTop = 8;
+
+// f(first class, eight logits, the bits of those kept) for all classes of a position; beyond the last: -inf
+template <typename T, typename F> __device__ __forceinline__ void each_eight(const T* z, int64_t stride, int V, const uint32_t (&kept)[kPlaneClasses / 32], F&& f) {
+#pragma unroll
+    for (int w = 0; w < kPlaneClasses / 32; ++w) {
+        const int end = V < w * 32 + 32 ? V : w * 32 + 32;
+        for (int q0 = w * 32; q0 < end; q0 += 8) {
+            float x[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) x[u] = q0 + u < V ? Elem<T>::to_f(z[(q0 + u) * stride]) : -INFINITY;
+            f(q0, x, (kept[w] >> (q0 & 31)) & 0xFFu);
+        }
+    }
+}
+
+template <typename T, bool GRAD>
+__global__ __launch_bounds__(256) void distill_planes_kernel(const DistillArgs a, int blocks_each) {
+    if (a.skip_if_one && a.upstream[0] == 1.f) return;
+    __shared__ float red[4];
+    const int64_t o = blockIdx.x / blocks_each, i = (int64_t)(blockIdx.x % blocks_each) * 256 + threadIdx.x;
+    const float c = a.invT * kLog2e;
+    const float gs = GRAD && !a.up_each ? grad_scale(a, 0) : 0.f;
+    float l = 0.f;
+    if (i < a.inner) {
+        const T* z = static_cast<const T*>(a.z) + o * a.ld + i;
+        const int64_t pos = o * a.inner + i, at = o * a.k * a.inner + i;
+        const float lse = a.tlse ? a.tlse[pos] : 0.f;
+        auto logit = [&](int cls) { return Elem<T>::to_f(z[cls * a.inner]); };
+        float top = -INFINITY;
+        if (!a.tlse)                          // renormalised: the greatest of the kept logits first
+            for (int j = 0; j < a.k; ++j)
+                if (load_class(a, at + j * a.inner) >= 0) top = fmaxf(top, load_kept(a, at + j * a.inner));
+        auto log_p = [&](int j) {             // base 2, before it is normalised where no logsumexp is given
+            const float t = load_kept(a, at + j * a.inner);
+            return a.tlse ? fmaf(t, a.invT, -lse) * kLog2e : (top == -INFINITY ? -INFINITY : (t - top) * c);
+        };
+        uint32_t kept[kPlaneClasses / 32] = {};
+        bool twice = false;
+        float mass = 0.f, plogp = 0.f, km = -INFINITY, sm = 0.f;
+        for (int j = 0; j < a.k; ++j) {
+            const int cls = load_class(a, at + j * a.inner);
+            if (cls < 0) continue;
+            const float lp = log_p(j), p = fast_exp2(lp);
+            mass += p;
+            plogp += p == 0.f ? 0.f : p * lp;
+            bool seen = false;
+#pragma unroll
+            for (int w = 0; w < kPlaneClasses / 32; ++w) {
+                const uint32_t bit = cls >> 5 == w ? 1u << (cls & 31) : 0u;
+                seen = seen || (kept[w] & bit);
+                kept[w] |= bit;
+            }
+            twice = twice || seen;
+            if (!seen) {
+                const float zj = logit(cls);
+                if (zj > km) {
+                    sm *= rebase(km, zj, c);
+                    km = zj;
+                }
+                sm += exp_over(zj, km == -INFINITY ? 0.f : km, c);
+            }
+        }
+        int distinct = 0;
+#pragma unroll
+        for (int w = 0; w < kPlaneClasses / 32; ++w) distinct += __popc(kept[w]);
+        float ko = -INFINITY, so = 0.f;
+        if (distinct)
+            each_eight(z, a.inner, a.V, kept, [&](int, float (&x)[8], uint32_t in) {
+                float m = ko;
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    x[u] = (in >> u) & 1u ? -INFINITY : x[u];
+                    m = fmaxf(m, x[u]);
+                }
+                so *= m > ko ? rebase(ko, m, c) : 1.f;
+                ko = m;
+                const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+                for (int u = 0; u < 8; ++u) so += exp_over(x[u], base, c);
+            });
+        float rest = 0.f, norm = 1.f;
+        if (a.tlse) {
+            rest = 1.f - mass;
+            if (!(rest > kRestFloor) || distinct == a.V) rest = 0.f;
+        } else {
+            norm = mass == 0.f ? 0.f : 1.f / mass;
+            plogp = mass == 0.f ? 0.f : plogp * norm - log2f(mass);
+            mass *= norm;
+        }
+        const float all = mass + rest;
+        const float kk = fmaxf(ko, km), bo = ko == -INFINITY ? 0.f : ko, bm = km == -INFINITY ? 0.f : km;
+        const float fo = rebase(ko, kk, c), fm = rebase(km, kk, c), s = so * fo + sm * fm + (so != so ? so : 0.f);
+        if (distinct) {
+            const float ls = log2f(s);
+            l = plogp;
+            for (int j = 0; j < a.k; ++j) {
+                const int cls = load_class(a, at + j * a.inner);
+                const float p = cls >= 0 ? fast_exp2(log_p(j)) * norm : 0.f;
+                if (cls >= 0 && p != 0.f) l -= p * ((logit(cls) - kk) * c - ls);
+            }
+            if (rest > 0.f) l += rest * (log2f(rest) - (log2f(so) + (ko - kk) * c - ls));
+            l *= kLn2 * a.T * a.T * a.weight;
+        }
+        if (a.row_loss) a.row_loss[pos] = l;
+        if constexpr (GRAD) {
+            const float g = a.up_each ? a.weight * a.T * a.upstream[pos] : gs;           // no mean goes with one gradient for each position
+            const float inv = 1.f / s, fk = g * all * fm * inv, fr = g * (all * fo * inv - (rest > 0.f ? rest / so : 0.f));
+            T* d = static_cast<T*>(a.dz) + o * a.ld_d + i;
+            if (distinct) {
+                each_eight(z, a.inner, a.V, kept, [&](int q0, float (&x)[8], uint32_t) {
+#pragma unroll
+                    for (int u = 0; u < 8; ++u)
+                        if (q0 + u < a.V) d[(q0 + u) * a.inner] = Elem<T>::from_f(exp_over(x[u], bo, c) * fr);
+                });
+                for (int j = 0; j < a.k; ++j) {
+                    const int cls = load_class(a, at + j * a.inner);
+                    if (cls < 0) continue;
+                    float p = fast_exp2(log_p(j));
+                    if (twice) {
+                        p = 0.f;
+                        for (int h = 0; h < a.k; ++h)
+                            if (load_class(a, at + h * a.inner) == cls) p += fast_exp2(log_p(h));
+                    }
+                    d[cls * a.inner] = Elem<T>::from_f(exp_over(logit(cls), bm, c) * fk - g * (p * norm));
+                }
+            } else {
+                for (int q = 0; q < a.V; ++q) d[q * a.inner] = Elem<T>::from_f(0.f);
+            }
+        }
+    }
+    if (a.partial) {
+        l = sum_wave(l);
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = l;
+        __syncthreads();
+        if (threadIdx.x == 0) a.partial[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+    }
+}
+
 // Positions with at least one kept logit: one partial count for each workgroup.
 // Rows: the entries of 64 / kp rows at a time, one for each lane, kp = k rounded up to a power of two.
 __global__ __launch_bounds__(256) void distill_count_rows_kernel(const DistillArgs a, int64_t rows, int log_kp, int* __restrict__ counts) {
@@ -1338,6 +1482,62 @@ __global__ __launch_bounds__(256) void top_pixels_kernel(const T* __restrict__ z
     }
 }
 
+// Class planes of 33 to 256 classes, up to KM of them kept: a thread for a position reads them once and keeps a sorted list in registers,
+// the keys of the logits and their classes; equal keys stay in the order of their classes.  8 x 80 x 256 x 256 fp32 logits, the best 1
+// (8): 36 (70) us, 4.6 (2.4) TB/s; copied into rows first 354 (483).
+template <typename T, int KM>
+__global__ __launch_bounds__(256) void top_planes_kernel(const T* __restrict__ z, int64_t ld, int64_t inner, int V, int k, float invT, T* __restrict__ values,
+                                                         int32_t* __restrict__ indices, float* __restrict__ lse, int blocks_each) {
+    const int64_t o = blockIdx.x / blocks_each, i = (int64_t)(blockIdx.x % blocks_each) * 256 + threadIdx.x;
+    if (i >= inner) return;
+    const float c = invT * kLog2e;
+    z += o * ld + i;
+    const uint32_t none[kPlaneClasses / 32] = {};
+    uint32_t key[KM];                          // 0: nothing yet, less than the key of any logit
+    int cls[KM];
+#pragma unroll
+    for (int j = 0; j < KM; ++j) {
+        key[j] = 0;
+        cls[j] = 0;
+    }
+    float top = -INFINITY, s = 0.f;
+    each_eight(z, inner, V, none, [&](int q0, float (&x)[8], uint32_t) {
+        float m = top;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) m = fmaxf(m, x[u]);
+        s *= m > top ? rebase(top, m, c) : 1.f;
+        top = m;
+        const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            s += exp_over(x[u], base, c);
+            uint32_t q = order_key(x[u]);
+            if (q0 + u < V && q > key[KM - 1]) {
+                int e = q0 + u;
+                bool in = false;               // from its place on everything moves down
+#pragma unroll
+                for (int j = 0; j < KM; ++j) {
+                    in = in || q > key[j];
+                    const uint32_t kj = key[j];
+                    const int cj = cls[j];
+                    key[j] = in ? q : kj;
+                    cls[j] = in ? e : cj;
+                    q = in ? kj : q;
+                    e = in ? cj : e;
+                }
+            }
+        }
+    });
+    if (lse) lse[o * inner + i] = (top == -INFINITY && s == 0.f) ? -INFINITY : (top == -INFINITY ? 0.f : top) * invT + log2f(s) * kLn2;
+    const int64_t t0 = o * k * inner + i;
+#pragma unroll
+    for (int j = 0; j < KM; ++j)
+        if (j < k) {
+            values[t0 + j * inner] = z[cls[j] * inner];
+            indices[t0 + j * inner] = cls[j];
+        }
+}
+
 // ------------------------------------------------------------------------------------------------ host
 constexpr int kPixelClasses = 32;    // more classes than this: one workgroup (or wave) per row
 
@@ -1372,12 +1572,12 @@ template <typename T, bool TOP, typename F> static void row_tier(const void* z, 
 }
 
 static int check_logits(const char* who, const void* z, int dtype, int64_t outer, int64_t C, int64_t inner, int64_t ld, int64_t k,
-                        float temperature) {
+                        float temperature, int most_planes) {
     SEGK_REQUIRE(z, SEGK_EINVAL, "%s: null pointer", who);
     SEGK_REQUIRE(dtype == SEGK_F32 || dtype == SEGK_BF16, SEGK_EINVAL, "%s: unknown dtype %d", who, dtype);
     SEGK_REQUIRE(outer > 0 && C > 0 && inner > 0 && outer < (1ll << 31) && C < (1ll << 30) && inner < (1ll << 31), SEGK_ESHAPE, "%s: bad shape", who);
     SEGK_REQUIRE(outer * inner < (1ll << 31), SEGK_ESHAPE, "%s: 2^31 positions and more", who);
-    SEGK_REQUIRE(inner == 1 || C <= kPixelClasses, SEGK_ESHAPE, "%s: more than %d classes have to be the innermost dimension", who, kPixelClasses);
+    SEGK_REQUIRE(inner == 1 || C <= most_planes, SEGK_ESHAPE, "%s: more than %d classes have to be the innermost dimension", who, most_planes);
     SEGK_REQUIRE(ld >= C * inner, SEGK_ESHAPE, "%s: ld smaller than one row / image", who);
     SEGK_REQUIRE(k >= 1 && k <= kTopMax && k <= C, SEGK_ESHAPE, "%s: k must be between 1 and %d and at most the number of classes", who, kTopMax);
     // so that neither 1 / T nor T^2 leaves the range of fp32
@@ -1410,6 +1610,8 @@ static Pixels pixels(int64_t outer, int64_t C, int64_t inner, int64_t ld, int64_
 // 4.1/5.1, 9.9/9.5, of 32 9.3/5.1, 18.0/9.4.
 static bool few(int64_t outer, int64_t C, int64_t inner) { return C <= kPixelClasses && (inner > 1 || C <= 8 || outer >= 512 * C); }
 
+static bool planes(int64_t C, int64_t inner) { return inner > 1 && C > kPixelClasses; }
+
 template <typename F> static void class_tier(int64_t C, int vp, F&& f) {
     if (C <= 4) return vp == 4 ? f(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{}) : f(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
     if (C <= 8) return vp == 4 ? f(std::integral_constant<int, 8>{}, std::integral_constant<int, 4>{}) : f(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
@@ -1423,16 +1625,20 @@ using namespace segk;
 
 extern "C" int segk_top_logits(const void* logits, int dtype, int64_t outer, int64_t C, int64_t inner, int64_t ld, int64_t k, float temperature,
                                void* values, int32_t* indices, float* lse, int dev, void* stream) {
-    if (const int rc = check_logits("top_logits", logits, dtype, outer, C, inner, ld, k, temperature)) return rc;
+    if (const int rc = check_logits("top_logits", logits, dtype, outer, C, inner, ld, k, temperature, k <= kPlaneTop ? kPlaneClasses : kPixelClasses)) return rc;
     SEGK_REQUIRE(values && indices, SEGK_EINVAL, "top_logits: null output");
     SEGK_REQUIRE(aligned16(values) && aligned16(indices) && aligned16(lse), SEGK_EALIGN, "top_logits: outputs must be 16-byte aligned");
-    const bool pix = few(outer, C, inner);
+    const bool wide = planes(C, inner), pix = wide || few(outer, C, inner);
     const Pixels px = pixels(outer, C, inner, ld, k, aligned16(logits));
     SEGK_REQUIRE(!pix || px.blocks < (1ll << 31), SEGK_ESHAPE, "top_logits: too many positions");
     SEGK_USE_DEVICE(dev);
     hipStream_t st = (hipStream_t)stream;
     SEGK_DISPATCH_DTYPE(dtype, T, {
-        if (pix) {
+        if (wide) {
+            auto kernel = k <= 2 ? top_planes_kernel<T, 2> : top_planes_kernel<T, kPlaneTop>;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)px.blocks), dim3(256), 0, st, (const T*)logits, ld, px.inner, (int)C, (int)k, 1.f / temperature, (T*)values,
+                               indices, lse, px.blocks_each);
+        } else if (pix) {
             class_tier(C, px.vp, [&](auto cm, auto vp) {
                 hipLaunchKernelGGL((top_pixels_kernel<T, cm(), vp()>), dim3((unsigned)px.blocks), dim3(256), 0, st, (const T*)logits, ld, px.s_c,
                                    px.s_p, px.inner, (int)C, (int)k, 1.f / temperature, (T*)values, indices, px.ts_c, px.ts_p, lse, px.blocks_each);
@@ -1465,7 +1671,7 @@ static constexpr int kCollect = 256, kFinal = 16384;      // from more than kFin
 static_assert(kCollect == kCountBlocks);
 // floats of the workspace: partial counts, level-1 sums, then one sum per row or workgroup
 static size_t distill_partials(int64_t outer, int64_t C, int64_t inner) {
-    if (!few(outer, C, inner)) return (size_t)outer * (outer <= 128 ? 1 + 2 * kShares + kRowFloats : 1) + 1;
+    if (!planes(C, inner) && !few(outer, C, inner)) return (size_t)outer * (outer <= 128 ? 1 + 2 * kShares + kRowFloats : 1) + 1;
     return (size_t)(pixels(outer, C, inner, C * inner, 1, false).blocks);      // an upper bound for either vector width
 }
 extern "C" size_t segk_distill_workspace(int64_t outer, int64_t C, int64_t inner) {
@@ -1477,7 +1683,7 @@ extern "C" int segk_distill(const void* logits, int dtype, int64_t outer, int64_
                             const void* indices, int index_bytes, const float* teacher_lse, int64_t k, float temperature, float weight, int flags,
                             const float* upstream, float* loss, float* position_loss, void* dlogits, int64_t ld_d, void* workspace,
                             size_t workspace_bytes, int dev, void* stream) {
-    if (const int rc = check_logits("distill", logits, dtype, outer, C, inner, ld, k, temperature)) return rc;
+    if (const int rc = check_logits("distill", logits, dtype, outer, C, inner, ld, k, temperature, kPlaneClasses)) return rc;
     const bool mean = flags & 1, each = flags & 2, skip = flags & 4;
     SEGK_REQUIRE(values && indices && workspace, SEGK_EINVAL, "distill: null pointer");
     SEGK_REQUIRE(values_dtype == SEGK_F32 || values_dtype == SEGK_BF16, SEGK_EINVAL, "distill: unknown dtype %d of the values", values_dtype);
@@ -1489,7 +1695,7 @@ extern "C" int segk_distill(const void* logits, int dtype, int64_t outer, int64_
     SEGK_REQUIRE(!dlogits || (ld_d >= C * inner && reinterpret_cast<uintptr_t>(dlogits) % esize(dtype) == 0), SEGK_ESHAPE, "distill: bad dlogits");
     SEGK_REQUIRE(workspace_bytes >= segk_distill_workspace(outer, C, inner), SEGK_EWORKSPACE, "distill: workspace too small");
     SEGK_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 4 == 0, SEGK_EALIGN, "distill: workspace must be 4-byte aligned");
-    const bool pix = few(outer, C, inner);
+    const bool wide = planes(C, inner), pix = wide || few(outer, C, inner);
     const bool vec = aligned16(logits) && (!dlogits || (aligned16(dlogits) && ld_d % 4 == 0)) && aligned16(values) && aligned16(indices) && aligned16(teacher_lse);
     const Pixels px = pixels(outer, C, inner, ld, k, vec);
     SEGK_REQUIRE(!pix || px.blocks < (1ll << 31), SEGK_ESHAPE, "distill: too many positions");
@@ -1531,7 +1737,10 @@ extern "C" int segk_distill(const void* logits, int dtype, int64_t outer, int64_
     int64_t n = pix ? px.blocks : outer;
     bool summed = false;
     SEGK_DISPATCH_DTYPE(dtype, T, {
-        if (pix) {
+        if (wide) {
+            auto kernel = dlogits ? distill_planes_kernel<T, true> : distill_planes_kernel<T, false>;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(256), 0, st, a, px.blocks_each);
+        } else if (pix) {
             class_tier(C, px.vp, [&](auto cm, auto vp) {
                 if (dlogits) hipLaunchKernelGGL((distill_pixels_kernel<T, cm(), vp(), true>), dim3((unsigned)n), dim3(256), 0, st, a, px.blocks_each);
                 else hipLaunchKernelGGL((distill_pixels_kernel<T, cm(), vp(), false>), dim3((unsigned)n), dim3(256), 0, st, a, px.blocks_each);

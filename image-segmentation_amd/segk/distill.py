@@ -11,7 +11,10 @@ from .ops import _env, dt
 
 MEAN, EACH, SKIP = 1, 2, 4          # flag bits of segk_distill
 MAX_K = 64
-PLANE_CLASSES = 32                  # up to this many classes the kernels read class planes [N, C, ...] as they are
+# Class planes [N, C, ...] are read as they are up to PLANE_FEW classes, and up to PLANE_CLASSES (selection: of PLANE_TOP at most) if there
+# are PLANE_POSITIONS; others are copied into rows.  In place / copied, selection and loss with gradient, fp32, 8 kept, us: 128 x 128
+# positions of 33 classes 11/22, 29/46, of 150 38/31, 45/59; 64 x 64 of 150 41/12, 45/28; 8 x 256 x 256 of 80 70/483, 320/829.
+PLANE_FEW, PLANE_CLASSES, PLANE_TOP, PLANE_POSITIONS = 32, 256, 8, 16384
 REST_FLOOR = 2.0 ** -20             # a rest of the teacher's mass up to this is rounding and counts as none
 
 
@@ -46,14 +49,14 @@ def _check(logits, dim, temperature):
     return dim % logits.dim()
 
 
-def _canonical(x, dim):
+def _canonical(x, dim, most=PLANE_CLASSES):
     """(tensor, outer, C, inner, ld, moved): x as `outer` images of C x `inner`, in place where its strides allow it.  More than
-    PLANE_CLASSES classes in front of other dimensions are moved to the end (a copy)."""
+    `most` classes in front of other dimensions are moved to the end (a copy), and more than PLANE_FEW of few positions."""
     shape = x.shape
     if dim == 1 and len(shape) == 2 and x.is_contiguous():            # the usual rows, for the sake of a short call
         return x, shape[0], shape[1], 1, shape[1], False
     C, outer, inner = shape[dim], math.prod(shape[:dim]), math.prod(shape[dim + 1:])
-    moved = inner > 1 and C > PLANE_CLASSES
+    moved = inner > 1 and C > (most if outer * inner >= PLANE_POSITIONS else PLANE_FEW)
     if moved:
         x, outer, inner = x.movedim(dim, -1), outer * inner, 1
     if x.is_contiguous():
@@ -70,7 +73,7 @@ def top_logits(logits, k, dim=1, temperature=1.0):
     +infinity).  float32, bfloat16 and float16 logits; values keep their type.  Not differentiable: a teacher's answer is data.
 
     The class dimension may stand anywhere: last (rows of any number of classes, read where they are) or in front of others as in
-    [N, C, H, W] (up to 32 classes read where they are, more are copied once into rows)."""
+    [N, C, H, W] (up to 32 classes, many positions of up to 256 if k <= 8, read where they are; others are copied once into rows)."""
     dim = _check(logits, dim, temperature)
     C = logits.shape[dim]
     if not 1 <= k <= min(MAX_K, C):
@@ -79,7 +82,7 @@ def top_logits(logits, k, dim=1, temperature=1.0):
     if not z.is_cuda or z.numel() == 0:
         return _host_top(z, k, dim, temperature)
     before, behind = z.shape[:dim], z.shape[dim + 1:]
-    z, outer, C, inner, ld, moved = _canonical(z.float() if z.dtype == torch.float16 else z, dim)
+    z, outer, C, inner, ld, moved = _canonical(z.float() if z.dtype == torch.float16 else z, dim, PLANE_CLASSES if k <= PLANE_TOP else PLANE_FEW)
     device, rest = z.device, before + behind
     kept = rest + (k,) if moved else before + (k,) + behind
     values = torch.empty(kept, dtype=z.dtype, device=device)

@@ -105,9 +105,9 @@ int segk_argmax_dice(const void* logits, int logits_dtype, const int64_t* labels
  * Distillation from a teacher's top logits.  No counterpart in the reference, whose networks learn from label maps only; stands
  * beside the losses above.  Logits are `outer` images (rows) of C classes x `inner` positions: element (o, c, i) at
  * logits[o*ld + c*inner + i], ld >= C*inner; inner = 1 gives rows [outer][C] with the classes innermost, C*inner = an NCHW image
- * otherwise (C <= 32 then).  fp32 or bf16, aligned to their type only.  Kept logits: `values` and `indices` [outer][k][inner],
- * contiguous, 1 <= k <= min(64, C); `lse` [outer][inner] fp32 = log(sum over the classes of exp(logit / temperature)).  Fewer than
- * 2^31 positions, 2^-40 <= temperature <= 2^40.
+ * otherwise (C <= 256 then; for the selection of more than 8, C <= 32).  fp32 or bf16, aligned to their type only.  Kept logits:
+ * `values` and `indices` [outer][k][inner], contiguous, 1 <= k <= min(64, C); `lse` [outer][inner] fp32 = log(sum over the classes of
+ * exp(logit / temperature)).  Fewer than 2^31 positions, 2^-40 <= temperature <= 2^40.
  * ---------------------------------------------------------------------------------------------- */
 
 /* The k greatest logits of every position in descending order (NaN counts as greatest; ties: the lower class first), the classes

@@ -118,7 +118,7 @@ def test_c_entry_points_refuse_bad_arguments_without_a_gpu():
     top_call = lambda **k: _lib.call("segk_top_logits", *{**dict(z=4096, dt=F32, o=4, c=80, i=1, ld=80, k=8, t=1.0, v=4096, x=4096, l=4096, d=0, s=None), **k}.values())  # noqa: E731
     for kw, text in ((dict(z=None), "null"), (dict(dt=7), "dtype"), (dict(o=0), "shape"), (dict(c=0), "shape"), (dict(c=1 << 30), "shape"), (dict(ld=79), "ld"),
                      (dict(k=0), "k must"), (dict(k=65), "k must"), (dict(k=9, c=8, ld=8), "k must"), (dict(t=0.0), "temperature"), (dict(t=math.inf), "temperature"),
-                     (dict(t=math.nan), "temperature"), (dict(z=4097), "aligned"), (dict(v=None), "null"), (dict(v=4100), "16-byte"), (dict(i=4, ld=320), "innermost"),
+                     (dict(t=math.nan), "temperature"), (dict(z=4097), "aligned"), (dict(v=None), "null"), (dict(v=4100), "16-byte"), (dict(i=4, ld=320, k=9), "innermost"), (dict(i=4, c=257, ld=1028), "innermost"),
                      (dict(o=1 << 20, i=1 << 12, c=4, ld=4 << 12), "positions"), (dict(t=1e-20), "temperature"),
                      (dict(t=1e20), "temperature")):
         with pytest.raises(_lib.SegkError, match=text):

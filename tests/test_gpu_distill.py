@@ -180,6 +180,86 @@ def test_planes(N, C, side, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N,C,side,k", [(2, 33, 5, 4), (1, 64, 9, 64), (3, 80, 7, 8), (1, 150, 12, 3), (2, 255, 6, 9), (1, 256, 17, 64), (1, 257, 4, 5), (4, 40, 32, 2)])
+def test_planes_of_many_classes(N, C, side, k, dtype, monkeypatch):
+    monkeypatch.setattr("segk.distill.PLANE_POSITIONS", 0)                # read in place, few as they are
+    test_planes(N, C, side, k, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_many_positions_of_many_classes(dtype):
+    """As many as are read in place, against the formulas on the host in 64 bits."""
+    g = torch.Generator().manual_seed(2)
+    z, t = torch.randn(1, 80, 130, 130, generator=g).to(dtype), (2 * torch.randn(1, 80, 130, 130, generator=g)).to(dtype)
+    got, host = top_logits(t.cuda(), 5, temperature=2.0), top_logits(t, 5, temperature=2.0)
+    assert torch.equal(got.values.cpu(), host.values) and torch.equal(got.indices.cpu(), host.indices)
+    x, y = z.cuda().requires_grad_(), z.double().requires_grad_()
+    a, b = distill_loss_topk(x, got, temperature=2.0), distill_loss_topk(y, TopLogits(host.values.double(), host.indices, got.lse.cpu().double()), temperature=2.0)
+    a.backward()
+    b.backward()
+    # as derived in distill_oracle.py, |logit| / T <= 5: u = 2^-21 (8 + 3 * 5); a position's loss T^2 u (3 + 10), its gradient T u (M q + p + 2 share)
+    u = 2.0 ** -21 * 23
+    assert abs(float(a.detach()) - float(b.detach())) <= 4 * u * 13 + 2.0 ** -23 * float(b.detach())
+    err = (x.grad.cpu().double() - y.grad).abs() * 130 * 130
+    assert bool((err <= 2 * u * 4 + (half_step(dtype) + 2.0 ** -21) * y.grad.abs() * 130 * 130).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("given", [True, False])
+@pytest.mark.parametrize("N,C,side,k", [(2, 4, 8, 3), (2, 32, 8, 6), (2, 33, 7, 5), (1, 150, 9, 12), (1, 256, 8, 64)])
+def test_planes_with_repeated_missing_and_masked_entries(N, C, side, k, given, dtype, monkeypatch):
+    monkeypatch.setattr("segk.distill.PLANE_POSITIONS", 0)
+    P = N * side * side
+    z, values, indices, lse = problem(P, C, k, seed=C, dtype=dtype)
+    g = torch.Generator().manual_seed(k)
+    indices[0::4, 1] = indices[0::4, 0]                                   # a class twice, with another value
+    indices[1::4] = torch.where(torch.rand(indices[1::4].shape, generator=g) < 0.5, C, indices[1::4].int()).int()     # entries that do not exist
+    indices[2::7] = -1                                                    # positions without entries
+    z[2::7] = math.nan
+    z[3::4, 0] = torch.finfo(dtype).min                                   # masked logits, where no teacher's mass is
+    gone = torch.arange(C).expand(P, C).clone()
+    for j in range(k):
+        gone.scatter_(1, indices[:, j:j + 1].long().clamp(0, C - 1), -1)
+    z = torch.where((gone[:, -1:] >= 0) & (torch.arange(P) % 5 == 0)[:, None] & (torch.arange(C) == C - 1), -math.inf, z.float()).to(dtype)
+    lse = lse + 0.1 if given else None                                    # repeated entries stay below 1 together, mostly
+    clean = torch.where(torch.isnan(z), torch.zeros((), dtype=dtype), z)
+    loss, grad, counted, lerr, gerr = loss_and_gradient(clean, values, indices, lse, 1.0)
+    planes = lambda t: t.view(N, side, side, -1).permute(0, 3, 1, 2).contiguous()  # noqa: E731
+    target = TopLogits(planes(values).cuda(), planes(indices).cuda(), None if lse is None else lse.view(N, side, side).cuda())
+    x = planes(z).cuda().requires_grad_()
+    got = distill_loss_topk(x, target, reduction="none")
+    got.sum().backward()
+    # Class 0 may be one with mass: (finfo.min - maximum) log2(e) is beyond fp32 then and the loss infinite, where 64 bits hold 10^38
+    huge, ok = loss > 2.0 ** 100, loss <= 2.0 ** 100
+    assert bool((got.detach().cpu().view(-1)[huge] > 2.0 ** 100).all())
+    assert bool(((got.detach().cpu().double().view(-1) - loss).abs() <= lerr + 2.0 ** -23 * loss.abs())[ok].all())
+    dx = x.grad.permute(0, 2, 3, 1).reshape(P, C).cpu().double()
+    assert bool(((dx - grad).abs() <= gerr + (half_step(dtype) + 2.0 ** -21) * grad.abs() + 2.0 ** -133)[ok].all()) and not dx[~counted].any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N,C,side", [(2, 33, 5), (1, 64, 9), (3, 150, 7), (1, 256, 12), (1, 257, 3)])
+def test_top_of_planes_of_many_classes(N, C, side, dtype, monkeypatch):
+    monkeypatch.setattr("segk.distill.PLANE_POSITIONS", 0)
+    g = torch.Generator().manual_seed(C)
+    z = torch.randint(-3, 4, (N, C, side, side), generator=g).to(dtype) / 2          # ties everywhere
+    z[0, C // 2, 0, 0] = z[0, C - 1, 0, 0] = math.nan
+    z[0, 3, 0, 1] = math.inf
+    z[0, :, 1, 1] = -math.inf
+    z[0, : C - 2, 1, 0] = -math.inf
+    for k in (1, 2, 3, 8, 9, 33):
+        for form in (lambda t: t, lambda t: torch.nn.functional.pad(t, (0, 3))[..., :side]):
+            got, host = top_logits(form(z.cuda()), k, temperature=2.0), top_logits(z, k, temperature=2.0)
+            assert torch.equal(got.indices.cpu(), host.indices)
+            same = got.values.cpu().eq(host.values) | (got.values.cpu().isnan() & host.values.isnan())
+            assert bool(same.all()) and got.values.dtype == dtype
+            want = torch.logsumexp(z.double() / 2, 1)
+            lse, fine = got.lse.cpu().double(), torch.isfinite(want)
+            assert bool(((lse - want).abs() <= 2.0 ** -21 * (8 + 3 * 1.5 / 2))[fine].all())
+            assert float(lse[0, 1, 1]) == -math.inf and math.isnan(float(lse[0, 0, 0])) and math.isnan(float(lse[0, 0, 1]))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("V", [5, 77, 1030, 9001])
 def test_strides_offsets_and_dimensions(V, dtype):
     z, values, indices, lse = problem(6, V, 3, seed=V, dtype=dtype)
