@@ -120,7 +120,7 @@ class _DistillFn(torch.autograd.Function):
         args = _DistillFn._launch(meta, z, values, indices, lse, None, MEAN if reduction == "mean" else 0, None if each else out, out if each else None, dz, ws)
         if want_grad:
             ctx.save_for_backward(z, values, indices, lse)
-            ctx.meta, ctx.dz, ctx.ws, ctx.args = meta, dz, ws, args
+            ctx.meta, ctx.dz, ctx.ws, ctx.args, ctx.stride = meta, dz, ws, args, z.stride()
         return out
 
     @staticmethod
@@ -148,18 +148,26 @@ class _DistillFn(torch.autograd.Function):
     @staticmethod
     def _gradients(ctx, g):
         z, values, indices, lse = ctx.saved_tensors
-        outer, C, inner, ld, moved, k, dim, T, weight, reduction, shape, in_dtype = ctx.meta
+        outer, C, inner, ld, moved, k, dim, T, weight, reduction, shape, in_dtype = meta = ctx.meta
         dz, ctx.dz, ws, ctx.ws = ctx.dz, None, ctx.ws, None      # handed over once; a second backward pass computes its own
         if g.dtype != torch.float32 or not g.is_contiguous():
             g = g.float().contiguous()
+        args = ctx.args
+        if z.data_ptr() != args[0] or z.stride() != ctx.stride:   # hooks on saved tensors brought back a copy, maybe in another layout
+            z, _, _, _, ld, _ = _canonical(z.reshape(outer, C, inner), 1, C)
+            meta = (outer, C, inner, ld) + meta[4:]
+            values, indices, lse = (t if t is None else t.contiguous() for t in (values, indices, lse))
+            args = None
         if dz is None:
-            dz = _DistillFn._gradient(ctx.meta, z)
+            dz = _DistillFn._gradient(meta, z)
             ws = torch.empty(query("segk_distill_workspace", outer, C, inner), dtype=torch.uint8, device=z.device)
-            _DistillFn._launch(ctx.meta, z, values, indices, lse, g, EACH if reduction == "none" else MEAN if reduction == "mean" else 0, None, None, dz, ws)
+            _DistillFn._launch(meta, z, values, indices, lse, g, EACH if reduction == "none" else MEAN if reduction == "mean" else 0, None, None, dz, ws)
+        elif args is None:
+            _DistillFn._launch(meta, z, values, indices, lse, g, SKIP | (MEAN if reduction == "mean" else 0), None, None, dz, ws)
         else:
             # the forward pass's arguments once more: this runs in autograd's thread, where every line costs several times its usual time
-            args = ctx.args
             args[14] |= SKIP
+            args[6], args[8], args[10] = values.data_ptr(), indices.data_ptr(), ops._p(lse)
             args[15], args[16], args[23] = g.data_ptr(), None, _env(z)[1]
             call("segk_distill", *args)
         if moved:

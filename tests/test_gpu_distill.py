@@ -320,6 +320,31 @@ def test_upstream_gradients_and_a_second_backward_pass(shape):
     torch.testing.assert_close(x.grad, g * w.unsqueeze(1), rtol=2.0 ** -20, atol=2 * 2 * 4 * 2.0 ** -24 * 2)
 
 
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+@pytest.mark.parametrize("classes_last", [True, False])
+def test_saved_tensors_that_come_back_as_copies(classes_last, reduction):
+    """Offloaded activations: the backward pass sees other memory, and contiguous where the logits were a padded view."""
+    g = torch.Generator().manual_seed(3)
+    shape = (6, 200) if classes_last else (2, 5, 12, 8)
+    z = torch.randn(shape, generator=g).cuda()
+    t = top_logits(2 * torch.randn(shape, generator=g).cuda(), 3)
+
+    def gradient(offload):
+        leaf = z.clone().requires_grad_()
+        view = torch.nn.functional.pad(leaf, (1, 2))[..., 1:-2] * 1.5 if classes_last else torch.nn.functional.pad(leaf, (0, 0, 0, 0, 0, 3))[:, :5]
+        view = torch.nn.functional.pad(view, (0, 4))[..., :shape[-1]] if classes_last else view
+        with torch.autograd.graph.save_on_cpu() if offload else torch.enable_grad():
+            loss = distill_loss_topk(view, t, reduction=reduction)
+        del view
+        junk = [torch.full(shape, 1e30, device="cuda") for _ in range(4)]          # takes the freed memory
+        first, = torch.autograd.grad(loss.sum() * 2.0, leaf, retain_graph=True)
+        second, = torch.autograd.grad(loss.sum(), leaf)
+        assert len(junk) == 4
+        return first, second
+    for a, b in zip(gradient(True), gradient(False)):
+        assert torch.equal(a, b) and a.any()
+
+
 def test_a_second_differentiation_is_refused():
     z, values, indices, lse = problem(4, 50, 3)
     x = z.cuda().requires_grad_()
