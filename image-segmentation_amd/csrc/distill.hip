@@ -10,6 +10,11 @@
 // All sums run over exp2((s - max) log2(e) / T) in fp32, the difference first: a mask of the type's lowest value times log2(e) would
 // overflow.  The classes outside the kept ones have a maximum and a sum of their own
 // (K_out, S_out): R and q_c / R then never come out of a difference of two almost equal sums, and cannot underflow.
+//
+// The loss is summed as  sum D(P_c, q_c) + D(r, R),  D(p, q) = p log(p / q) - p + q,  over the kept classes: the probabilities on either
+// side sum to 1, so what D adds cancels.  D has no negative value and is taken from q - p where the two are alike.  The terms
+// p log(p / q) themselves are of the order 1 / T and cancel to 1 / T^2 at high temperatures (1000 classes, 8 kept, worst of 64 rows:
+// 3e-3 of the loss lost at T = 20, 0.8 at T = 256).
 #include "common.h"
 
 namespace segk {
@@ -81,7 +86,7 @@ template <typename I> __device__ __forceinline__ int load_class_as(const Distill
 // loss of a row; -0 says that it has no entry, where the final sum counts them, and no other row has that value
 __device__ __forceinline__ float loss_of_empty(const DistillArgs& a) { return a.count_losses ? -0.f : 0.f; }
 __device__ __forceinline__ float loss_of_row(const DistillArgs& a, float l) {
-    l *= kLn2 * a.T * a.T * a.weight;
+    l *= a.T * a.T * a.weight;
     return l == 0.f ? 0.f : l;
 }
 __device__ __forceinline__ float load_kept(const DistillArgs& a, int64_t at) {
@@ -164,6 +169,31 @@ __device__ __forceinline__ float grad_scale(const DistillArgs& a, int64_t positi
 __device__ __forceinline__ float exp_over(float z, float base, float c) { return fast_exp2((z - base) * c); }
 // the same for a maximum that may be "no element" (-inf), whatever the base
 __device__ __forceinline__ float rebase(float k, float base, float c) { return k == -INFINITY ? 0.f : exp_over(k, base, c); }
+
+// p ln(p / q) - p + q = p (y - 1 - ln y), y = q / p; log_ratio(): the logarithm (base 2) of p / q, used where y leaves the range.  Near 1, y - 1
+// is exact and the logarithm good to one unit of its own last place (all y in [1/2, 2]), so y - 1 - ln y is off by at most 2^-22 |y - 1|, as if y were
+// off by 2^-22; what that leaves below 0 is 0.
+template <typename F> __device__ __forceinline__ float divergence(float p, float q, F&& log_ratio) {
+    const float y = q * __builtin_amdgcn_rcpf(p);
+    if (y > 0x1p-100f && y < 0x1p100f) {
+        const float h = fmaf(-kLn2, __builtin_amdgcn_logf(y), y - 1.f);
+        return p * (h < 0.f ? 0.f : h);
+    }
+    return p == 0.f ? q : (q - p) + p * (log_ratio() * kLn2);
+}
+// What an entry adds to its row's loss.  p, lp: its own probability and logarithm; total: that of all entries with its class, for which
+// the first of them stands.
+__device__ __forceinline__ float entry_loss(bool first, float p, float lp, float total, float q, float lq) {
+    float l = first ? divergence(total, q, [&] { return (total == p ? lp : log2f(total)) - lq; }) : 0.f;
+    if (total != p && p != 0.f) l += p * ((lp - log2f(total)) * kLn2);
+    return l;
+}
+// The same for everything outside the kept classes (R: the student's probability there, lr its logarithm).  Where the teacher has no rest
+// there, what D added does not cancel: mass - 1 + R is left (a row whose entries have no probability at all counts as 0).
+__device__ __forceinline__ float rest_loss(const DistillArgs& a, float l, float rest, float mass, float R, float lr) {
+    if (rest > 0.f) return l + divergence(rest, R, [&] { return log2f(rest) - lr; });
+    return mass == 0.f ? 0.f : l + (a.tlse ? mass - 1.f : 0.f) + R;
+}
 
 // ------------------------------------------------------------------------------------------------ rows in registers
 // A row is read in 16-byte pieces that are aligned in memory; the row may begin and end inside a piece.
@@ -311,6 +341,7 @@ struct Kept {
     float total;             // p of all entries with this class
     float rest, mass;        // of the row: what the teacher gave to the other classes; sum of p and rest
     float top, sum;          // of the row: the student's maximum over the kept classes and the sum of exp over it
+    bool first;              // the first entry with this class
 };
 template <typename T>
 __device__ __forceinline__ Kept kept_entries(const DistillArgs& a, int64_t row, const T* __restrict__ z, int cls, int lane, float c) {
@@ -365,6 +396,7 @@ __device__ __forceinline__ Kept kept_entries(const DistillArgs& a, int64_t row, 
             if (j < lane) first = false;
         }
     }
+    e.first = first;
     const int distinct = __popcll(__ballot(first));
     e.rest = a.tlse ? 1.f - mass : 0.f;
     if (!(e.rest > kRestFloor) || distinct == a.V) e.rest = 0.f;
@@ -382,13 +414,11 @@ __device__ __forceinline__ Joined join(float ko, float so, float km, float sm, f
     w.sum = so * w.share + sm * rebase(km, w.top, c) + (so != so ? so : 0.f);      // a NaN among the logits reaches the row
     return w;
 }
-// the row's loss in units of ln 2 T^2, for a whole wave
-__device__ __forceinline__ float kept_loss(const Kept& e, const Joined& w, float ko, float so, float c) {
-    const float ls = log2f(w.sum);
-    float l = e.p == 0.f ? 0.f : e.p * (e.lp - ((e.z - w.top) * c - ls));
-    l = sum_wave(l);
-    if (e.rest > 0.f) l += e.rest * (log2f(e.rest) - (log2f(so) + (ko - w.top) * c - ls));
-    return l;
+// the row's loss in units of T^2, for a whole wave
+__device__ __forceinline__ float kept_loss(const DistillArgs& a, const Kept& e, const Joined& w, float ko, float so, float c) {
+    const float ls = log2f(w.sum), inv = __builtin_amdgcn_rcpf(w.sum), q = exp_over(e.z, w.top, c) * inv;
+    const float l = sum_wave(entry_loss(e.first, e.p, e.lp, e.total, q, (e.z - w.top) * c - ls));
+    return rest_loss(a, l, e.rest, e.mass, so * w.share * inv, log2f(so) + (ko - w.top) * c - ls);
 }
 // the gradient of a class outside is this times exp of its logit over ko
 __device__ __forceinline__ float outside_factor(const Joined& w, float so, float rest, float mass, float gs) {
@@ -501,7 +531,7 @@ __global__ __launch_bounds__(NT) void distill_rows_kernel(const DistillArgs a) {
     for (int w = 0; w < NW; ++w) so += sh_k[w] == -INFINITY ? sh_s[w] : sh_s[w] * exp_over(sh_k[w], ko, c);
     const Joined w = join(ko, so, sh_x[0], sh_x[1], c);
     if (wave == 0) {
-        const float l = kept_loss(e, w, ko, so, c);
+        const float l = kept_loss(a, e, w, ko, so, c);
         if (lane == 0) a.row_loss[row] = loss_of_row(a, l);
     }
     if constexpr (GRAD) {
@@ -655,7 +685,7 @@ __global__ __launch_bounds__(64) void distill_join_kernel(const DistillArgs a, c
     const float ko = wave_max(k), so = sum_wave(k == -INFINITY ? s : s * exp_over(k, ko, c));
     const Kept e = kept_entries<T>(a, row, z, cls, lane, c);
     const Joined w = join(ko, so, e.top, e.sum, c);
-    const float l = kept_loss(e, w, ko, so, c);
+    const float l = kept_loss(a, e, w, ko, so, c);
     if (joined) {
         const float gs = grad_scale(a, row);
         float* out = joined + row * kRowFloats;
@@ -743,7 +773,8 @@ __global__ __launch_bounds__(256) void distill_pixels_kernel(const DistillArgs a
                 for (int v = 0; v < VP; ++v) x[q][v] = -INFINITY;
             }
         }
-        float e[CM][VP], top[VP], sum[VP], plogp[VP], lse[VP];
+        float e[CM][VP], top[VP], sum[VP], lse[VP];
+        bool twice[VP];                       // two entries have the same class
         uint32_t kept[VP];
         if constexpr (VP == 4) {
             if (a.tlse) Elem<float>::load4(a.tlse + o * a.inner + i0, lse);
@@ -751,8 +782,9 @@ __global__ __launch_bounds__(256) void distill_pixels_kernel(const DistillArgs a
 #pragma unroll
         for (int v = 0; v < VP; ++v) {
             top[v] = -INFINITY;
-            sum[v] = plogp[v] = 0.f;
+            sum[v] = 0.f;
             kept[v] = 0;
+            twice[v] = false;
 #pragma unroll
             for (int q = 0; q < CM; ++q) e[q][v] = 0.f;
         }
@@ -766,6 +798,9 @@ __global__ __launch_bounds__(256) void distill_pixels_kernel(const DistillArgs a
 #pragma unroll
                 for (int v = 0; v < VP; ++v) top[v] = cj[v] >= 0 ? fmaxf(top[v], t[v]) : top[v];
             }
+        auto log_p = [&](float t, int v) {    // base 2, before it is normalised where no logsumexp is given
+            return a.tlse ? fmaf(t, a.invT, -lse[v]) * kLog2e : (top[v] == -INFINITY ? -INFINITY : (t - top[v]) * c);
+        };
         for (int j = 0; j < a.k; ++j) {
             int cj[VP];
             float t[VP];
@@ -773,11 +808,11 @@ __global__ __launch_bounds__(256) void distill_pixels_kernel(const DistillArgs a
             load_kepts<VP>(a, at + j * a.ts_c, t);
 #pragma unroll
             for (int v = 0; v < VP; ++v) {
-                const float lp = a.tlse ? fmaf(t[v], a.invT, -lse[v]) * kLog2e : (top[v] == -INFINITY ? -INFINITY : (t[v] - top[v]) * c);
-                const float ej = cj[v] >= 0 ? fast_exp2(lp) : 0.f;
-                kept[v] |= cj[v] >= 0 ? 1u << cj[v] : 0u;
+                const float ej = cj[v] >= 0 ? fast_exp2(log_p(t[v], v)) : 0.f;
+                const uint32_t bit = cj[v] >= 0 ? 1u << cj[v] : 0u;
+                twice[v] = twice[v] || (kept[v] & bit);
+                kept[v] |= bit;
                 sum[v] += ej;
-                plogp[v] += ej == 0.f ? 0.f : ej * lp;
 #pragma unroll
                 for (int q = 0; q < CM; ++q) e[q][v] += q == cj[v] ? ej : 0.f;
             }
@@ -788,16 +823,15 @@ __global__ __launch_bounds__(256) void distill_pixels_kernel(const DistillArgs a
             float l = 0.f, g = gs;
             if constexpr (GRAD)
                 if (a.up_each) g = a.weight * a.T * a.upstream[pos];       // no mean goes with one gradient for each position
-            float mass = sum[v], rest = 0.f;
+            float mass = sum[v], rest = 0.f, norm = 1.f;
             if (a.tlse) {
                 rest = 1.f - mass;
                 if (!(rest > kRestFloor) || __popc(kept[v]) == a.V) rest = 0.f;
             } else {
-                const float inv = sum[v] == 0.f ? 0.f : 1.f / sum[v];
+                norm = sum[v] == 0.f ? 0.f : 1.f / sum[v];
 #pragma unroll
-                for (int q = 0; q < CM; ++q) e[q][v] *= inv;
-                plogp[v] = sum[v] == 0.f ? 0.f : plogp[v] * inv - log2f(sum[v]);
-                mass = sum[v] * inv;
+                for (int q = 0; q < CM; ++q) e[q][v] *= norm;
+                mass = sum[v] * norm;
             }
             const float all = mass + rest;
             float zo = -INFINITY, zm = -INFINITY;
@@ -819,18 +853,40 @@ __global__ __launch_bounds__(256) void distill_pixels_kernel(const DistillArgs a
             }
             const float fo = rebase(ko, kk, c), fm = rebase(km, kk, c);
             const float s = so * fo + sm * fm + (so != so ? so : 0.f);
+            const float inv = 1.f / s;
             if (kept[v]) {
                 const float ls = log2f(s);
-                l = plogp[v];
+                if (!twice[v]) {
 #pragma unroll
-                for (int q = 0; q < CM; ++q) l -= e[q][v] == 0.f ? 0.f : e[q][v] * ((x[q][v] - kk) * c - ls);
-                if (rest > 0.f) l += rest * (log2f(rest) - (log2f(so) + (ko - kk) * c - ls));
-                l *= kLn2 * a.T * a.T * a.weight;
+                    for (int q = 0; q < CM; ++q)
+                        if (q < a.V) {
+                            const bool in = (kept[v] >> q) & 1u;
+                            if (CM > 8 && !in) continue;      // neighbours often share their classes; of few, D(1, 1) = 0 costs less than a branch
+                            const float p = in ? e[q][v] : 1.f;
+                            l += divergence(p, in ? w[q] * (fm * inv) : 1.f, [&] { return log2f(p) - ((x[q][v] - kk) * c - ls); });
+                        }
+                } else {                                      // two entries share a class: entry by entry
+                    uint32_t seen = 0;
+                    for (int j = 0; j < a.k; ++j) {
+                        const int cls = load_class(a, at + v + j * a.ts_c);
+                        if (cls < 0) continue;
+                        float z = x[0][v], total = e[0][v];
+#pragma unroll
+                        for (int q = 1; q < CM; ++q) {
+                            z = q == cls ? x[q][v] : z;
+                            total = q == cls ? e[q][v] : total;
+                        }
+                        const float lp = log_p(load_kept(a, at + v + j * a.ts_c), v);
+                        l += entry_loss(!(seen >> cls & 1u), fast_exp2(lp) * norm, a.tlse ? lp : lp - log2f(sum[v]), total, exp_over(z, kk, c) * inv, (z - kk) * c - ls);
+                        seen |= 1u << cls;
+                    }
+                }
+                l = rest_loss(a, l, rest, mass, so * fo * inv, log2f(so) + (ko - kk) * c - ls);
+                l *= a.T * a.T * a.weight;
             }
             if (a.row_loss) a.row_loss[pos] = l;
             block += l;
             if constexpr (GRAD) {
-                const float inv = 1.f / s;
                 const float fk = g * all * fm * inv, fr = g * (all * fo * inv - (rest > 0.f ? rest / so : 0.f));
 #pragma unroll
                 for (int q = 0; q < CM; ++q)
@@ -899,13 +955,11 @@ __global__ __launch_bounds__(256) void distill_planes_kernel(const DistillArgs a
         };
         uint32_t kept[kPlaneClasses / 32] = {};
         bool twice = false;
-        float mass = 0.f, plogp = 0.f, km = -INFINITY, sm = 0.f;
+        float mass = 0.f, km = -INFINITY, sm = 0.f;
         for (int j = 0; j < a.k; ++j) {
             const int cls = load_class(a, at + j * a.inner);
             if (cls < 0) continue;
-            const float lp = log_p(j), p = fast_exp2(lp);
-            mass += p;
-            plogp += p == 0.f ? 0.f : p * lp;
+            mass += fast_exp2(log_p(j));
             bool seen = false;
 #pragma unroll
             for (int w = 0; w < kPlaneClasses / 32; ++w) {
@@ -941,28 +995,38 @@ __global__ __launch_bounds__(256) void distill_planes_kernel(const DistillArgs a
 #pragma unroll
                 for (int u = 0; u < 8; ++u) so += exp_over(x[u], base, c);
             });
-        float rest = 0.f, norm = 1.f;
+        float rest = 0.f, norm = 1.f, log_norm = 0.f;
         if (a.tlse) {
             rest = 1.f - mass;
             if (!(rest > kRestFloor) || distinct == a.V) rest = 0.f;
         } else {
             norm = mass == 0.f ? 0.f : 1.f / mass;
-            plogp = mass == 0.f ? 0.f : plogp * norm - log2f(mass);
+            log_norm = log2f(mass);
             mass *= norm;
         }
         const float all = mass + rest;
         const float kk = fmaxf(ko, km), bo = ko == -INFINITY ? 0.f : ko, bm = km == -INFINITY ? 0.f : km;
         const float fo = rebase(ko, kk, c), fm = rebase(km, kk, c), s = so * fo + sm * fm + (so != so ? so : 0.f);
         if (distinct) {
-            const float ls = log2f(s);
-            l = plogp;
+            const float ls = log2f(s), inv = 1.f / s;
             for (int j = 0; j < a.k; ++j) {
                 const int cls = load_class(a, at + j * a.inner);
-                const float p = cls >= 0 ? fast_exp2(log_p(j)) * norm : 0.f;
-                if (cls >= 0 && p != 0.f) l -= p * ((logit(cls) - kk) * c - ls);
+                if (cls < 0) continue;
+                const float lp = log_p(j), p = fast_exp2(lp), zj = logit(cls);
+                float total = p;
+                bool first = true;
+                if (twice) {
+                    total = 0.f;
+                    for (int h = 0; h < a.k; ++h)
+                        if (load_class(a, at + h * a.inner) == cls) {
+                            total += fast_exp2(log_p(h));
+                            first = first && h >= j;
+                        }
+                }
+                l += entry_loss(first, p * norm, lp - log_norm, total * norm, exp_over(zj, kk, c) * inv, (zj - kk) * c - ls);
             }
-            if (rest > 0.f) l += rest * (log2f(rest) - (log2f(so) + (ko - kk) * c - ls));
-            l *= kLn2 * a.T * a.T * a.weight;
+            l = rest_loss(a, l, rest, mass, so * fo * inv, log2f(so) + (ko - kk) * c - ls);
+            l *= a.T * a.T * a.weight;
         }
         if (a.row_loss) a.row_loss[pos] = l;
         if constexpr (GRAD) {

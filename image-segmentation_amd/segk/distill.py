@@ -190,8 +190,11 @@ def distill_loss_topk(pred, target, temperature=1.0, reduction="mean", dim=1, we
     `weight` scales loss and gradient; it costs nothing, where multiplying the returned loss costs another pass over the logits.
 
     pred: float32, bfloat16 or float16, any strides; target: TopLogits or a tuple (values, indices[, lse]) with float32 / bfloat16 /
-    float16 values and int32 / int64 indices.  Returns float32; the gradient has pred's type.  Sums run in float32;
-    log p carries the rounding of the kept lse, 2^-24 |lse|, so logits / T of some thousands leave no exact probabilities."""
+    float16 values and int32 / int64 indices.  Returns float32; the gradient has pred's type.  Sums run in float32 (in float64 on the
+    CPU).  log p carries the rounding of the kept lse, 2^-24 |lse|, so logits / T of some thousands leave no exact probabilities.
+    Student and teacher differ by d / T in log q where their logits differ by d, and that is known to about 2^-22: loss and
+    gradient are good to about T 2^-22 / d of themselves.  Where every class is kept with an lse, the rounding of the lse adds up to
+    T^2 2^-22 (1 + |lse|): leave the lse away there."""
     dim = _check(pred, dim, temperature)
     if reduction not in ("mean", "sum", "none"):
         raise ValueError('Reduction parameter unknown.')
@@ -243,7 +246,8 @@ def _host_top(z, k, dim, temperature):
 
 
 def _host_distill(pred, values, indices, lse, dim, T, weight, reduction):
-    z = (pred if pred.dtype == torch.float64 else pred.float()).movedim(dim, -1) / T
+    # in 64 bits: the terms of a row cancel to 1 / T of themselves, and a temperature costs nothing that way
+    z = pred.double().movedim(dim, -1) / T
     t = values.movedim(dim, -1).to(z.dtype) / T
     at = indices.movedim(dim, -1).to(torch.int64)
     valid = (at >= 0) & (at < z.shape[-1])
@@ -273,4 +277,5 @@ def _host_distill(pred, values, indices, lse, dim, T, weight, reduction):
     if reduction == "none":
         return row.to(torch.float32 if pred.dtype != torch.float64 else torch.float64)
     total = row.sum()
-    return total / counted.sum().clamp(min=1) if reduction == "mean" else total
+    total = total / counted.sum().clamp(min=1) if reduction == "mean" else total
+    return total.to(torch.float32 if pred.dtype != torch.float64 else torch.float64)

@@ -122,7 +122,9 @@ int segk_top_logits(const void* logits, int dtype, int64_t outer, int64_t C, int
  *   teacher_lse given:  p_j = exp(value_j / T - teacher_lse), r = 1 - sum p (counted as 0 up to 2^-20, and where every class was
  *                       kept), R = sum of q over the classes that were not kept
  * An entry whose index lies outside [0, C) does not exist; the p of entries with the same index add up; a position without any
- * entry has loss 0 and gradient 0 and its logits are not read.  All losses and gradients are times `weight`.
+ * entry has loss 0 and gradient 0 and its logits are not read.  All losses and gradients are times `weight`.  Where logits of student
+ * and teacher differ by d, both are good to about temperature * 2^-22 / d of themselves; where every class was kept and a teacher_lse
+ * is given, its rounding adds up to temperature^2 * 2^-22 * (1 + |teacher_lse|).
  *   loss          (optional) fp32: sum over the positions; flags bit0: their mean over the positions with an entry (0 if none)
  *   position_loss (optional) fp32 [outer][inner]
  *   dlogits       (optional) gradient of `loss` times *upstream (1 if NULL); element (o, c, i) at o*ld_d + c*inner + i, dtype of

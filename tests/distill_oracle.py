@@ -70,3 +70,40 @@ def top(z, k):
 
 def half_step(dtype):
     return torch.finfo(dtype).eps / 2
+
+
+def cancellation_bounds(z, values, indices, lse, T):
+    """Error bounds of an fp32 evaluation that lets nothing cancel, of the loss [P] and of the gradient [P, V] before it is rounded to its
+    type, for positions without repeated entries.
+
+    Every probability is known to E = 2^-24 (12 B + n + 16), relative, B = max(|z|, |t|) / T + |lse|: 1 / T, the difference of two
+    logits, log2(e) / T and the products round the argument of exp2 (four roundings of at most 2 B; three of |t| / T + |lse| for the teacher), exp2,
+    quotients and reciprocals are good to 2^-23, and a sum has at most n = min(V, 128) additions one after the other, or 256 of
+    planes with more.  The loss is sum D(p, q) + D(r, R), D = p log(p / q) - p + q: dD/dp = log(p / q), dD/dq = 1 - p / q, and r = 1 - sum p is off by
+    E of 1.  Where r counts as 0, R (renormalised) and mass - 1 (a given lse) are added as they are."""
+    z, values = z.double(), values.double()
+    loss, grad, counted, _, _ = loss_and_gradient(z, values, indices, lse, T)
+    lerr, gerr = torch.zeros_like(loss), torch.zeros_like(grad)
+    V = z.shape[1]
+    for i in torch.nonzero(counted).flatten().tolist():
+        valid = (indices[i] >= 0) & (indices[i] < V)
+        at, t = indices[i][valid].long(), values[i][valid] / T
+        assert at.unique().numel() == at.numel()
+        logq = torch.log_softmax(z[i] / T, 0)
+        logp = torch.log_softmax(t, 0) if lse is None else t - lse[i].double()
+        E = 2.0 ** -24 * (12 * (max(float(z[i].abs().max()) / T, float(t.abs().max())) + (0.0 if lse is None else abs(float(lse[i])))) + (256 if V > 128 else V) + 16)
+        p, q = logp.exp(), logq.exp()
+        parts = float((p * (logp - logq[at]).abs() + (q[at] - p).abs()).sum())
+        outside = torch.ones(V, dtype=torch.bool)
+        outside[at] = False
+        R, r = float(q[outside].sum()), 0.0 if lse is None else 1.0 - float(p.sum())
+        ge = q.clone()
+        ge[at] += p
+        if r > 2.0 ** -20 and R > 0:
+            parts += abs(math.log(r / R)) + abs(R - r)
+            ge[outside] += q[outside] * (r + 1) / R
+        else:
+            parts += R + (0.0 if lse is None else 1.0)
+        lerr[i] = T * T * E * parts + 2.0 ** -21 * abs(float(loss[i]))
+        gerr[i] = T * E * ge + 2.0 ** -126
+    return lerr, gerr

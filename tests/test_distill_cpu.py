@@ -162,3 +162,18 @@ def test_training_loop_takes_the_loss_and_its_targets():
         return seen[-1]
     avg = train(loader, net, [loss], 0, 1, torch.device("cpu"), 2)
     assert len(seen) == 2 and abs(avg - sum(float(s) for s in seen) / 2) < 1e-6 and not torch.equal(before, net.weight)
+
+
+@pytest.mark.parametrize("T", [8.0, 20.0, 64.0, 256.0, 4096.0])
+@pytest.mark.parametrize("rest", [False, True])
+def test_host_loss_at_high_temperatures(T, rest):
+    """The terms of a row are of the order 1 / T and cancel to 1 / T^2: in fp32 nothing of the loss would be left."""
+    z, target = problem(32, 300, 8, seed=2, T=T)
+    target = target if rest else target._replace(lse=None)
+    loss, grad, _, _, _ = loss_and_gradient(z, *target, T)
+    x = z.clone().requires_grad_()
+    got = distill_loss_topk(x, target, temperature=T, reduction="none")
+    # 64-bit terms, log q of up to 8, times T^2, on both sides; one rounding to fp32
+    assert got.dtype == torch.float32 and bool(((got.double() - loss).abs() <= 2.0 ** -24 * loss.abs() + T * T * 2.0 ** -47).all())
+    got.sum().backward()
+    assert bool(((x.grad.double() - grad).abs() <= 2.0 ** -24 * grad.abs() + T * 2.0 ** -47).all())

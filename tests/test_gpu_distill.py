@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from distill_oracle import half_step, loss_and_gradient, top
+from distill_oracle import cancellation_bounds, half_step, loss_and_gradient, top
 from loss.distill import TopLogits, distill_loss_topk, top_logits
 
 pytestmark = pytest.mark.gpu
@@ -630,3 +630,46 @@ def test_far_rows_of_a_large_tensor():
     y = z[-3:].detach().clone().requires_grad_()
     w, = torch.autograd.grad(distill_loss_topk(y, TopLogits(*(t[-3:] for t in keep))), y)
     assert torch.equal(g[-3:], w) and not g[:4].any() and not g[-4].any()
+
+
+@pytest.mark.parametrize("T", [1.0, 8.0, 20.0, 64.0, 256.0])
+@pytest.mark.parametrize("shape,k", [((40, 1000), 8), ((64, 80), 8), ((4700, 9), 3), ((16, 6), 2), ((16, 6), 6), ((2, 70000), 5),
+                                     ((2, 4, 8, 12), 2), ((1, 5, 7, 9), 3), ((1, 21, 8, 8), 4), ((1, 21, 8, 8), 21), ((2, 80, 128, 64), 3)])
+def test_high_temperatures(shape, k, T):
+    """The loss where its terms cancel: rows of a wave, of a thread and shared by workgroups, class planes of each kind; a given logsumexp,
+    one at which nothing is left outside, and renormalised."""
+    C = shape[1]
+    P = math.prod(shape) // C
+    n = min(P, 64)
+    z, values, indices, lse = problem(n, C, k, seed=C + k, T=T)
+    again = -(-P // n)
+
+    def planes(x):                                               # the positions of [P, c] as [N, c, H, W]
+        x = x.repeat((again,) + (1,) * (x.dim() - 1))[:P]
+        if len(shape) == 2:
+            return x.cuda()
+        rest = (shape[0],) + shape[2:]
+        return x.reshape(rest).cuda() if x.dim() == 1 else x.reshape(rest + (-1,)).movedim(-1, 1).contiguous().cuda()
+
+    def back(x):
+        return (x if len(shape) == 2 else x.reshape(-1) if x.dim() == len(shape) - 1 else x.movedim(1, -1).reshape(P, -1)).detach().cpu().double()[:n]
+    for given in (lse, None):
+        loss, grad, _, _, _ = loss_and_gradient(z, values, indices, given, T)
+        lerr, gerr = cancellation_bounds(z, values, indices, given, T)
+        x = planes(z).requires_grad_()
+        target = TopLogits(planes(values), planes(indices), None if given is None else planes(given))
+        got = distill_loss_topk(x, target, temperature=T, reduction="none")
+        err = (back(got) - loss).abs()
+        assert bool((err <= lerr).all()), (float((err / loss).max()), float((lerr / loss).max()))
+        if given is None or k < C:                               # both sides add up to 1: no term is negative
+            assert float(got.detach().min()) >= 0
+        plain = distill_loss_topk(x.detach(), target, temperature=T, reduction="sum")
+        x2 = x.detach().requires_grad_()
+        total = distill_loss_topk(x2, target, temperature=T, reduction="sum")
+        every = got.detach().double().sum().cpu()
+        for s in (plain, total.detach()):
+            assert abs(float(s) - float(every)) <= 2.0 ** -20 * float(got.detach().abs().double().sum())
+        got.sum().backward()
+        total.backward()
+        for g in (x.grad, x2.grad):
+            assert bool(((back(g) - grad).abs() <= gerr + 2.0 ** -24 * grad.abs()).all())
