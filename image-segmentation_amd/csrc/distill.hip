@@ -1698,6 +1698,14 @@ static Pixels pixels(int64_t outer, int64_t C, int64_t inner, int64_t ld, int64_
 // 4.1/5.1, 9.9/9.5, of 32 9.3/5.1, 18.0/9.4.
 static bool few(int64_t outer, int64_t C, int64_t inner) { return C <= kPixelClasses && (inner > 1 || C <= 8 || outer >= 512 * C); }
 
+// f(first, n) for all units (rows, images) of so many threads each: a launch has to have fewer than 2^32 threads
+template <typename F> static void by_launches(int64_t units, int64_t threads, F&& f) {
+    const int64_t fit = (1ll << 31) / threads, most = fit < 1 ? 1 : fit;      // a single unit has at most 2^31 + 255 threads
+    for (int64_t u = 0; u < units; u += most) f(u, units - u < most ? units - u : most);
+}
+template <typename T> static T* advance(T* p, int64_t elements) { return p ? p + elements : p; }
+static const void* advance(const void* p, int64_t elements, size_t size) { return static_cast<const char*>(p) + elements * (int64_t)size; }
+
 static bool planes(int64_t C, int64_t inner) { return inner > 1 && C > kPixelClasses; }
 
 template <typename F> static void class_tier(int64_t C, int vp, F&& f) {
@@ -1722,20 +1730,29 @@ extern "C" int segk_top_logits(const void* logits, int dtype, int64_t outer, int
     SEGK_USE_DEVICE(dev);
     hipStream_t st = (hipStream_t)stream;
     SEGK_DISPATCH_DTYPE(dtype, T, {
-        if (wide) {
-            auto kernel = k <= 2 ? top_planes_kernel<T, 2> : top_planes_kernel<T, kPlaneTop>;
-            hipLaunchKernelGGL(kernel, dim3((unsigned)px.blocks), dim3(256), 0, st, (const T*)logits, ld, px.inner, (int)C, (int)k, 1.f / temperature, (T*)values,
-                               indices, lse, px.blocks_each);
-        } else if (pix) {
-            class_tier(C, px.vp, [&](auto cm, auto vp) {
-                hipLaunchKernelGGL((top_pixels_kernel<T, cm(), vp()>), dim3((unsigned)px.blocks), dim3(256), 0, st, (const T*)logits, ld, px.s_c,
-                                   px.s_p, px.inner, (int)C, (int)k, 1.f / temperature, (T*)values, indices, px.ts_c, px.ts_p, lse, px.blocks_each);
+        const float inv_t = 1.f / temperature;
+        if (pix) {
+            by_launches(px.outer, px.blocks_each * 256ll, [&](int64_t o, int64_t n) {
+                const dim3 grid((unsigned)(n * px.blocks_each));
+                const int64_t kept = o * k * px.inner;
+                if (wide) {
+                    auto kernel = k <= 2 ? top_planes_kernel<T, 2> : top_planes_kernel<T, kPlaneTop>;
+                    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, (const T*)logits + o * ld, ld, px.inner, (int)C, (int)k, inv_t, (T*)values + kept,
+                                       indices + kept, advance(lse, o * px.inner), px.blocks_each);
+                } else {
+                    class_tier(C, px.vp, [&](auto cm, auto vp) {
+                        hipLaunchKernelGGL((top_pixels_kernel<T, cm(), vp()>), grid, dim3(256), 0, st, (const T*)logits + o * ld, ld, px.s_c, px.s_p, px.inner, (int)C,
+                                           (int)k, inv_t, (T*)values + kept, indices + kept, px.ts_c, px.ts_p, advance(lse, o * px.inner), px.blocks_each);
+                    });
+                }
             });
         } else {
             row_tier<T, true>(logits, ld, C, k, [&](auto nt, auto nch) {
                 constexpr int r = rows_per_group(nt(), nch());
-                hipLaunchKernelGGL((top_rows_kernel<T, nt(), nch()>), dim3((unsigned)((outer + r - 1) / r)), dim3(nt(), r), 0, st, (const T*)logits, outer, ld, (int)C, (int)k,
-                                   1.f / temperature, (T*)values, indices, lse);
+                by_launches(outer, nt(), [&](int64_t o, int64_t n) {
+                    hipLaunchKernelGGL((top_rows_kernel<T, nt(), nch()>), dim3((unsigned)((n + r - 1) / r)), dim3(nt(), r), 0, st, (const T*)logits + o * ld, n, ld, (int)C,
+                                       (int)k, inv_t, (T*)values + o * k, indices + o * k, advance(lse, o));
+                });
             });
         }
     });
@@ -1822,16 +1839,36 @@ extern "C" int segk_distill(const void* logits, int dtype, int64_t outer, int64_
         }
         SEGK_LAUNCH_CHECK();
     }
+    // the arguments from image or row o on (rows counted in place need no second launch)
+    auto from = [&](int64_t o) {
+        DistillArgs b = a;
+        const int64_t positions = o * a.inner;
+        b.z = advance(a.z, o * ld, esize(dtype));
+        b.t = advance(a.t, positions * k, esize(values_dtype));
+        b.idx = advance(a.idx, positions * k, (size_t)index_bytes);
+        b.tlse = advance(a.tlse, positions);
+        if (each) b.upstream = advance(a.upstream, positions);
+        b.row_loss = advance(a.row_loss, positions);
+        b.partial = advance(a.partial, o * px.blocks_each);
+        if (dlogits) b.dz = const_cast<void*>(advance(a.dz, o * ld_d, esize(dtype)));
+        return b;
+    };
     int64_t n = pix ? px.blocks : outer;
     bool summed = false;
     SEGK_DISPATCH_DTYPE(dtype, T, {
-        if (wide) {
-            auto kernel = dlogits ? distill_planes_kernel<T, true> : distill_planes_kernel<T, false>;
-            hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(256), 0, st, a, px.blocks_each);
-        } else if (pix) {
-            class_tier(C, px.vp, [&](auto cm, auto vp) {
-                if (dlogits) hipLaunchKernelGGL((distill_pixels_kernel<T, cm(), vp(), true>), dim3((unsigned)n), dim3(256), 0, st, a, px.blocks_each);
-                else hipLaunchKernelGGL((distill_pixels_kernel<T, cm(), vp(), false>), dim3((unsigned)n), dim3(256), 0, st, a, px.blocks_each);
+        if (pix) {
+            by_launches(px.outer, px.blocks_each * 256ll, [&](int64_t o, int64_t images) {
+                const DistillArgs b = from(o);
+                const dim3 grid((unsigned)(images * px.blocks_each));
+                if (wide) {
+                    auto kernel = dlogits ? distill_planes_kernel<T, true> : distill_planes_kernel<T, false>;
+                    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, b, px.blocks_each);
+                } else {
+                    class_tier(C, px.vp, [&](auto cm, auto vp) {
+                        if (dlogits) hipLaunchKernelGGL((distill_pixels_kernel<T, cm(), vp(), true>), grid, dim3(256), 0, st, b, px.blocks_each);
+                        else hipLaunchKernelGGL((distill_pixels_kernel<T, cm(), vp(), false>), grid, dim3(256), 0, st, b, px.blocks_each);
+                    });
+                }
             });
         } else if (const int shares = shares_of(outer, C, dtype); shares > 1) {
             float *parts = partial + outer, *joined = parts + outer * 2 * kShares;
@@ -1842,8 +1879,11 @@ extern "C" int segk_distill(const void* logits, int dtype, int64_t outer, int64_
             if (dlogits) hipLaunchKernelGGL((distill_share_grad_kernel<T>), dim3(shares, (unsigned)outer), dim3(256), 0, st, a, joined);
         } else {
             row_tier<T, false>(logits, ld, C, k, [&](auto nt, auto nch) {
-                if (dlogits) hipLaunchKernelGGL((distill_rows_kernel<T, nt(), nch(), true>), dim3((unsigned)n), dim3(nt()), 0, st, a);
-                else hipLaunchKernelGGL((distill_rows_kernel<T, nt(), nch(), false>), dim3((unsigned)n), dim3(nt()), 0, st, a);
+                by_launches(outer, nt(), [&](int64_t o, int64_t rows) {
+                    const DistillArgs b = from(o);
+                    if (dlogits) hipLaunchKernelGGL((distill_rows_kernel<T, nt(), nch(), true>), dim3((unsigned)rows), dim3(nt()), 0, st, b);
+                    else hipLaunchKernelGGL((distill_rows_kernel<T, nt(), nch(), false>), dim3((unsigned)rows), dim3(nt()), 0, st, b);
+                });
             });
         }
     });

@@ -673,3 +673,37 @@ def test_high_temperatures(shape, k, T):
         total.backward()
         for g in (x.grad, x2.grad):
             assert bool(((back(g) - grad).abs() <= gerr + 2.0 ** -24 * grad.abs()).all())
+
+
+@pytest.mark.parametrize("shape", [((1 << 26) + 5, 33), ((1 << 24) + 3, 4, 1, 2), ((1 << 24) + 3, 40, 1, 2)])
+def test_more_threads_than_one_launch_may_have(shape, monkeypatch):
+    """Rows, and images of few positions, whose threads number 2^32 and more (a launch has fewer): the same bits as parts of them give
+    (by the same kernel: a part's planes are not copied into rows for being few)."""
+    from segk import distill
+    monkeypatch.setattr(distill, "PLANE_POSITIONS", 0)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    N = shape[0]
+    teacher, student = (torch.empty(shape, dtype=BF16, device="cuda").normal_(generator=g) for _ in range(2))
+    target = top_logits(teacher, 2, temperature=2.0)
+    x = student.requires_grad_()
+    each = distill_loss_topk(x, target, temperature=2.0, reduction="none")
+    up = torch.rand(each.shape, generator=g, device="cuda")
+    grad, = torch.autograd.grad(each, x, up)
+    mean = distill_loss_topk(x, target, temperature=2.0)
+    grad_mean, = torch.autograd.grad(mean, x)
+    with torch.no_grad():
+        plain = distill_loss_topk(x, target, temperature=2.0)
+    want = float(each.detach().double().mean())
+    for got in (mean, plain):                                    # sums of up to 1024 losses in fp32 before those in double
+        assert abs(float(got.detach()) - want) <= 2.0 ** -20 * want
+    for lo in (0, N // 8 - 500, N // 4 - 500, N // 2 - 500, 3 * (N // 4) - 500, N - 1000):
+        part = slice(lo, lo + 1000)
+        top_part = top_logits(teacher[part], 2, temperature=2.0)
+        assert all(torch.equal(a[part], b) for a, b in zip(target, top_part))
+        y = x.detach()[part].requires_grad_()
+        few = distill_loss_topk(y, top_part, temperature=2.0, reduction="none")
+        assert torch.equal(few, each[part])
+        assert torch.equal(torch.autograd.grad(few, y, up[part], retain_graph=True)[0], grad[part])
+        # the scale is rounded once, the product once more, then to bf16, on both sides
+        sums = torch.autograd.grad(few.sum(), y)[0].double() / each.numel()
+        assert bool(((grad_mean[part].double() - sums).abs() <= 2.0 ** -6 * sums.abs() + 2.0 ** -133).all())
