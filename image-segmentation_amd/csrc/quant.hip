@@ -510,7 +510,6 @@ static int quantize(int dtype, const void* x, int64_t ld, int64_t rows, int64_t 
 template <typename TO, int BM, int BN, int WM, int WN, bool WIDE, int STAGES> static int launch_tile(const LinearArgs& a, hipStream_t st) {
     constexpr int bytes = STAGES * TileLds<BM, BN>::kStage;
     const int64_t tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN;
-    SEGK_REQUIRE(tm * tn < (1ll << 31), SEGK_ESHAPE, "mxfp4_linear: too many tiles");
     auto kernel = mxfp4_tile_kernel<TO, BM, BN, WM, WN, WIDE, STAGES>;
     if constexpr (bytes > 65536) {
         static std::atomic<bool> allowed[64] = {};               // once per device
@@ -574,6 +573,10 @@ extern "C" int segk_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const 
         SEGK_REQUIRE(packs_inside(M, K, N) || (workspace && workspace_bytes >= segk_mxfp4_linear_workspace(M, K, N)), SEGK_EWORKSPACE, "mxfp4_linear: workspace too small");
         SEGK_REQUIRE(aligned16(workspace), SEGK_EALIGN, "mxfp4_linear: workspace must be 16-byte aligned");
     } else if (const int rc = check_packed("mxfp4_linear", x_codes, x_scales)) return rc;
+    const int choice = kernel_of(M, N);
+    // a launch has fewer than 2^32 threads; those of the rows kernel are few
+    SEGK_REQUIRE(choice == 16 || ((M + choice - 1) / choice) * ((N + choice - 1) / choice) < (1ll << 32) / (choice == 256 ? 512 : 256), SEGK_ESHAPE,
+                 "mxfp4_linear: too many outputs for one launch");
     SEGK_USE_DEVICE(dev);
     hipStream_t st = (hipStream_t)stream;
     const bool pack_inside = x && packs_inside(M, K, N);
@@ -587,7 +590,6 @@ extern "C" int segk_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const 
     a.bias = bias; a.y = y; a.M = M; a.N = N; a.xs_rows = x && !pack_inside ? (int64_t)align_up(M, 4) : M; a.ldc = slices_of(K) * 64; a.ldy = ldy; a.slices = (int)slices_of(K);
     for (int v : {4, 8})
         if (reinterpret_cast<uintptr_t>(y) % (v * esize(y_dtype)) == 0 && ldy % v == 0) a.vec = v;
-    const int choice = kernel_of(M, N);
     const bool wide = N % 4 == 0 && a.xs_rows % 4 == 0 && aligned16(w_scales) && aligned16(x_scales);
     SEGK_DISPATCH_DTYPE(y_dtype, TO, {
         if (choice == 256 && wide) return launch_tile<TO, 256, 256, 2, 4, true, 2>(a, st);

@@ -581,7 +581,7 @@ int segk_mxfp4_dequantize(int dtype, const void* codes, const void* scales, int6
 /* y[M][N] = x[M][K] w[N][K]^T + bias with both operands in packed form on the scaled matrix instructions, fp32 accumulation in an
  * order fixed by the shape (deterministic), one rounding to y's type.  x is given as a matrix, packed by the call as above, or as
  * x_codes / x_scales (the other NULL).  bias: fp32 [N] or NULL.
- * M, N < 2^28, K < 2^24.  workspace: segk_mxfp4_linear_workspace(M, K, N) bytes (0 where x is packed on the way), 16-byte aligned; contents
+ * M, N < 2^28, K < 2^24, and fewer than 2^23 tiles of 256 x 256 outputs.  workspace: segk_mxfp4_linear_workspace(M, K, N) bytes (0 where x is packed on the way), 16-byte aligned; contents
  * need not be cleared. */
 size_t segk_mxfp4_linear_workspace(int64_t M, int64_t K, int64_t N);
 int segk_mxfp4_linear(const void* x, int x_dtype, int64_t ldx, const void* x_codes, const void* x_scales, int64_t M, int64_t K,

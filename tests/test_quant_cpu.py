@@ -110,3 +110,13 @@ def test_c_entry_points_refuse_bad_arguments_without_a_gpu():
             _lib.call("segk_mxfp4_linear", *{**base, **kw}.values())
     assert _lib.query("segk_mxfp4_codes_bytes", 3, 129) == 3 * 128 and _lib.query("segk_mxfp4_scales_bytes", 3, 129) == 24
     assert _lib.query("segk_mxfp4_codes_bytes", 0, 5) == 0
+
+
+def test_more_outputs_than_one_launch_holds_are_refused_without_a_gpu():
+    """A launch has fewer than 2^32 threads, 512 for each 256 x 256 tile; refused before anything is launched."""
+    from segk import _lib
+    for M, N in ((1 << 27, 1 << 27), (256 * (1 << 12), 256 * (1 << 11)), ((1 << 28) - 1, 65281)):
+        for packed in (False, True):
+            with pytest.raises(_lib.SegkError, match="too many outputs"):
+                _lib.call("segk_mxfp4_linear", None if packed else 4096, _lib.SEGK_BF16, 64, 4096 if packed else None, 4096 if packed else None, M, 64, 4096, 4096, N,
+                          None, 4096, _lib.SEGK_BF16, N, 4096, 1 << 60, 0, None)
