@@ -80,7 +80,7 @@ def top_logits(logits, k, dim=1, temperature=1.0):
         raise ValueError(f"k has to be between 1 and min({MAX_K}, {C} classes), got {k}")
     z = logits.detach() if logits.requires_grad else logits
     if not z.is_cuda or z.numel() == 0:
-        return _host_top(z, k, dim, temperature)
+        return _host_top(z.detach(), k, dim, temperature)            # detached from a forward-mode derivative as well
     before, behind = z.shape[:dim], z.shape[dim + 1:]
     z, outer, C, inner, ld, moved = _canonical(z.float() if z.dtype == torch.float16 else z, dim, PLANE_CLASSES if k <= PLANE_TOP else PLANE_FEW)
     device, rest = z.device, before + behind
@@ -190,7 +190,7 @@ def distill_loss_topk(pred, target, temperature=1.0, reduction="mean", dim=1, we
     `weight` scales loss and gradient; it costs nothing, where multiplying the returned loss costs another pass over the logits.
 
     pred: float32, bfloat16 or float16, any strides; target: TopLogits or a tuple (values, indices[, lse]) with float32 / bfloat16 /
-    float16 values and int32 / int64 indices.  Returns float32; the gradient has pred's type.  Sums run in float32 (in float64 on the
+    float16 values and int32 / int64 indices.  Differentiable once, backwards (on the CPU in any mode).  Returns float32; the gradient has pred's type.  Sums run in float32 (in float64 on the
     CPU).  log p carries the rounding of the kept lse, 2^-24 |lse|, so logits / T of some thousands leave no exact probabilities.
     Student and teacher differ by d / T in log q where their logits differ by d, and that is known to about 2^-22: loss and
     gradient are good to about T 2^-22 / d of themselves.  Where every class is kept with an lse, the rounding of the lse adds up to
@@ -216,7 +216,7 @@ def distill_loss_topk(pred, target, temperature=1.0, reduction="mean", dim=1, we
     device = pred.device
     if values.device != device or indices.device != device or (lse is not None and lse.device != device):
         raise ValueError("logits and target have to be on the same device")
-    if values.requires_grad or (lse is not None and lse.requires_grad):
+    if any(t is not None and (t.requires_grad or ops.has_tangent(t)) for t in (values, lse)):
         raise ValueError("the target is data: detach the teacher's logits")
     if not pred.is_cuda or pred.numel() == 0:
         return _host_distill(pred, values, indices, lse, dim, temperature, weight, reduction)
@@ -226,6 +226,8 @@ def distill_loss_topk(pred, target, temperature=1.0, reduction="mean", dim=1, we
     want_grad = torch.is_grad_enabled() and pred.requires_grad
     if lse is not None and lse.dtype != torch.float32:
         lse = lse.float()
+    if ops.has_tangent(pred):
+        raise NotImplementedError("distill_loss_topk has no forward-mode derivative on the GPU")
     if not want_grad:                                        # no node to be made (3 us)
         return _DistillFn.forward(None, pred, values, indices, lse, dim, temperature, weight, reduction, False)
     return _DistillFn.apply(pred, values, indices, lse, dim, temperature, weight, reduction, True)

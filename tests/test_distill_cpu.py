@@ -112,6 +112,24 @@ def test_refusals():
         distill_loss_topk(z, TopLogits(target.values.to("meta"), target.indices, None))
 
 
+def test_forward_mode_derivatives():
+    """Kept by the loss on the CPU; a target is data in this mode too."""
+    import torch.autograd.forward_ad as fwd
+    z, target = problem(5, 30, 4, T=2.0)
+    tangent = torch.randn(z.shape, generator=torch.Generator().manual_seed(9))
+    _, grad, _, _, _ = loss_and_gradient(z, *target, 2.0)
+    with fwd.dual_level():
+        dual = fwd.make_dual(z.double(), tangent.double())
+        got = fwd.unpack_dual(distill_loss_topk(dual, target, temperature=2.0, reduction="sum")).tangent
+        assert abs(float(got) - float((grad * tangent.double()).sum())) < 1e-9
+        for f in top_logits(fwd.make_dual(z, tangent), 3):
+            assert fwd.unpack_dual(f).tangent is None
+        with pytest.raises(ValueError, match="detach"):
+            distill_loss_topk(z, target._replace(values=fwd.make_dual(target.values, torch.ones_like(target.values))))
+        with pytest.raises(ValueError, match="detach"):
+            distill_loss_topk(z, target._replace(lse=fwd.make_dual(target.lse, torch.ones_like(target.lse))))
+
+
 def test_c_entry_points_refuse_bad_arguments_without_a_gpu():
     from segk import _lib
     F32, BF16 = _lib.SEGK_F32, _lib.SEGK_BF16

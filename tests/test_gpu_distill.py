@@ -707,3 +707,22 @@ def test_more_threads_than_one_launch_may_have(shape, monkeypatch):
         # the scale is rounded once, the product once more, then to bf16, on both sides
         sums = torch.autograd.grad(few.sum(), y)[0].double() / each.numel()
         assert bool(((grad_mean[part].double() - sums).abs() <= 2.0 ** -6 * sums.abs() + 2.0 ** -133).all())
+
+
+@pytest.mark.parametrize("shape", [(6, 40), (2, 4, 3, 5)])
+def test_forward_mode_is_refused(shape):
+    """The kernels give no tangent: a dual number is refused with and without a gradient, never answered without its tangent."""
+    import torch.autograd.forward_ad as fwd
+    x = torch.randn(shape, device="cuda")
+    target = top_logits(x, 2)
+    with fwd.dual_level():
+        for form in (x, x.clone().requires_grad_()):
+            dual = fwd.make_dual(form, torch.ones_like(x))
+            for f in top_logits(dual, 2):
+                assert fwd.unpack_dual(f).tangent is None
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
+                    distill_loss_topk(dual, target)
+        assert torch.isfinite(distill_loss_topk(x, target))         # no dual: answered
+    with pytest.raises(NotImplementedError):
+        torch.func.jvp(lambda y: distill_loss_topk(y, target), (x,), (torch.ones_like(x),))
