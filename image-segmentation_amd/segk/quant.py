@@ -64,6 +64,8 @@ def _rows(x, what):
         if torch.is_grad_enabled():
             raise RuntimeError(f"{what} requires a gradient and 4-bit rounding has none: call under torch.no_grad() or detach it")
         x = x.detach()
+    if ops.has_tangent(x):
+        raise RuntimeError(f"{what} carries a forward-mode derivative and 4-bit rounding has none: detach it")
     if x.dtype == torch.float16:
         x = x.float()
     dt(x.dtype)
@@ -139,6 +141,8 @@ def mxfp4_linear(x, w, bias=None, out_dtype=None):
             raise ValueError(f"bias has to be a floating point tensor [{N}] on the device of w")
         if bias.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("bias requires a gradient: call under torch.no_grad() or detach it")
+        if ops.has_tangent(bias):
+            raise RuntimeError("bias carries a forward-mode derivative: detach it")
         if bias.dtype != torch.float32 or bias.requires_grad or not bias.is_contiguous():
             bias = bias.detach().float().contiguous()
     if not w.codes.is_cuda:

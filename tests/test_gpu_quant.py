@@ -6,7 +6,7 @@ import torch
 from distill_oracle import loss_and_gradient, top
 from loss.distill import distill_loss_topk, top_logits
 from segk.quant import MXFP4, mxfp4_dequantize, mxfp4_linear, mxfp4_quantize
-from test_quant_cpu import four_bit
+from test_quant_cpu import forward_mode_is_refused, four_bit
 
 pytestmark = pytest.mark.gpu
 F32, BF16 = torch.float32, torch.bfloat16
@@ -206,3 +206,7 @@ def test_chain_other_stream_and_captured_graph():
             g.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(a, c.detach()) for a, c in zip(want, out))
+
+
+def test_forward_mode():
+    forward_mode_is_refused("cuda")

@@ -120,3 +120,23 @@ def test_more_outputs_than_one_launch_holds_are_refused_without_a_gpu():
             with pytest.raises(_lib.SegkError, match="too many outputs"):
                 _lib.call("segk_mxfp4_linear", None if packed else 4096, _lib.SEGK_BF16, 64, 4096 if packed else None, 4096 if packed else None, M, 64, 4096, 4096, N,
                           None, 4096, _lib.SEGK_BF16, N, 4096, 1 << 60, 0, None)
+
+
+def forward_mode_is_refused(device):
+    import torch.autograd.forward_ad as fwd
+    w = mxfp4_quantize(torch.randn(4, 40, device=device))
+    x, b = torch.randn(3, 40, device=device), torch.zeros(4, device=device)
+    want = mxfp4_linear(x, w, b)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                for call in (lambda: mxfp4_quantize(dual), lambda: mxfp4_linear(dual, w), lambda: mxfp4_linear(x, w, fwd.make_dual(b, torch.ones_like(b)))):
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        call()
+        assert torch.equal(mxfp4_linear(dual.detach(), w, b), want)
+
+
+def test_forward_mode_is_refused():
+    """4-bit rounding has no derivative: a dual number is refused like a tensor that requires a gradient, also under no_grad."""
+    forward_mode_is_refused("cpu")
