@@ -402,7 +402,8 @@ __device__ __forceinline__ Kept kept_entries(const DistillArgs& a, int64_t row, 
     if (!(e.rest > kRestFloor) || distinct == a.V) e.rest = 0.f;
     e.mass = mass + e.rest;
     e.top = wave_max(first ? e.z : -INFINITY);
-    e.sum = sum_wave(first && e.top != -INFINITY ? exp_over(e.z, e.top, c) : 0.f);
+    // no maximum: -inf, whose exp is 0, or NaN, which has to reach the row
+    e.sum = sum_wave(!first ? 0.f : e.top != -INFINITY ? exp_over(e.z, e.top, c) : e.z != e.z ? e.z : 0.f);
     return e;
 }
 // maximum and sum of exp over all classes, from those outside (ko, so) and those kept; share: exp of ko over the maximum

@@ -726,3 +726,26 @@ def test_forward_mode_is_refused(shape):
         assert torch.isfinite(distill_loss_topk(x, target))         # no dual: answered
     with pytest.raises(NotImplementedError):
         torch.func.jvp(lambda y: distill_loss_topk(y, target), (x,), (torch.ones_like(x),))
+
+
+@pytest.mark.parametrize("shape,k", [((5, 80), 1), ((5, 300), 2), ((9, 4), 1), ((5, 40000), 1), ((5, 140000), 1), ((2, 4, 3, 5), 1), ((2, 40, 128, 64), 1)])
+def test_nan_at_the_only_kept_classes(shape, k):
+    """softmax of a row with a NaN is NaN everywhere: so are its loss and its whole gradient, wherever the NaN stands."""
+    C = shape[1]
+    g = torch.Generator().manual_seed(C)
+    z = torch.randn(shape, generator=g)
+    z[1].view(C, -1)[C // 2:C // 2 + k, 0] = math.nan
+    indices = (C // 2 + torch.arange(k, dtype=torch.int32)).view((1, k) + (1,) * (len(shape) - 2)).expand((shape[0], k) + shape[2:]).contiguous()
+    for lse in (None, torch.full(shape[:1] + shape[2:], math.log(2.0 * k))):
+        target = TopLogits(torch.zeros(indices.shape), indices, lse)
+        host, x = z.clone().requires_grad_(), z.cuda().requires_grad_()
+        want, got = (distill_loss_topk(t, TopLogits(*(None if f is None else f.to(t.device) for f in target)), reduction="none") for t in (host, x))
+        want.sum().backward()
+        got.sum().backward()
+        bad = torch.zeros(shape, dtype=torch.bool)
+        bad[1].view(C, -1)[:, 0] = True
+        assert torch.equal(host.grad.isnan(), bad) and torch.equal(x.grad.isnan().cpu(), bad)
+        assert torch.equal(want.isnan(), got.isnan().cpu()) and int(want.isnan().sum()) == 1
+        y = z.cuda().requires_grad_()
+        distill_loss_topk(y, TopLogits(*(None if f is None else f.cuda() for f in target)), reduction="sum").backward()
+        assert torch.equal(y.grad.isnan().cpu(), bad)
