@@ -358,7 +358,7 @@ __device__ __forceinline__ Kept kept_entries(const DistillArgs& a, int64_t row, 
         e.p = cls >= 0 ? fast_exp2(e.lp) : 0.f;
     } else {
         const float top = wave_max(t);
-        const float x = cls >= 0 && top != -INFINITY ? fast_exp2((t - top) * c) : 0.f;
+        const float x = t == -INFINITY ? 0.f : fast_exp2((t - top) * c);      // NaN stays, also where nothing else was kept
         const float sum = sum_wave(x);
         e.p = sum == 0.f ? 0.f : x / sum;
         e.lp = (t - top) * c - log2f(sum);
@@ -800,7 +800,7 @@ __global__ __launch_bounds__(256) void distill_pixels_kernel(const DistillArgs a
                 for (int v = 0; v < VP; ++v) top[v] = cj[v] >= 0 ? fmaxf(top[v], t[v]) : top[v];
             }
         auto log_p = [&](float t, int v) {    // base 2, before it is normalised where no logsumexp is given
-            return a.tlse ? fmaf(t, a.invT, -lse[v]) * kLog2e : (top[v] == -INFINITY ? -INFINITY : (t - top[v]) * c);
+            return a.tlse ? fmaf(t, a.invT, -lse[v]) * kLog2e : (t == -INFINITY ? -INFINITY : (t - top[v]) * c);
         };
         for (int j = 0; j < a.k; ++j) {
             int cj[VP];
@@ -952,7 +952,7 @@ __global__ __launch_bounds__(256) void distill_planes_kernel(const DistillArgs a
                 if (load_class(a, at + j * a.inner) >= 0) top = fmaxf(top, load_kept(a, at + j * a.inner));
         auto log_p = [&](int j) {             // base 2, before it is normalised where no logsumexp is given
             const float t = load_kept(a, at + j * a.inner);
-            return a.tlse ? fmaf(t, a.invT, -lse) * kLog2e : (top == -INFINITY ? -INFINITY : (t - top) * c);
+            return a.tlse ? fmaf(t, a.invT, -lse) * kLog2e : (t == -INFINITY ? -INFINITY : (t - top) * c);
         };
         uint32_t kept[kPlaneClasses / 32] = {};
         bool twice = false;

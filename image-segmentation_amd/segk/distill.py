@@ -261,7 +261,7 @@ def _host_distill(pred, values, indices, lse, dim, T, weight, reduction):
     logq = torch.log_softmax(z, -1)
     if lse is None:
         top = t.amax(-1, keepdim=True)
-        e = torch.where(valid & (top > -math.inf), torch.exp(t - top), torch.zeros((), dtype=z.dtype))
+        e = torch.where(t == minus, torch.zeros((), dtype=z.dtype), torch.exp(t - top))
         s = e.sum(-1, keepdim=True)
         p = torch.where(s == 0, torch.zeros((), dtype=z.dtype), e / s)
     else:

@@ -195,3 +195,28 @@ def test_host_loss_at_high_temperatures(T, rest):
     assert got.dtype == torch.float32 and bool(((got.double() - loss).abs() <= 2.0 ** -24 * loss.abs() + T * T * 2.0 ** -47).all())
     got.sum().backward()
     assert bool(((x.grad.double() - grad).abs() <= 2.0 ** -24 * grad.abs() + T * 2.0 ** -47).all())
+
+
+def nan_among_the_values(device):
+    """A teacher's NaN without a logsumexp: softmax over the kept entries is NaN, and so are loss and gradient; entries that do not exist
+    may hold anything, and a row of nothing but -inf counts as 0."""
+    for shape in ((5, 9), (5, 80), (5, 40000), (5, 140000), (5, 4, 2, 3), (5, 40, 64, 64)):
+        C, behind = shape[1], shape[2:]
+        for k in (1, 3):
+            for dtype in (torch.float32, torch.bfloat16):
+                values = torch.zeros((5, k) + behind, dtype=dtype)
+                indices = torch.arange(k).view((1, k) + (1,) * len(behind)).repeat((5, 1) + behind)
+                values[1, 0], values[2], values[3, k - 1] = math.nan, math.nan, math.nan
+                indices[3, k - 1] = -1
+                values[4] = -math.inf
+                x = torch.zeros(shape, device=device, requires_grad=True)
+                loss = distill_loss_topk(x, TopLogits(values.to(device), indices.to(device)), reduction="none")
+                loss.sum().backward()
+                rows, grads = loss.detach().view(5, -1), x.grad.view(5, -1)
+                assert rows[1:3].isnan().all() and grads[1:3].isnan().all()
+                assert torch.isfinite(rows[[0, 3, 4]]).all() and torch.isfinite(grads[[0, 3, 4]]).all() and not rows[4].any() and not grads[4].any()
+                assert float(distill_loss_topk(x.detach(), TopLogits(values.to(device), indices.to(device)), reduction="sum").isnan())
+
+
+def test_nan_among_the_values():
+    nan_among_the_values("cpu")

@@ -7,6 +7,7 @@ import torch
 
 from distill_oracle import cancellation_bounds, half_step, loss_and_gradient, top
 from loss.distill import TopLogits, distill_loss_topk, top_logits
+from test_distill_cpu import nan_among_the_values
 
 pytestmark = pytest.mark.gpu
 F32, BF16 = torch.float32, torch.bfloat16
@@ -749,3 +750,7 @@ def test_nan_at_the_only_kept_classes(shape, k):
         y = z.cuda().requires_grad_()
         distill_loss_topk(y, TopLogits(*(None if f is None else f.cuda() for f in target)), reduction="sum").backward()
         assert torch.equal(y.grad.isnan().cpu(), bad)
+
+
+def test_nan_among_the_values():
+    nan_among_the_values("cuda")
