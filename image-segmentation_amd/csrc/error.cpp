@@ -23,3 +23,13 @@ int fail(int code, const char* fmt, ...) {
 
 extern "C" const char* segk_last_error(void) { return segk::g_err; }
 extern "C" int segk_version(void) { return 100; }
+
+extern "C" size_t segk_capture_id(void* stream) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo((hipStream_t)stream, &status, &id) != hipSuccess) {
+        (void)hipGetLastError();
+        return 0;
+    }
+    return status == hipStreamCaptureStatusActive ? (size_t)id : 0;
+}

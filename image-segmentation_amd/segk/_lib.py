@@ -19,6 +19,7 @@ P, I, L, F, Z = c_void_p, c_int, c_int64, c_float, c_size_t
 # name -> (restype, argtypes); int-returning functions are status codes
 _PROTOS = {
     "segk_last_error": (ctypes.c_char_p, []),
+    "segk_capture_id": (Z, [P]),
     "segk_version": (I, []),
     "segk_dice_focal_workspace": (Z, [L, L, L]),
     "segk_dice_focal_fwd": (I, [P, I, P, P, L, L, L, F, P, I, P, P, P, P, Z, I, P]),

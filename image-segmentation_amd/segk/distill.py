@@ -99,7 +99,9 @@ def top_logits(logits, k, dim=1, temperature=1.0):
 
 class _DistillFn(torch.autograd.Function):
     """(student logits, target) -> loss.  Where a scalar's gradient will be wanted, the forward pass writes it for an upstream
-    gradient of 1 while the row is still in registers; the backward pass hands it over, recomputed only if upstream is not 1."""
+    gradient of 1 while the row is still in registers; the backward pass hands it over, recomputed only if upstream is not 1.  That needs
+    one forward pass for each backward pass: where only one of them is captured into a graph, or each into its own, a replayed backward
+    pass would find what an earlier replay left, so it computes a gradient of its own."""
 
     @staticmethod
     def forward(ctx, logits, values, indices, lse, dim, temperature, weight, reduction, want_grad):
@@ -120,7 +122,7 @@ class _DistillFn(torch.autograd.Function):
         args = _DistillFn._launch(meta, z, values, indices, lse, None, MEAN if reduction == "mean" else 0, None if each else out, out if each else None, dz, ws)
         if want_grad:
             ctx.save_for_backward(z, values, indices, lse)
-            ctx.meta, ctx.dz, ctx.ws, ctx.args, ctx.stride = meta, dz, ws, args, z.stride()
+            ctx.meta, ctx.dz, ctx.ws, ctx.args, ctx.stride, ctx.capture = meta, dz, ws, args, z.stride(), query("segk_capture_id", args[23])
         return out
 
     @staticmethod
@@ -153,6 +155,8 @@ class _DistillFn(torch.autograd.Function):
         if g.dtype != torch.float32 or not g.is_contiguous():
             g = g.float().contiguous()
         args = ctx.args
+        if dz is not None and query("segk_capture_id", _env(z)[1]) != ctx.capture:
+            dz = None
         if z.data_ptr() != args[0] or z.stride() != ctx.stride:   # hooks on saved tensors brought back a copy, maybe in another layout
             z, _, _, _, ld, _ = _canonical(z.reshape(outer, C, inner), 1, C)
             meta = (outer, C, inner, ld) + meta[4:]

@@ -39,6 +39,8 @@ enum {
 };
 
 const char* segk_last_error(void);
+/* What `stream` is being captured into: a number of that capture's own, 0 if nothing.  Two calls whose numbers differ do not run equally often. */
+size_t segk_capture_id(void* stream);
 int segk_version(void);
 
 /* ------------------------------------------------------------------------------------------------
@@ -131,7 +133,8 @@ int segk_top_logits(const void* logits, int dtype, int64_t outer, int64_t C, int
  *                 logits.  flags bit1: upstream has one value per position (not with bit0): gradient of position_loss.
  * flags bit2 (upstream and dlogits given, no other output): dlogits already holds the gradient for an upstream of 1, written by a
  * call with the same arguments, and the call leaves it as it is if *upstream is 1 -- a backward pass that finds the gradient of
- * the forward pass still right.  `workspace` has to be that call's, with its contents.
+ * the forward pass still right.  `workspace` has to be that call's, with its contents.  Once per such call: an upstream that is not 1 replaces
+ * dlogits, so this flag does not belong into a captured graph without the call itself.
  * values_dtype fp32 or bf16, index_bytes 4 or 8 (int32 / int64).  Deterministic. */
 size_t segk_distill_workspace(int64_t outer, int64_t C, int64_t inner);
 int segk_distill(const void* logits, int dtype, int64_t outer, int64_t C, int64_t inner, int64_t ld, const void* values, int values_dtype,

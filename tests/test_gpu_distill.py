@@ -754,3 +754,49 @@ def test_nan_at_the_only_kept_classes(shape, k):
 
 def test_nan_among_the_values():
     nan_among_the_values("cuda")
+
+
+@pytest.mark.parametrize("shape,k", [((40, 300), 5), ((3, 4, 9, 16), 2), ((2, 140000), 3), ((1, 40, 128, 128), 2)])
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_backward_pass_replayed_without_its_forward_pass(shape, k, captured):
+    """Captured by itself (the forward pass eager, or in a graph of its own) and replayed with other upstream gradients: nothing of one replay
+    is left for the next.  The node is called directly, on the capturing stream."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    target = top_logits(torch.randn(shape, generator=g, device="cuda"), k, temperature=2.0)
+    x = torch.randn(shape, generator=g, device="cuda").requires_grad_()
+    up = torch.ones((), device="cuda")
+    forward, backward = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    if captured:
+        with torch.cuda.graph(forward):
+            loss = distill_loss_topk(x, target, temperature=2.0)
+    else:
+        loss = distill_loss_topk(x, target, temperature=2.0)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(backward):
+        grad = loss.grad_fn.apply(up)[0]
+    for turn, scale in enumerate((2.0, 1.0, 0.5, 1.0, 1.0, -3.0)):
+        if captured and turn % 2 == 0:
+            with torch.no_grad():
+                x.copy_(torch.randn(shape, generator=g, device="cuda"))
+            forward.replay()
+        up.fill_(scale)
+        backward.replay()
+        torch.cuda.synchronize()
+        y = x.detach().clone().requires_grad_()
+        want = distill_loss_topk(y, target, temperature=2.0)
+        assert torch.equal(loss.detach(), want.detach())
+        assert torch.equal(grad, torch.autograd.grad(want, y, torch.full((), scale, device="cuda"))[0])
+
+
+def test_graphed_callable():
+    """torch.cuda.make_graphed_callables: forward and backward pass in graphs of their own, inside an eager program."""
+    z, values, indices, lse = problem(30, 90, 4, T=2.0)
+    target = TopLogits(values.cuda(), indices.cuda(), lse.cuda())
+    run = torch.cuda.make_graphed_callables(lambda x: distill_loss_topk(x, target, temperature=2.0), (z.cuda().requires_grad_(),))
+    for seed, scale in ((1, 1.0), (2, 3.0), (3, 1.0)):
+        x = torch.randn(30, 90, generator=torch.Generator().manual_seed(seed)).cuda().requires_grad_()
+        y = x.detach().clone().requires_grad_()
+        (run(x) * scale).backward()
+        (distill_loss_topk(y, target, temperature=2.0) * scale).backward()
+        torch.cuda.synchronize()
+        assert torch.equal(x.grad, y.grad)
