@@ -121,8 +121,9 @@ class _DistillFn(torch.autograd.Function):
         ws = torch.empty(query("segk_distill_workspace", outer, C, inner), dtype=torch.uint8, device=z.device)
         args = _DistillFn._launch(meta, z, values, indices, lse, None, MEAN if reduction == "mean" else 0, None if each else out, out if each else None, dz, ws)
         if want_grad:
-            ctx.save_for_backward(z, values, indices, lse)
-            ctx.meta, ctx.dz, ctx.ws, ctx.args, ctx.stride, ctx.capture = meta, dz, ws, args, z.stride(), query("segk_capture_id", args[23])
+            # the gradient among them, as large as the logits: offloading and recomputation (hooks on saved tensors) get hold of it
+            ctx.save_for_backward(z, values, indices, lse, dz, None if each else ws)
+            ctx.meta, ctx.first, ctx.args, ctx.stride, ctx.capture = meta, dz is not None, args, z.stride(), query("segk_capture_id", args[23])
         return out
 
     @staticmethod
@@ -149,14 +150,16 @@ class _DistillFn(torch.autograd.Function):
 
     @staticmethod
     def _gradients(ctx, g):
-        z, values, indices, lse = ctx.saved_tensors
+        z, values, indices, lse, dz, ws = ctx.saved_tensors
         outer, C, inner, ld, moved, k, dim, T, weight, reduction, shape, in_dtype = meta = ctx.meta
-        dz, ctx.dz, ws, ctx.ws = ctx.dz, None, ctx.ws, None      # handed over once; a second backward pass computes its own
+        first, ctx.first = ctx.first, False                      # handed over once; a second backward pass computes its own
         if g.dtype != torch.float32 or not g.is_contiguous():
             g = g.float().contiguous()
         args = ctx.args
-        if dz is not None and query("segk_capture_id", _env(z)[1]) != ctx.capture:
+        if not first or query("segk_capture_id", _env(z)[1]) != ctx.capture or not dz.is_contiguous() or not ws.is_contiguous():
             dz = None
+        else:
+            dz = dz.data             # what the caller does to its gradient is no change to a saved tensor: that one is not read again
         if z.data_ptr() != args[0] or z.stride() != ctx.stride:   # hooks on saved tensors brought back a copy, maybe in another layout
             z, _, _, _, ld, _ = _canonical(z.reshape(outer, C, inner), 1, C)
             meta = (outer, C, inner, ld) + meta[4:]
@@ -172,7 +175,7 @@ class _DistillFn(torch.autograd.Function):
             # the forward pass's arguments once more: this runs in autograd's thread, where every line costs several times its usual time
             args[14] |= SKIP
             args[6], args[8], args[10] = values.data_ptr(), indices.data_ptr(), ops._p(lse)
-            args[15], args[16], args[23] = g.data_ptr(), None, _env(z)[1]
+            args[15], args[16], args[18], args[20], args[23] = g.data_ptr(), None, dz.data_ptr(), ws.data_ptr(), _env(z)[1]
             call("segk_distill", *args)
         if moved:
             dz = dz.movedim(-1, dim)

@@ -800,3 +800,50 @@ def test_graphed_callable():
         (distill_loss_topk(y, target, temperature=2.0) * scale).backward()
         torch.cuda.synchronize()
         assert torch.equal(x.grad, y.grad)
+
+
+@pytest.mark.parametrize("scale", [1.0, 2.0])
+@pytest.mark.parametrize("shape,k", [((512, 4096), 5), ((4, 8, 256, 256), 2)])
+def test_saved_memory_can_be_offloaded_and_recomputed(shape, k, scale):
+    """Nothing as large as the logits stays on the device between the passes, where saved tensors are kept on the host or computed again."""
+    from torch.utils.checkpoint import checkpoint
+    g = torch.Generator(device="cuda").manual_seed(3)
+    target = top_logits(torch.randn(shape, generator=g, device="cuda"), k, temperature=2.0)
+    z = torch.randn(shape, generator=g, device="cuda")
+    x = z.clone().requires_grad_()
+    want, = torch.autograd.grad(scale * distill_loss_topk(x, target, temperature=2.0), x)
+
+    def offloaded(y):
+        with torch.autograd.graph.save_on_cpu():
+            return distill_loss_topk(y, target, temperature=2.0)
+
+    def again(y):
+        return checkpoint(lambda t: distill_loss_topk(t, target, temperature=2.0), y, use_reentrant=False)
+    for form in (offloaded, again):
+        y = z.clone().requires_grad_()
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        loss = form(y)
+        torch.cuda.synchronize()
+        assert torch.cuda.memory_allocated() - before < z.numel() * z.element_size() // 4
+        (scale * loss).backward()
+        assert torch.equal(y.grad, want)
+
+
+def test_the_gradient_belongs_to_the_caller():
+    """Changing it in place is no change to what a second backward pass needs."""
+    z, values, indices, lse = problem(20, 70, 4, T=2.0)
+    x = z.cuda().requires_grad_()
+    loss = distill_loss_topk(x, TopLogits(values.cuda(), indices.cuda(), lse.cuda()), temperature=2.0)
+    want, = torch.autograd.grad(loss, x, retain_graph=True)
+    kept = want.clone()
+    want.mul_(0.25)
+    for _ in range(2):
+        got, = torch.autograd.grad(loss, x, retain_graph=True)
+        assert torch.equal(got, kept)
+        got.zero_()
+    loss.backward(retain_graph=True)
+    x.grad.mul_(2.0)
+    x.grad = None
+    loss.backward()
+    assert torch.equal(x.grad, kept)
