@@ -1633,17 +1633,19 @@ constexpr int kPixelClasses = 32;    // more classes than this: one workgroup (o
 // Threads of a row's workgroup and pieces in registers per thread, by the row's length.  Rows of 16 to 64 KB: 512 threads with 8
 // pieces serve the loss, 256 with 16 the selection, whose search by the first wave leaves the others idle (4096 rows of 32000 bf16
 // logits: loss and gradient 103 against 107 us, selection 66 against 56; six waves of the latter per SIMD instead of five: 67 -> 63).
-template <typename T, bool TOP, typename F> static void row_tier(const void* z, int64_t ld, int64_t V, int64_t k, F&& f) {
+template <typename T, bool TOP, typename F> static void row_tier(const void* z, int64_t rows, int64_t ld, int64_t V, int64_t k, F&& f) {
     constexpr int VEC = 16 / (int)sizeof(T);
     // Rows that begin between two pieces may touch one more.  (4096 rows of 16384 bf16 logits, 2048 pieces: selection 52 -> 39 us, loss with
     // gradient 83 -> 62 since they are not taken for 2049.)
     const int64_t pieces = (V + (aligned16(z) && ld % VEC == 0 ? VEC - 1 : 2 * (VEC - 1))) / VEC;
 #define SEGK_TIER(nt, nch) if (pieces <= (int64_t)(nt) * (nch)) return f(std::integral_constant<int, nt>{}, std::integral_constant<int, nch>{})
     SEGK_TIER(64, 1);
-    // The selection's bound lets few candidates through while k is well below the number of threads.  64 / 256 threads, 20000 rows of 2000
-    // bf16 logits: 24 kept 51/68 us, 32 kept 70/71, 64 kept 527/111; of 300 fp32 logits, all of which its list holds, 64 kept: 72/115.
-    if (!TOP || k <= 24 || V <= 512) SEGK_TIER(64, 2);
-    if (!TOP || k <= 24) {
+    // The selection's bound lets few candidates through while k is well below the number of threads; a wave for each row still wins where its list
+    // holds all that pass and the rows fill the chip.  64 / 256 threads, us: 20000 rows of 2000 bf16 logits, 24 kept 51/68, 32 kept 70/71,
+    // 64 kept 517/111; of 1000, 32 kept 50/72, 40 kept 65/80, 48 kept 99/96; 8000 rows of 1000, 32 kept 32/34, 40 kept 37/37; 1000 rows
+    // 20/13, 24/14.  fp32, 32 kept: 20000 rows of 1000 58/64, 8000 28/30, 4000 17/19, 2000 15/12.  20000 rows of 300, 64 kept: 71/114.
+    if (!TOP || k <= 24 || V <= 512 || (V <= 1024 && k <= 40 && rows >= 6144)) {
+        SEGK_TIER(64, 2);
         SEGK_TIER(64, 4);
         SEGK_TIER(64, 8);
     }
@@ -1748,7 +1750,7 @@ extern "C" int segk_top_logits(const void* logits, int dtype, int64_t outer, int
                 }
             });
         } else {
-            row_tier<T, true>(logits, ld, C, k, [&](auto nt, auto nch) {
+            row_tier<T, true>(logits, outer, ld, C, k, [&](auto nt, auto nch) {
                 constexpr int r = rows_per_group(nt(), nch());
                 by_launches(outer, nt(), [&](int64_t o, int64_t n) {
                     hipLaunchKernelGGL((top_rows_kernel<T, nt(), nch()>), dim3((unsigned)((n + r - 1) / r)), dim3(nt(), r), 0, st, (const T*)logits + o * ld, n, ld, (int)C,
@@ -1879,7 +1881,7 @@ extern "C" int segk_distill(const void* logits, int dtype, int64_t outer, int64_
             hipLaunchKernelGGL((distill_join_kernel<T>), dim3((unsigned)outer), dim3(64), 0, st, a, parts, shares, dlogits ? joined : nullptr, rows_done, loss);
             if (dlogits) hipLaunchKernelGGL((distill_share_grad_kernel<T>), dim3(shares, (unsigned)outer), dim3(256), 0, st, a, joined);
         } else {
-            row_tier<T, false>(logits, ld, C, k, [&](auto nt, auto nch) {
+            row_tier<T, false>(logits, outer, ld, C, k, [&](auto nt, auto nch) {
                 by_launches(outer, nt(), [&](int64_t o, int64_t rows) {
                     const DistillArgs b = from(o);
                     if (dlogits) hipLaunchKernelGGL((distill_rows_kernel<T, nt(), nch(), true>), dim3((unsigned)rows), dim3(nt()), 0, st, b);

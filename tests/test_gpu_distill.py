@@ -847,3 +847,21 @@ def test_the_gradient_belongs_to_the_caller():
     x.grad = None
     loss.backward()
     assert torch.equal(x.grad, kept)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("P", [6143, 6144])
+@pytest.mark.parametrize("V", [511, 513, 1024, 1025])
+def test_top_of_rows_by_a_wave_or_a_workgroup(P, V, dtype):
+    """Both sides of the borders between them, in rows, classes and kept logits; rows that begin anywhere."""
+    g = torch.Generator().manual_seed(V)
+    z = torch.randn(P, V + 1, generator=g).to(dtype)
+    z[::7] = z[::7].mul(4).round()                               # ties
+    for form in (z[:, :-1].contiguous(), z[:, 1:]):
+        x = form.cuda() if form.is_contiguous() else z.cuda()[:, 1:]
+        for k in (24, 25, 40, 41):
+            got = top_logits(x, k)
+            if k == 24:
+                order = torch.sort(form.float(), dim=1, descending=True, stable=True).indices[:, :41]
+                values = form.gather(1, order)
+            assert torch.equal(got.indices.cpu().long(), order[:, :k]) and torch.equal(got.values.cpu(), values[:, :k])
