@@ -11,10 +11,7 @@ from .ops import _env, dt
 
 MEAN, EACH, SKIP = 1, 2, 4          # flag bits of segk_distill
 MAX_K = 64
-# Class planes [N, C, ...] are read as they are up to PLANE_FEW classes, and up to PLANE_CLASSES (selection: of PLANE_TOP at most) if there
-# are PLANE_POSITIONS; others are copied into rows.  In place / copied, selection and loss with gradient, fp32, 8 kept, us: 128 x 128
-# positions of 33 classes 11/22, 29/46, of 150 38/31, 45/59; 64 x 64 of 150 41/12, 45/28; 8 x 256 x 256 of 80 70/483, 320/829.
-PLANE_FEW, PLANE_CLASSES, PLANE_TOP, PLANE_POSITIONS = 32, 256, 8, 16384
+PLANE_FEW, PLANE_CLASSES, PLANE_TOP, PLANE_POSITIONS, PLANE_INNER = 32, 256, 8, 16384, 16
 REST_FLOOR = 2.0 ** -20             # a rest of the teacher's mass up to this is rounding and counts as none
 
 
@@ -49,14 +46,31 @@ def _check(logits, dim, temperature):
     return dim % logits.dim()
 
 
-def _canonical(x, dim, most=PLANE_CLASSES):
-    """(tensor, outer, C, inner, ld, moved): x as `outer` images of C x `inner`, in place where its strides allow it.  More than
-    `most` classes in front of other dimensions are moved to the end (a copy), and more than PLANE_FEW of few positions."""
+def _in_place(C, outer, inner, size, selected):
+    """Whether class planes [N, C, ...] are read as they are, not copied into rows; selected: as many are selected (0: the loss).
+
+    Up to PLANE_FEW classes always (a thread holds them).  Up to PLANE_CLASSES, and PLANE_TOP selected, where the positions fill the chip: until
+    they do a thread for each costs the same time however few they are, about in proportion to the classes (and, of the selection, half as
+    much again beyond 2 kept), while the copy's grows with the positions.  In place / copied, fp32 (bf16), us: 128 x 128 positions, loss
+    with gradient, 8 kept: 33 classes 32/50 (34/61), 80 38/53 (47/59), 150 47/62 (66/70), 256 69/70 (94/72), 64 kept of 80 134/134
+    (145/182); selection of 1: 80 classes 13/19 (18/19), 150 22/28 (30/27), 256 33/37 (48/32); of 8: 80 23/23 (28/33), 150 40/32 (48/32), 256
+    63/41 (78/36); 192 x 192: 150 40/61 (48/61), 256 70/82 (78/64).  An image has a workgroup of its own, so those of few positions
+    leave it idle: 16384 images of 2 x 2 (4096 of 4 x 4) positions, 80 classes, loss with gradient 334/126 (104/128).  With
+    PLANE_POSITIONS 0 whatever the kernels can read is read in place."""
+    if inner == 1 or C <= PLANE_FEW:
+        return True
+    full = (164 if size == 4 else 102) * (2 / 3 if selected > 2 else 1)      # classes of which PLANE_POSITIONS are enough
+    return C <= PLANE_CLASSES and selected <= PLANE_TOP and inner >= min(PLANE_INNER, PLANE_POSITIONS) and outer * inner >= PLANE_POSITIONS * max(1.0, C / full)
+
+
+def _canonical(x, dim, selected=0, keep=False):
+    """(tensor, outer, C, inner, ld, moved): x as `outer` images of C x `inner`, in place where its strides allow it.  Classes in front
+    of other dimensions are moved to the end (a copy) where _in_place does not hold; never with `keep`."""
     shape = x.shape
     if dim == 1 and len(shape) == 2 and x.is_contiguous():            # the usual rows, for the sake of a short call
         return x, shape[0], shape[1], 1, shape[1], False
     C, outer, inner = shape[dim], math.prod(shape[:dim]), math.prod(shape[dim + 1:])
-    moved = inner > 1 and C > (most if outer * inner >= PLANE_POSITIONS else PLANE_FEW)
+    moved = not (keep or _in_place(C, outer, inner, x.element_size(), selected))
     if moved:
         x, outer, inner = x.movedim(dim, -1), outer * inner, 1
     if x.is_contiguous():
@@ -82,7 +96,7 @@ def top_logits(logits, k, dim=1, temperature=1.0):
     if not z.is_cuda or z.numel() == 0:
         return _host_top(z.detach(), k, dim, temperature)            # detached from a forward-mode derivative as well
     before, behind = z.shape[:dim], z.shape[dim + 1:]
-    z, outer, C, inner, ld, moved = _canonical(z.float() if z.dtype == torch.float16 else z, dim, PLANE_CLASSES if k <= PLANE_TOP else PLANE_FEW)
+    z, outer, C, inner, ld, moved = _canonical(z.float() if z.dtype == torch.float16 else z, dim, k)
     device, rest = z.device, before + behind
     kept = rest + (k,) if moved else before + (k,) + behind
     values = torch.empty(kept, dtype=z.dtype, device=device)
@@ -161,7 +175,7 @@ class _DistillFn(torch.autograd.Function):
         else:
             dz = dz.data             # what the caller does to its gradient is no change to a saved tensor: that one is not read again
         if z.data_ptr() != args[0] or z.stride() != ctx.stride:   # hooks on saved tensors brought back a copy, maybe in another layout
-            z, _, _, _, ld, _ = _canonical(z.reshape(outer, C, inner), 1, C)
+            z, _, _, _, ld, _ = _canonical(z.reshape(outer, C, inner), 1, keep=True)
             meta = (outer, C, inner, ld) + meta[4:]
             values, indices, lse = (t if t is None else t.contiguous() for t in (values, indices, lse))
             args = None

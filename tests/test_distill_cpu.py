@@ -220,3 +220,17 @@ def nan_among_the_values(device):
 
 def test_nan_among_the_values():
     nan_among_the_values("cpu")
+
+
+def test_which_planes_are_read_in_place():
+    """Every side of the rule, at sizes on which it was measured; whatever it says, the kernels' own limits hold."""
+    from segk.distill import _in_place
+    yes = [(32, 1, 2, 4, 8), (32, 5, 4, 2, 32), (33, 1, 16384, 4, 8), (80, 1, 16384, 4, 2), (80, 16, 1024, 2, 0), (150, 1, 16384, 4, 1), (256, 1, 36864, 4, 0), (256, 1, 65536, 2, 8),
+           (150, 1, 36864, 4, 8), (80, 4096, 16, 4, 0), (300, 9, 1, 4, 64)]
+    no = [(33, 1, 16383, 4, 1), (80, 1, 65536, 4, 9), (257, 1, 1 << 20, 4, 1), (150, 1, 16384, 4, 8), (256, 1, 16384, 4, 0), (256, 1, 36864, 2, 0), (80, 16384, 4, 4, 0)]
+    assert all(_in_place(*c) for c in yes) and not any(_in_place(*c) for c in no)
+    for C in (2, 32, 33, 256, 257, 5000):
+        for outer in (1, 1000, 1 << 20):
+            for inner in (2, 16, 1 << 10):
+                for selected in (0, 1, 8, 9, 64):
+                    assert not _in_place(C, outer, inner, 4, selected) or C <= (256 if selected <= 8 else 32)

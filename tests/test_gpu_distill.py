@@ -865,3 +865,27 @@ def test_top_of_rows_by_a_wave_or_a_workgroup(P, V, dtype):
                 order = torch.sort(form.float(), dim=1, descending=True, stable=True).indices[:, :41]
                 values = form.gather(1, order)
             assert torch.equal(got.indices.cpu().long(), order[:, :k]) and torch.equal(got.values.cpu(), values[:, :k])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N,C,side,k", [(1, 150, 128, 8), (1, 150, 128, 2), (1, 256, 128, 3), (4500, 40, 2, 3), (1100, 40, 4, 3)])
+def test_planes_in_place_and_copied(N, C, side, k, dtype, monkeypatch):
+    """Sizes on both sides of the rule give what the definition says, whichever way they are read."""
+    g = torch.Generator().manual_seed(C)
+    t, z = (2 * torch.randn(N, C, side, side, generator=g) for _ in range(2))
+    t, z = t.to(dtype), z.to(dtype)
+    order = torch.sort(t.float(), dim=1, descending=True, stable=True).indices[:, :k]
+    rows = lambda x: x.cpu().movedim(1, -1).reshape(N * side * side, -1)                     # noqa: E731
+    some = torch.randint(0, N * side * side, (20,), generator=g)
+    for positions in (0, None, 1 << 30):
+        if positions is not None:
+            monkeypatch.setattr("segk.distill.PLANE_POSITIONS", positions)
+        got = top_logits(t.cuda(), k, temperature=2.0)
+        assert torch.equal(got.indices.cpu().long(), order) and torch.equal(got.values.cpu(), t.gather(1, order))
+        x = z.cuda().requires_grad_()
+        each = distill_loss_topk(x, got, temperature=2.0, reduction="none")
+        grad, = torch.autograd.grad(each.sum(), x)
+        loss, want, _, lerr, gerr = loss_and_gradient(rows(z)[some], rows(got.values)[some], rows(got.indices)[some], got.lse.cpu().reshape(-1)[some], 2.0)
+        assert bool(((each.detach().cpu().reshape(-1)[some].double() - loss).abs() <= lerr + 2.0 ** -23 * loss).all())
+        assert bool(((rows(grad)[some].double() - want).abs() <= gerr + (half_step(dtype) + 2.0 ** -21) * want.abs()).all())
+        monkeypatch.undo()
