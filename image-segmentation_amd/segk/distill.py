@@ -249,6 +249,8 @@ def distill_loss_topk(pred, target, temperature=1.0, reduction="mean", dim=1, we
         lse = lse.float()
     if ops.has_tangent(pred):
         raise NotImplementedError("distill_loss_topk has no forward-mode derivative on the GPU")
+    if isinstance(weight, torch.Tensor) and (weight.requires_grad or ops.has_tangent(weight)):
+        raise ValueError("weight is a number on the GPU, and gets no derivative: multiply the loss by it, or detach it")
     if not want_grad:                                        # no node to be made (3 us)
         return _DistillFn.forward(None, pred, values, indices, lse, dim, temperature, weight, reduction, False)
     return _DistillFn.apply(pred, values, indices, lse, dim, temperature, weight, reduction, True)

@@ -889,3 +889,25 @@ def test_planes_in_place_and_copied(N, C, side, k, dtype, monkeypatch):
         assert bool(((each.detach().cpu().reshape(-1)[some].double() - loss).abs() <= lerr + 2.0 ** -23 * loss).all())
         assert bool(((rows(grad)[some].double() - want).abs() <= gerr + (half_step(dtype) + 2.0 ** -21) * want.abs()).all())
         monkeypatch.undo()
+
+
+def test_a_weight_that_wants_a_derivative_is_refused():
+    x = torch.randn(6, 40, device="cuda", requires_grad=True)
+    target = top_logits(x, 2)
+    for grad in (True, False):
+        for weight in (torch.tensor(2.0, requires_grad=True), torch.tensor(2.0, device="cuda", requires_grad=True)):
+            with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="weight"):
+                distill_loss_topk(x, target, weight=weight)
+            assert torch.equal(distill_loss_topk(x, target, weight=weight.detach()), distill_loss_topk(x, target, weight=2.0))
+
+
+def test_empty_batches():
+    for shape in ((0, 9), (0, 4, 3, 3), (2, 4, 0, 3)):
+        x = torch.zeros(shape, device="cuda", requires_grad=True)
+        target = top_logits(x, 2)
+        assert target.values.shape == shape[:1] + (2,) + shape[2:] and target.lse.shape == shape[:1] + shape[2:] and target.lse.is_cuda
+        for reduction in ("mean", "sum", "none"):
+            for t in (target, target._replace(lse=None)):
+                loss = distill_loss_topk(x, t, reduction=reduction)
+                loss.sum().backward()
+                assert float(loss.detach().sum()) == 0 and x.grad.shape == shape and loss.dtype == F32 and loss.is_cuda
