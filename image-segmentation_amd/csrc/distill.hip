@@ -428,7 +428,7 @@ __device__ __forceinline__ float outside_factor(const Joined& w, float so, float
 
 // One workgroup per row; with NCH > 0 the row stays in registers (NCH pieces per thread), with NCH == 0 it is read twice.
 // In registers the forward pass and the gradient cost one read and one write of the logits, and memory bounds it: 4096 rows of 32000
-// bf16 logits, 32 kept: 524 MB in 101 us, 5.2 TB/s (a copy of that size: 5.4).  The first wave handles the kept entries, one for
+// bf16 logits, 32 kept, a tenth of the rows without: 509 MB in 98 us, 5.2 TB/s (a copy of that size: 5.4).  The first wave handles the kept entries, one for
 // each lane, while the others wait for their pieces; their classes are taken out of the registers, so the two groups of classes have
 // separate maxima without a second pass.
 template <typename T, int NT, int NCH, bool GRAD>
@@ -749,8 +749,9 @@ __global__ __launch_bounds__(256) void distill_share_grad_kernel(const DistillAr
 // ------------------------------------------------------------------------------------------------ one thread per position
 // Few classes (up to 32), all of them in the registers of one thread, VP neighbouring positions per thread: the class planes of
 // [N, C, ...] logits are read with coalesced 16-byte loads (VP = 4), class-last rows with strided ones (VP = 1).
-// Memory bounds it: 32 x 4 x 384 x 384 fp32 logits with 2 kept entries, loss and gradient: 245 MB in 52 us, 4.7 TB/s (a copy: 5.4).
-// With scalar loads of the kept entries all kernels of that call took 168 us instead of 97.
+// Memory bounds it: 32 x 4 x 384 x 384 fp32 logits with 2 kept entries, loss and gradient: 246 MB in 53 us, 4.6 TB/s (a copy: 5.4).
+// With scalar loads of the kept entries all kernels of that call took 168 us instead of 97.  The loss class by class, not entry by entry
+// with their logits looked up again: 65 against 94 us of kernels.
 template <typename T, int CM, int VP, bool GRAD>
 __global__ __launch_bounds__(256) void distill_pixels_kernel(const DistillArgs a, int blocks_each) {
     if (a.skip_if_one && a.upstream[0] == 1.f) return;

@@ -19,7 +19,7 @@ class TopLogits(NamedTuple):
     """What is kept of a teacher's logits: the k greatest of each position in descending order, their classes (int32; -1 or any
     other value that is no class marks an entry that does not exist), and the logsumexp of all classes at the temperature the
     loss will use (None: the kept logits are renormalised).  `values` and `indices` have the logits' shape with k in place of the
-    class dimension, `lse` the shape without it.  Batches like any named tuple in a DataLoader."""
+    class dimension, `lse` the shape without it.  Batches like any named tuple in a DataLoader (whose default collation takes no None: without lse, store (values, indices))."""
     values: torch.Tensor
     indices: torch.Tensor
     lse: Optional[torch.Tensor] = None
@@ -211,8 +211,8 @@ def distill_loss_topk(pred, target, temperature=1.0, reduction="mean", dim=1, we
     `weight` scales loss and gradient; it costs nothing, where multiplying the returned loss costs another pass over the logits.
 
     pred: float32, bfloat16 or float16, any strides; target: TopLogits or a tuple (values, indices[, lse]) with float32 / bfloat16 /
-    float16 values and int32 / int64 indices.  Differentiable once, backwards (on the CPU in any mode).  Returns float32; the gradient has pred's type.  Sums run in float32 (in float64 on the
-    CPU).  log p carries the rounding of the kept lse, 2^-24 |lse|, so logits / T of some thousands leave no exact probabilities.
+    float16 values and int32 / int64 indices.  Differentiable once, backwards (on the CPU in any mode).  Returns float32; the gradient has
+    pred's type.  Sums run in float32 (in float64 on the CPU).  log p carries the rounding of the kept lse, 2^-24 |lse|, so logits / T of some thousands leave no exact probabilities.
     Student and teacher differ by d / T in log q where their logits differ by d, and that is known to about 2^-22: loss and
     gradient are good to about T 2^-22 / d of themselves.  Where every class is kept with an lse, the rounding of the lse adds up to
     T^2 2^-22 (1 + |lse|): leave the lse away there."""

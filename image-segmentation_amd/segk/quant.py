@@ -1,6 +1,6 @@
 """Microscaled 4-bit floating point: packing, unpacking and the linear layer on packed operands, over the C ABI (segk_mxfp4_*), for
-serving networks whose linear layers (nn.Linear: models/densenet3d.py, models/resnt.py; 1x1 convolutions over channels-last
-pixels) hold their trained weights in 4 bits.  CPU tensors are served by the same definitions in torch ops (`_host_*`)."""
+serving linear layers (nn.Linear, 1x1 convolutions over channels-last pixels) whose trained weights are held in 4 bits.  Functions for a
+caller's own layers: the networks of models/ run theirs in fp32.  CPU tensors are served by the same definitions in torch ops (`_host_*`)."""
 import math
 
 import torch

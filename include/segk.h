@@ -115,7 +115,8 @@ int segk_argmax_dice(const void* logits, int logits_dtype, const int64_t* labels
 /* The k greatest logits of every position in descending order (NaN counts as greatest; ties: the lower class first), the classes
  * they belong to (int32) and, if lse is not NULL, the logsumexp of all classes (NaN where a logit is NaN or +inf).  values have the dtype of
  * logits.
- * Outputs 16-byte aligned.  One pass over the logits. */
+ * Outputs 16-byte aligned.  One pass over the logits while a row has up to 16384 pieces of 16 bytes; of longer ones, and where equal logits or a NaN
+ * make an exact search necessary, parts are read again. */
 int segk_top_logits(const void* logits, int dtype, int64_t outer, int64_t C, int64_t inner, int64_t ld, int64_t k, float temperature,
                     void* values, int32_t* indices, float* lse, int dev, void* stream);
 
